@@ -113,6 +113,13 @@ size_t dt_size(int dt) { return dt == DT_F32 ? 4 : 2; }
 
 }  // namespace
 
+int current_launch(TcLaunch* out) {
+  DeviceInfo* d = nullptr;
+  const int rc = device_info(&d);
+  if (rc == FPV2_OK) *out = tc_launch(*d);
+  return rc;
+}
+
 // Record `msg` as the calling thread's last error and return `code` (for entry
 // points defined in other translation units).
 int report_error(int code, const char* msg) {

@@ -177,6 +177,69 @@ bool encode_attn_maps(const AttnArgs& a, CUtensorMap (&m)[6]);
 bool attn_wide_supported(const AttnArgs& a);
 cudaError_t launch_attn_wide(const AttnArgs& a, const TcLaunch& L, int* sched, cudaStream_t stream);
 
+// ---- decode step -------------------------------------------------------------
+// qk_rope.cu: RMS norm + rotary embedding of q and k heads, K/V into cache pages.
+// Strides are in elements; `st`/`sh` are the token and head strides, `sp`/`sr`
+// a cache's page and row strides. k_cache null: k goes to k_out and v is unused.
+struct RopeArgs {
+  const void *q, *k, *v;
+  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;
+  const void* positions;      // int32 or int64 [tokens]
+  const float* table;         // [max_pos, rot]: cosines, then sines
+  const void *q_weight, *k_weight;   // nullable [D]
+  void* q_out;
+  int64_t qo_st, qo_sh;
+  void* k_out;
+  int64_t ko_st, ko_sh;
+  void *k_cache, *v_cache;    // [pages, page_size, Hkv, D]
+  int64_t kc_sp, kc_sr, kc_sh, vc_sp, vc_sr, vc_sh;
+  const int64_t* slots;       // [tokens]: page * page_size + row; out of range: not written
+  int64_t tokens, max_pos, num_slots;
+  int Hq, Hkv, D, rot, interleaved, pos64, weight_dt, page_size;
+  float eps;
+};
+cudaError_t launch_qk_rope(const RopeArgs& a, int dt, int num_sms, cudaStream_t stream);
+
+// decode.cu: attention of the newest tokens of each sequence over paged K/V.
+struct DecodeArgs {
+  const void *q, *k, *v;      // q [B, T, Hq, D]; k, v page pools [pages, page_size, Hkv, D]
+  int64_t q_sb, q_st, q_sh, k_sp, k_sr, k_sh, v_sp, v_sr, v_sh;
+  const int32_t* tables;      // [B, table_width], row stride table_stride
+  const int32_t* lengths;     // [B], the new tokens included
+  int64_t table_stride;
+  int B, T, Hq, Hkv, G, D, num_pages, page_size, table_width;
+  int window, sinks;          // window 0: every key up to the query is seen
+  float scale_log2;
+  void* out;                  // [B, T, Hq, D]
+  float* lse;                 // nullable [B, T, Hq]
+  void* workspace;
+  int* status;
+};
+bool decode_supported(int D);
+size_t decode_workspace_bytes(int T, int Hq, int Hkv, int D);
+cudaError_t launch_decode(const DecodeArgs& a, int dt, cudaStream_t stream);
+
+// sample.cu: next tokens from logits and given exponential noise.
+struct SampleArgs {
+  const void* logits;         // [rows, vocab], row stride logits_stride
+  const float* noise;         // [rows, vocab], row stride noise_stride
+  int64_t logits_stride, noise_stride;
+  const float* temperature;   // nullable [rows], else the scalar below
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  float temperature_s, top_p_s, min_p_s;
+  int top_k_s;
+  int rows, vocab;
+  int64_t* tokens;            // [rows]
+  float* logprobs;            // nullable [rows]
+};
+cudaError_t launch_sample(const SampleArgs& a, int dt, int num_sms, cudaStream_t stream);
+
+// The current device's launch record, or an FPV2_ERR_* code (capi.cu).
+int current_launch(TcLaunch* out);
+int report_error(int code, const char* msg);
+
 // selftest.cu: bounded-wait failure detection.
 cudaError_t launch_wait_selftest(const TcLaunch& L, cudaStream_t stream);
 

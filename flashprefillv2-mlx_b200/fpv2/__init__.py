@@ -5,6 +5,7 @@ on PyTorch CUDA tensors; the compute runs in the hand-written CUDA kernels of
 ``libfpv2_b200.so`` (see include/fpv2_b200.h).
 """
 
+from fpv2.decode import decode_attention, qk_norm_rope, rope_table, sample_tokens
 from fpv2.kernel import (
     SUPPORTED_HEAD_DIMS,
     TileConfig,
@@ -25,6 +26,7 @@ __all__ = [
     "block_scores_and_select",
     "block_sparsity",
     "compact_block_indices",
+    "decode_attention",
     "default_tile",
     "density",
     "disable",
@@ -34,6 +36,9 @@ __all__ = [
     "is_enabled",
     "pool_blocks",
     "pool_pages",
+    "qk_norm_rope",
+    "rope_table",
+    "sample_tokens",
     "sdpa_from_host",
     "sparse_attention",
     "sparse_attention_paged",

@@ -1,0 +1,307 @@
+"""The decode step next to the sparse prefill (no reference counterpart: the
+reference leaves it to its model library).
+
+``qk_norm_rope`` norms and rotates the query and key heads and writes K and V into
+the page pools that ``pool_pages`` / ``sparse_attention_paged`` prefill from and
+``decode_attention`` reads; ``decode_attention`` attends the newest tokens of every
+sequence over them; ``sample_tokens`` picks the next tokens. The kernels have no
+backward: inputs that require grad are refused while grad mode is on.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from fpv2 import _lib
+
+DECODE_HEAD_DIMS = (64, 96, 128, 256)
+_HALF = (torch.float16, torch.bfloat16)
+_INT32_MAX = 2**31 - 1
+
+
+def _no_grad(what: str, *tensors: torch.Tensor | None) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError(f"{what} has no backward; call it under torch.no_grad()")
+
+
+def _call(name: str, on: torch.Tensor, *args) -> None:
+    """One library call on ``on``'s device and its current stream."""
+    fn = getattr(_lib.lib(), name)
+    if on.device.index == torch.cuda.current_device():
+        _lib.check(fn(*args, _lib.stream_of(on)))
+    else:
+        with torch.cuda.device(on.device):
+            _lib.check(fn(*args, _lib.stream_of(on)))
+
+
+def _strides(*values: int):
+    return (ctypes.c_int64 * len(values))(*values)
+
+
+def rope_table(positions: int, rotary_dim: int, *, theta: float = 10000.0,
+               device: torch.device | str | None = None) -> torch.Tensor:
+    """Rotation table ``[positions, rotary_dim]`` for ``qk_norm_rope``: the cosines of
+    ``p * theta ** (-2 i / rotary_dim)``, then their sines, computed in float64 and
+    rounded to float32."""
+    if positions <= 0 or rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError("positions must be positive and rotary_dim even and positive")
+    half = rotary_dim // 2
+    freq = theta ** (-torch.arange(half, dtype=torch.float64, device=device) / half)
+    angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * freq
+    return torch.cat([angle.cos(), angle.sin()], -1).float()
+
+
+def qk_norm_rope(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    positions: torch.Tensor,
+    table: torch.Tensor,
+    *,
+    q_weight: torch.Tensor | None = None,
+    k_weight: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    interleaved: bool = False,
+    heads_first: bool = False,
+    v: torch.Tensor | None = None,
+    k_cache: torch.Tensor | None = None,
+    v_cache: torch.Tensor | None = None,
+    slots: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """RMS norm of every query and key head, then rotary embedding, in one pass.
+
+    ``q`` is ``[tokens, q_heads, dim]`` and ``k`` ``[tokens, kv_heads, dim]`` (any token
+    and head strides, so views of one fused projection do). Each head is divided by
+    ``sqrt(mean(x^2) + eps)``, multiplied by ``q_weight`` / ``k_weight`` ``[dim]`` where
+    given, and its first ``table.shape[1]`` dimensions are rotated by the row of
+    ``table`` (see ``rope_table``) of the token's position (int32 or int64, clamped
+    into the table): pairs ``(i, i + rotary / 2)``, or ``(2i, 2i + 1)`` with
+    ``interleaved``. Float32 arithmetic, rounded once.
+
+    Returns ``(q, k)`` as ``[tokens, heads, dim]``, or ``[heads, tokens, dim]`` (the
+    prefill operators' layout) with ``heads_first``. With ``v``, ``k_cache``, ``v_cache``
+    (page pools ``[pages, page_size, kv_heads, dim]``, any strides) and ``slots`` (int64
+    ``[tokens]``, ``page * page_size + row``; negative or past the pool: the token is
+    not written) k and v go into the cache and the returned k is None. Slots must
+    not repeat.
+    """
+    if q.ndim != 3 or k.ndim != 3:
+        raise ValueError("q and k must have shape [tokens, heads, dim]")
+    tokens, q_heads, dim = q.shape
+    kv_heads = k.shape[1]
+    if k.shape[0] != tokens or k.shape[2] != dim:
+        raise ValueError("q and k must have the same tokens and head dimension")
+    if not q_heads or not kv_heads:
+        raise ValueError("q and k must have heads")
+    if not 0 < dim <= 256:
+        raise ValueError("head dimension must be in [1, 256]")
+    dtype = q.dtype
+    code = _lib.dtype_code(dtype)
+    if k.dtype != dtype:
+        raise ValueError("q and k must share their dtype")
+    if positions.ndim != 1 or positions.shape[0] != tokens or positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError("positions must be an int32 or int64 tensor [tokens]")
+    if table.ndim != 2 or table.dtype != torch.float32 or not table.shape[0]:
+        raise ValueError("table must be a float32 tensor [positions, rotary_dim]")
+    rotary = table.shape[1]
+    if not rotary or rotary % 2 or rotary > dim:
+        raise ValueError("rotary_dim must be even and in [2, head_dim]")
+    weight_code = code
+    weights = [w for w in (q_weight, k_weight) if w is not None]
+    for w in weights:
+        if w.ndim != 1 or w.shape[0] != dim or w.dtype != weights[0].dtype:
+            raise ValueError("norm weights must share one dtype and have shape [head_dim]")
+        weight_code = _lib.dtype_code(w.dtype)
+    cache = (v, k_cache, v_cache, slots)
+    paged = k_cache is not None
+    if any((x is not None) != paged for x in cache):
+        raise ValueError("v, k_cache, v_cache and slots go together")
+    if paged:
+        if v.shape != k.shape or v.dtype != dtype:
+            raise ValueError("v must have the shape and dtype of k")
+        for c in (k_cache, v_cache):
+            if c.ndim != 4 or c.shape[2] != kv_heads or c.shape[3] != dim or c.dtype != dtype:
+                raise ValueError("caches must have shape [pages, page_size, kv_heads, dim] and k's dtype")
+            if c.stride(3) != 1 and dim > 1:
+                raise ValueError("a cache's head dimension must be contiguous")
+        if k_cache.shape != v_cache.shape or not k_cache.shape[0] or not k_cache.shape[1]:
+            raise ValueError("k_cache and v_cache must have identical non-empty shapes")
+        if slots.ndim != 1 or slots.shape[0] != tokens or slots.dtype != torch.int64:
+            raise ValueError("slots must be an int64 tensor [tokens]")
+    _no_grad("qk_norm_rope", q, k, table, q_weight, k_weight, *cache)
+    _lib.require_cuda(q, k, positions, table, q_weight, k_weight, *cache)
+    q, k = _rows(q), _rows(k)
+    positions, table = positions.contiguous(), table.contiguous()
+    if q_weight is not None:
+        q_weight = q_weight.contiguous()
+    if k_weight is not None:
+        k_weight = k_weight.contiguous()
+    k_out = None
+    if heads_first:
+        q_out = torch.empty((q_heads, tokens, dim), dtype=dtype, device=q.device)
+        out = [dim, tokens * dim, dim, tokens * dim]
+    else:
+        q_out = torch.empty((tokens, q_heads, dim), dtype=dtype, device=q.device)
+        out = [q_heads * dim, dim, kv_heads * dim, dim]
+    inn = [q.stride(0), q.stride(1), k.stride(0), k.stride(1), 0, 0]
+    cache_strides, pages, page_size = None, 0, 0
+    if paged:
+        v, slots = _rows(v), slots.contiguous()
+        inn[4:] = v.stride(0), v.stride(1)
+        pages, page_size = k_cache.shape[:2]
+        cache_strides = _strides(*k_cache.stride()[:3], *v_cache.stride()[:3])
+    else:
+        k_out = torch.empty((kv_heads, tokens, dim) if heads_first else (tokens, kv_heads, dim),
+                            dtype=dtype, device=q.device)
+    _call("fpv2_qk_norm_rope", q, q.data_ptr(), k.data_ptr(), _lib.ptr(v), code, tokens, q_heads, kv_heads,
+          dim, _strides(*inn), positions.data_ptr(), positions.dtype == torch.int64, table.data_ptr(),
+          table.shape[0], rotary, bool(interleaved), _lib.ptr(q_weight), _lib.ptr(k_weight), weight_code,
+          float(eps), q_out.data_ptr(), _lib.ptr(k_out), _strides(*out), _lib.ptr(k_cache),
+          _lib.ptr(v_cache), cache_strides, _lib.ptr(slots), pages, page_size)
+    return q_out, k_out
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """``x`` with a contiguous last dimension (a copy only where it is not)."""
+    return x if x.stride(-1) == 1 else x.contiguous()
+
+
+def decode_attention(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    block_tables: torch.Tensor,
+    lengths: torch.Tensor,
+    *,
+    scale: float,
+    window: int = 0,
+    sinks: int = 0,
+    return_lse: bool = False,
+) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+    """Attention of the newest token (or the newest few) of each sequence over its paged K/V.
+
+    ``q`` is ``[batch, heads, dim]``, or ``[batch, new, heads, dim]`` for several new
+    tokens (drafts to verify); ``k_cache`` and ``v_cache`` are page pools ``[pages,
+    page_size, kv_heads, dim]`` with any page, row and head strides (multiples of 8
+    elements); ``block_tables`` int32 ``[batch, max_pages]`` holds each sequence's
+    pages and ``lengths`` int32 ``[batch]`` its keys, the new tokens' included.
+    Query ``t`` sits at position ``p = length - new + t`` and sees the keys ``j <= p``
+    with ``j < sinks`` or ``j > p - window``; ``window=0`` sees all of them. A query
+    without a visible key gets zeros. float16 / bfloat16, head_dim 64, 96, 128 or
+    256, any page size. Returns the output in ``q``'s shape, and with ``return_lse``
+    the float32 log-sum-exp of the scaled scores (without the last dimension).
+    """
+    if q.ndim not in (3, 4):
+        raise ValueError("q must have shape [batch, heads, dim] or [batch, new, heads, dim]")
+    shape = q.shape
+    q4 = q if q.ndim == 4 else q.unsqueeze(1)
+    batch, new, q_heads, dim = q4.shape
+    kshape = k_cache.shape
+    if len(kshape) != 4:
+        raise ValueError("k_cache must have shape [pages, page_size, kv_heads, dim]")
+    dtype = q.dtype
+    if dtype not in _HALF or k_cache.dtype != dtype or v_cache.dtype != dtype:
+        raise ValueError("q and the caches must share float16 or bfloat16 dtype")
+    if v_cache.shape != kshape:
+        raise ValueError("k_cache and v_cache must have identical shapes")
+    pages, page_size, kv_heads, kdim = kshape
+    if dim != kdim or dim not in DECODE_HEAD_DIMS:
+        raise ValueError(f"head dimension must be one of {DECODE_HEAD_DIMS}")
+    if not kv_heads or not q_heads or q_heads % kv_heads:
+        raise ValueError("query heads must be divisible by KV heads")
+    if not new:
+        raise ValueError("q must hold at least one new token a sequence")
+    if not pages or not page_size:
+        raise ValueError("the caches are empty")
+    if block_tables.ndim != 2 or block_tables.dtype != torch.int32 or block_tables.shape[0] != batch:
+        raise ValueError("block_tables must be an int32 tensor [batch, max_pages]")
+    if lengths.ndim != 1 or lengths.dtype != torch.int32 or lengths.shape[0] != batch:
+        raise ValueError("lengths must be an int32 tensor [batch]")
+    width = block_tables.shape[1]
+    if not width:
+        raise ValueError("block_tables holds no pages")
+    if not (0 <= window <= _INT32_MAX and 0 <= sinks <= _INT32_MAX):
+        raise ValueError("window and sinks must be non-negative 32-bit integers")
+    _no_grad("decode_attention", q, k_cache, v_cache)
+    _lib.require_cuda(q, k_cache, v_cache, block_tables, lengths)
+    out = torch.empty((batch, new, q_heads, dim), dtype=dtype, device=q.device)
+    lse = torch.empty((batch, new, q_heads), dtype=torch.float32, device=q.device) if return_lse else None
+    if batch:
+        qs, ks, vs = q4.stride(), k_cache.stride(), v_cache.stride()
+        if qs[3] != 1 or (qs[0] | qs[1] | qs[2]) & 1 or q4.data_ptr() & 3:
+            q4 = q4.clone(memory_format=torch.contiguous_format)
+            qs = q4.stride()
+        if ks[3] != 1 or vs[3] != 1:
+            raise ValueError("a cache's head dimension must be contiguous")
+        if block_tables.stride(1) != 1:
+            block_tables = block_tables.contiguous()
+        lengths = lengths.contiguous()
+        nbytes = _lib.lib().fpv2_decode_workspace_bytes(new, q_heads, kv_heads, dim)
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        _call("fpv2_decode_attention", q4, q4.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+              _lib.dtype_code(dtype), batch, new, q_heads, kv_heads, dim,
+              _strides(*qs[:3], *ks[:3], *vs[:3]), block_tables.data_ptr(), block_tables.stride(0), width,
+              lengths.data_ptr(), pages, page_size, float(scale), window, sinks, out.data_ptr(), _lib.ptr(lse),
+              workspace.data_ptr(), nbytes)
+    out = out.view(shape)
+    return (out, lse.view(shape[:-1])) if return_lse else out
+
+
+def _setting(value, name: str, dtype: torch.dtype, rows: int, plain: float):
+    """(tensor, scalar) of a per-row or common setting."""
+    if isinstance(value, torch.Tensor):
+        if value.ndim != 1 or value.shape[0] != rows or value.dtype != dtype:
+            raise ValueError(f"{name} must be a number or a {dtype} tensor [rows]")
+        return value.contiguous(), plain
+    return None, value
+
+
+def sample_tokens(
+    logits: torch.Tensor,
+    noise: torch.Tensor,
+    *,
+    temperature: float | torch.Tensor = 1.0,
+    top_k: int | torch.Tensor = 0,
+    top_p: float | torch.Tensor = 1.0,
+    min_p: float | torch.Tensor = 0.0,
+    return_logprobs: bool = False,
+) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+    """The next token of each row of ``logits`` ``[rows, vocab]`` from given random numbers.
+
+    ``noise`` is float32 ``[rows, vocab]`` of positive, exponentially distributed
+    numbers (``torch.empty(...).exponential_()``). Each setting is one number or a
+    tensor ``[rows]`` (float32; int32 for ``top_k``). With ``z = (x - max) / T`` and
+    ``w = exp(z)``, tokens in the order of (x descending, index ascending) pass
+    ``top_k`` (the first k; 0 or less: all), then ``top_p`` (the shortest prefix of
+    those whose weight reaches ``top_p`` of theirs; 1 or more: all), then ``min_p``
+    (``w >= min_p``); the first token always stays. The result, int64 ``[rows]``, is the
+    argmax of ``z - log(noise)`` over what is left: a draw with probabilities
+    proportional to ``w``. ``T <= 0`` takes the lowest index of the maximum. NaN logits
+    count as -inf; a row without a logit above -inf gives -1. With
+    ``return_logprobs`` also float32 ``[rows]``: the token's log-probability under
+    ``softmax(x / T)`` over the whole row (``T = 1`` where ``T <= 0``).
+    """
+    if logits.ndim != 2 or noise.ndim != 2 or logits.shape != noise.shape:
+        raise ValueError("logits and noise must have the same shape [rows, vocab]")
+    rows, vocab = logits.shape
+    if not vocab:
+        raise ValueError("logits must have a vocabulary")
+    code = _lib.dtype_code(logits.dtype)
+    if noise.dtype != torch.float32:
+        raise ValueError("noise must have float32 dtype")
+    heat, heat_all = _setting(temperature, "temperature", torch.float32, rows, 1.0)
+    k, k_all = _setting(top_k, "top_k", torch.int32, rows, 0)
+    p, p_all = _setting(top_p, "top_p", torch.float32, rows, 1.0)
+    least, least_all = _setting(min_p, "min_p", torch.float32, rows, 0.0)
+    if not -_INT32_MAX <= k_all <= _INT32_MAX:
+        raise ValueError("top_k must be a 32-bit integer")
+    _no_grad("sample_tokens", logits)
+    _lib.require_cuda(logits, noise, heat, k, p, least)
+    logits, noise = _rows(logits), _rows(noise)
+    tokens = torch.empty(rows, dtype=torch.int64, device=logits.device)
+    logprobs = torch.empty(rows, dtype=torch.float32, device=logits.device) if return_logprobs else None
+    _call("fpv2_sample_tokens", logits, logits.data_ptr(), code, rows, vocab, logits.stride(0),
+          noise.data_ptr(), noise.stride(0), _lib.ptr(heat), float(heat_all), _lib.ptr(k), int(k_all),
+          _lib.ptr(p), float(p_all), _lib.ptr(least), float(least_all), tokens.data_ptr(), _lib.ptr(logprobs))
+    return (tokens, logprobs) if return_logprobs else tokens
