@@ -164,6 +164,9 @@ int fpv2_decode_attention(const void* q, const void* k_pages, const void* v_page
   a.D = head_dim;
   a.num_pages = num_pages;
   a.page_size = page_size;
+  a.page_shift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (page_size == 1 << i) a.page_shift = i;
   a.table_width = table_width;
   a.window = window;
   a.sinks = sinks;

@@ -8,12 +8,12 @@
 //
 // Every visible K and V row is read once for 4 G T D operations on 4 D bytes, so
 // DRAM bandwidth bounds the call until G * T passes about 100 query rows; the
-// tensor work is small and shaped 16 rows high, so it runs on mma.sync m16n8k16
-// straight from shared memory, without TMEM round trips.
+// tensor work is small and a few rows wide, so it runs on mma.sync m16n8k16 straight
+// from shared memory, without TMEM round trips.
 //
 // Split: the visible keys of all sequences are one stream of TK-key tiles, cut
 // into equal parts whatever the sequences' lengths are. One warp takes one part
-// for one KV head (and one block of 16 query rows), with its own cp.async ring
+// for one KV head (and up to 32 of its query rows), with its own cp.async ring
 // and running softmax, so warps never wait for each other; neighbouring warps
 // take neighbouring heads of the same keys, which keeps the page reads of a
 // block of threads contiguous. A sequence that lies inside one part is finished
@@ -40,7 +40,16 @@ template <> struct Shape<256> { static constexpr int TK = 16, ST = 3, NW = 4; };
 template <int D> constexpr int kPitch = D * 2 + 16;
 template <int D> constexpr int kStageBytes = 2 * Shape<D>::TK * kPitch<D>;
 
-__host__ __device__ inline int row_blocks(int G, int T) { return (G * T + 15) / 16; }
+// Blocks of eight query rows a warp takes, and the warps that share a KV head's rows.
+// More blocks reuse a tile in shared memory but need their own accumulators in
+// registers: 16 bytes of head_dim a block and lane, so two blocks at most for 256.
+__host__ __device__ inline int blocks_of(int rows, int D) {
+  return rows <= 8 ? 1 : rows <= 16 || D == 256 ? 2 : 4;
+}
+__host__ __device__ inline int row_groups(int rows, int D) {
+  const int per = 8 * blocks_of(rows, D);
+  return (rows + per - 1) / per;
+}
 
 // The visible tiles of one sequence: tile t holds keys from (t < head ? t : t + jump) * TK.
 struct Seq {
@@ -93,7 +102,10 @@ __device__ __forceinline__ int64_t part_tiles(int64_t total, int parts) {
   return (total + parts - 1) / parts;
 }
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool read) {
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp16_if(uint32_t dst, const void* src, bool read) {
   const int n = read ? 16 : 0;   // 0: the chunk is filled with zeros and nothing is read
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
@@ -115,6 +127,13 @@ __device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
                : "memory");
 }
 
+// 8 x 8 transpose of 16-bit values spread over the warp.
+__device__ __forceinline__ uint32_t turn(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
 // c += a b for a 16 x 16 by 16 x 8 tile.
 template <int DT>
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -132,44 +151,53 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Walks the tiles of a part for the copies: sequence, tile in it, and the table
-// entry of this lane's row, loaded one tile before it is needed.
+// Walks the tiles of a part for the copies: sequence, tile in it, and this lane's
+// row of it: its page (loaded one tile before it is needed) and place in the page.
 template <int TK> struct Feed {
   int b, t;
   Seq s;
-  int entry;
+  int page, in_page;
 
   __device__ __forceinline__ int key0() const { return (t < s.head ? t : t + s.jump) * TK; }
-  __device__ __forceinline__ void fetch(const DecodeArgs& a, int lane) {
-    const int key = min(key0() + lane % TK, s.len - 1);   // past the end: the last key's page
-    entry = a.tables[(int64_t)b * a.table_stride + key / a.page_size];
+  __device__ __forceinline__ void fetch(const DecodeArgs& a, int lane, bool whole) {
+    // every lane of a tile inside one page: its first row; past the end: the last key
+    const int key = min(key0() + (whole ? 0 : lane % TK), s.len - 1);
+    const int at = a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size;
+    in_page = key - at * a.page_size;
+    page = a.tables[(int64_t)b * a.table_stride + at];
   }
-  __device__ __forceinline__ void next(const DecodeArgs& a, int lane, bool more) {
-    if (!more) return;
+  __device__ __forceinline__ void next(const DecodeArgs& a, int lane, bool whole) {
     ++t;
     while (t >= s.tiles) {   // a part that goes on has a sequence with tiles ahead
       ++b;
       t = 0;
       s = seq_of<TK>(a, b);
     }
-    fetch(a, lane);
+    fetch(a, lane, whole);
   }
 };
 
-template <int DT, int D>
+// Scores are taken transposed, S^T = K Q^T with 16 keys by 8 query rows a product, so a
+// GQA group of up to eight rows fills the tile, and O^T = V^T P^T likewise; P^T comes
+// from S^T's registers by an 8 x 8 transpose.
+template <int DT, int D, int NB>
 __global__ void __launch_bounds__(Shape<D>::NW * 32, 1) decode_kernel(const DecodeArgs a, int parts) {
   constexpr int TK = Shape<D>::TK, ST = Shape<D>::ST, NW = Shape<D>::NW;
-  constexpr int PITCH = kPitch<D>, CH = D / 8, KS = D / 16, NT = TK / 8, ON = D / 8;
+  constexpr int PITCH = kPitch<D>, CH = D / 8, KS = D / 16, MT = TK / 16;
+  constexpr int CL = CH <= 8 ? 8 : CH <= 16 ? 16 : 32;   // lanes that copy one row
+  constexpr int RPS = 32 / CL;                           // rows a warp-wide copy covers
+  constexpr float kSlack = 8.f;
   using T = typename Elem<DT>::T;
   extern __shared__ __align__(16) unsigned char smem[];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = lane >> 2, c = lane & 3;   // mma fragment: rows g and g + 8, column pair c
-  const int rbs = row_blocks(a.G, a.T), cols = a.Hkv * rbs;
+  const int g = lane >> 2, c = lane & 3;   // mma fragments: rows g and g + 8, column pair c
+  const int R = a.G * a.T;                 // query rows of a KV head
+  const int groups = row_groups(R, D), cols = a.Hkv * groups;
   const int64_t wi = (int64_t)blockIdx.x * NW + warp;
   const int64_t part = wi / cols;
   const int col = (int)(wi - part * cols);
-  const int h = col / rbs, rb = col - h * rbs;
+  const int h = col / groups, rbase = (col - h * groups) * 8 * NB;
   if (part >= parts) return;
 
   // this warp's range of the tile stream, and the sequence it starts in
@@ -178,7 +206,8 @@ __global__ void __launch_bounds__(Shape<D>::NW * 32, 1) decode_kernel(const Deco
   const int64_t chunk = part_tiles(total, parts);
   const int64_t begin = part * chunk, end = min(begin + chunk, total);
   if (begin >= end) return;
-  int count = (int)(end - begin);
+  const int count = (int)(end - begin);
+  const bool whole = a.page_size % TK == 0;
   Feed<TK> f;
   {
     int64_t run = 0;
@@ -203,254 +232,289 @@ __global__ void __launch_bounds__(Shape<D>::NW * 32, 1) decode_kernel(const Deco
     }
     f.s = seq_of<TK>(a, f.b);
   }
-  f.fetch(a, lane);
+  f.fetch(a, lane, whole);
   int b = f.b, t = f.t, seg0 = f.t;   // the consumer's sequence, tile, and the segment's first tile
   Seq s = f.s;
   bool first = true;
 
-  const uint32_t ring = smem_u32(smem) + warp * ST * kStageBytes<D>;
-  const T* kh = reinterpret_cast<const T*>(a.k) + h * a.k_sh;
-  const T* vh = reinterpret_cast<const T*>(a.v) + h * a.v_sh;
-  const bool whole_pages = a.page_size % TK == 0;
-  int ahead = 0;   // tiles whose copies were issued
+  unsigned char* const ring_ptr = smem + warp * ST * kStageBytes<D>;
+  const uint32_t ring = smem_u32(ring_ptr);
+  const int lrow = lane / CL, lch = lane % CL;           // this lane's row and chunk of a copy
+  const T* kh = reinterpret_cast<const T*>(a.k) + h * a.k_sh + lch * 8;
+  const T* vh = reinterpret_cast<const T*>(a.v) + h * a.v_sh + lch * 8;
+  const uint32_t ldst = lrow * PITCH + lch * 16;
+  int ahead = 0, fill = 0;   // tiles whose copies were issued, and the ring slot of the next
 
   auto issue = [&]() {
     if (ahead < count) {
-      const uint32_t dst = ring + (ahead % ST) * kStageBytes<D>;
+      const uint32_t dst = ring + fill * kStageBytes<D> + ldst;
+      fill = fill + 1 == ST ? 0 : fill + 1;
       const int key0 = f.key0();
-      // element offsets of this lane's row (every lane of a whole page: row 0)
-      const int page = clamp_entry(f.entry, 0, a.num_pages - 1, a.status);
-      const int mine = whole_pages ? key0 : key0 + lane % TK;
-      const int in_page = mine < f.s.len ? mine % a.page_size : 0;
-      const int64_t ko = page * a.k_sp + in_page * a.k_sr, vo = page * a.v_sp + in_page * a.v_sr;
+      const int page = clamp_entry(f.page, 0, a.num_pages - 1, a.status);
+      const int64_t ko = page * a.k_sp + f.in_page * a.k_sr, vo = page * a.v_sp + f.in_page * a.v_sr;
+      const bool all = key0 + TK <= f.s.len && (key0 >= f.s.low || key0 + TK <= a.sinks);
+      if (whole && all) {
+        const T* kp = kh + ko + lrow * a.k_sr;
+        const T* vp = vh + vo + lrow * a.v_sr;
+        if (CL == CH || lch < CH) {
 #pragma unroll
-      for (int i = 0; i < TK * CH / 32; ++i) {
-        const int id = lane + 32 * i, row = id / CH, ch = id % CH;
-        int64_t kr = ko, vr = vo;
-        if (whole_pages) {
-          kr += row * a.k_sr;
-          vr += row * a.v_sr;
-        } else {
-          kr = __shfl_sync(0xffffffffu, ko, row);
-          vr = __shfl_sync(0xffffffffu, vo, row);
+          for (int i = 0; i < TK / RPS; ++i) {
+            cp16(dst + i * RPS * PITCH, kp);
+            kp += RPS * a.k_sr;
+          }
+#pragma unroll
+          for (int i = 0; i < TK / RPS; ++i) {
+            cp16(dst + (TK + i * RPS) * PITCH, vp);
+            vp += RPS * a.v_sr;
+          }
         }
-        const int key = key0 + row;
-        // keys that no row sees are zeros, whatever their page holds
-        const bool seen = key < f.s.len && (key >= f.s.low || key < a.sinks);
-        cp16(dst + row * PITCH + ch * 16, kh + kr + ch * 8, seen);
-        cp16(dst + TK * PITCH + row * PITCH + ch * 16, vh + vr + ch * 8, seen);
+      } else {
+#pragma unroll
+        for (int i = 0; i < TK / RPS; ++i) {
+          const int row = lrow + i * RPS, key = key0 + row;
+          const int64_t kr = whole ? ko + row * a.k_sr : __shfl_sync(0xffffffffu, ko, row);
+          const int64_t vr = whole ? vo + row * a.v_sr : __shfl_sync(0xffffffffu, vo, row);
+          // keys that no row sees are zeros, whatever their page holds
+          const bool seen = key < f.s.len && (key >= f.s.low || key < a.sinks);
+          if (CL == CH || lch < CH) {
+            cp16_if(dst + i * RPS * PITCH, kh + kr, seen);
+            cp16_if(dst + (TK + i * RPS) * PITCH, vh + vr, seen);
+          }
+        }
       }
-      ++ahead;
-      f.next(a, lane, ahead < count);
+      if (++ahead < count) f.next(a, lane, whole);
     }
     cp_commit();
   };
 #pragma unroll
   for (int i = 0; i < ST - 1; ++i) issue();
 
-  const int R = a.G * a.T;                       // query rows of a KV head
-  const int r0 = rb * 16 + g, r1 = r0 + 8;       // this lane's two rows
-  uint32_t qf[KS][4];
-  float o[ON][4];
-  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+  uint32_t qf[NB][KS][2];
+  float o[NB][KS][4];
+  float m[NB][2], e[NB][2], l[NB][2];   // running maximum, the same with -inf as 0, sum: rows 2 c, 2 c + 1
+  int tq[NB][2];                        // their new-token index
+#pragma unroll
+  for (int n = 0; n < NB; ++n)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) tq[n][j] = (rbase + n * 8 + c * 2 + j) / a.G;
   auto start_segment = [&]() {
-    const int t0 = r0 / a.G, t1 = r1 / a.G;
-    const T* q0 = reinterpret_cast<const T*>(a.q) + b * a.q_sb + t0 * a.q_st + (int64_t)(h * a.G + r0 - t0 * a.G) * a.q_sh;
-    const T* q1 = reinterpret_cast<const T*>(a.q) + b * a.q_sb + t1 * a.q_st + (int64_t)(h * a.G + r1 - t1 * a.G) * a.q_sh;
 #pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      const int d = k * 16 + c * 2;
-      qf[k][0] = r0 < R ? *reinterpret_cast<const uint32_t*>(q0 + d) : 0u;
-      qf[k][1] = r1 < R ? *reinterpret_cast<const uint32_t*>(q1 + d) : 0u;
-      qf[k][2] = r0 < R ? *reinterpret_cast<const uint32_t*>(q0 + d + 8) : 0u;
-      qf[k][3] = r1 < R ? *reinterpret_cast<const uint32_t*>(q1 + d + 8) : 0u;
+    for (int n = 0; n < NB; ++n) {
+      const int r = rbase + n * 8 + g, rt = r / a.G;
+      const T* q = reinterpret_cast<const T*>(a.q) + b * a.q_sb + rt * a.q_st +
+                   (int64_t)(h * a.G + r - rt * a.G) * a.q_sh + c * 2;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        qf[n][k][0] = r < R ? *reinterpret_cast<const uint32_t*>(q + k * 16) : 0u;
+        qf[n][k][1] = r < R ? *reinterpret_cast<const uint32_t*>(q + k * 16 + 8) : 0u;
+        o[n][k][0] = o[n][k][1] = o[n][k][2] = o[n][k][3] = 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        m[n][j] = -INFINITY;
+        e[n][j] = l[n][j] = 0.f;
+      }
     }
-#pragma unroll
-    for (int n = 0; n < ON; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-    m0 = m1 = -INFINITY;
-    l0 = l1 = 0.f;
   };
   start_segment();
 
+  // lane addresses of the ldmatrix tiles
+  const uint32_t k_at = ((lane & 7) + ((lane >> 3) & 1) * 8) * PITCH + (lane >> 4) * 16;
+  const uint32_t v_at = (TK + (lane & 7) + (lane >> 4) * 8) * PITCH + ((lane >> 3) & 1) * 16;
+  int slot = 0;
   for (int i = 0; i < count; ++i) {
     cp_wait<ST - 2>();
     __syncwarp();
     issue();
-    const uint32_t kt = ring + (i % ST) * kStageBytes<D>, vt = kt + TK * PITCH;
-    float sc[NT][4];
+    const uint32_t tile = ring + slot * kStageBytes<D>;
+    const unsigned char* vtile = ring_ptr + slot * kStageBytes<D> + TK * PITCH;
+    slot = slot + 1 == ST ? 0 : slot + 1;
+    float sc[MT][NB][4];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+    for (int mt = 0; mt < MT; ++mt) {
+      float s2[NB][4];   // odd steps apart: two chains of dependent products
 #pragma unroll
-    for (int k = 0; k < KS; ++k) {
+      for (int n = 0; n < NB; ++n)
 #pragma unroll
-      for (int n = 0; n < NT; n += 2) {
+        for (int j = 0; j < 4; ++j) sc[mt][n][j] = s2[n][j] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
         uint32_t kf[4];
-        ldsm4(kt + (n * 8 + (lane & 7) + (lane >> 4) * 8) * PITCH + (2 * k + ((lane >> 3) & 1)) * 16, kf);
-        mma<DT>(sc[n], qf[k], kf[0], kf[1]);
-        mma<DT>(sc[n + 1], qf[k], kf[2], kf[3]);
+        ldsm4(tile + k_at + mt * 16 * PITCH + k * 32, kf);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) mma<DT>(k & 1 ? s2[n] : sc[mt][n], kf, qf[n][k][0], qf[n][k][1]);
       }
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sc[mt][n][j] = (sc[mt][n][j] + s2[n][j]) * a.scale_log2;
     }
     const int key0 = (t < s.head ? t : t + s.jump) * TK;
     // a tile that every row sees whole needs no mask
     const int p_first = s.len - a.T;
-    const bool open = key0 + TK <= p_first + 1 && (a.window == 0 || key0 + TK <= a.sinks ||
-                                                   key0 > s.len - 1 - a.window);
-    const int p0 = p_first + r0 / a.G, p1 = p_first + r1 / a.G;
-    float x0 = -INFINITY, x1 = -INFINITY;
+    const bool open = key0 + TK <= p_first + 1 &&
+                      (a.window == 0 || key0 + TK <= a.sinks || key0 > s.len - 1 - a.window);
+    if (!open) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+      for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float v = sc[n][j] * a.scale_log2;
-        if (!open) {
-          const int key = key0 + n * 8 + c * 2 + (j & 1), p = j < 2 ? p0 : p1;
-          const bool sees = key <= p && (a.window == 0 || key < a.sinks || key > p - a.window);
-          v = sees ? v : -INFINITY;
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int key = key0 + mt * 16 + g + (j >> 1) * 8, p = p_first + tq[n][j & 1];
+            const bool sees = key <= p && (a.window == 0 || key < a.sinks || key > p - a.window);
+            if (!sees) sc[mt][n][j] = -INFINITY;
+          }
+    }
+    // The maximum is only moved when a score passes it by kSlack (a factor of 2^8 in P,
+    // far from any type's range), which after the first tiles is rare: one vote a
+    // tile then replaces the reduction over the keys.
+    float x[NB][2];
+    bool past = false;
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        x[n][j] = fmaxf(sc[0][n][j], sc[0][n][j + 2]);
+#pragma unroll
+        for (int mt = 1; mt < MT; ++mt) x[n][j] = fmaxf(x[n][j], fmaxf(sc[mt][n][j], sc[mt][n][j + 2]));
+        past |= x[n][j] > m[n][j] + kSlack;
+      }
+    if (__any_sync(0xffffffffu, past)) {
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+          for (int w = 4; w < 32; w <<= 1) x[n][j] = fmaxf(x[n][j], __shfl_xor_sync(0xffffffffu, x[n][j], w));
+          const float to = fmaxf(m[n][j], x[n][j]);
+          e[n][j] = to == -INFINITY ? 0.f : to;
+          const float f2 = ex2(m[n][j] - e[n][j]);
+          m[n][j] = to;
+          l[n][j] *= f2;
+#pragma unroll
+          for (int k = 0; k < KS; ++k) {
+            o[n][k][j] *= f2;
+            o[n][k][j + 2] *= f2;
+          }
         }
-        sc[n][j] = v;
-        if (j < 2)
-          x0 = fmaxf(x0, v);
-        else
-          x1 = fmaxf(x1, v);
-      }
-    }
-    x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1));
-    x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
-    x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
-    x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
-    const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
-    const float e0 = n0 == -INFINITY ? 0.f : n0, e1 = n1 == -INFINITY ? 0.f : n1;
-    if (__any_sync(0xffffffffu, n0 != m0 || n1 != m1)) {
-      const float a0 = ex2(m0 - e0), a1 = ex2(m1 - e1);
-      l0 *= a0;
-      l1 *= a1;
-#pragma unroll
-      for (int n = 0; n < ON; ++n) {
-        o[n][0] *= a0;
-        o[n][1] *= a0;
-        o[n][2] *= a1;
-        o[n][3] *= a1;
-      }
-      m0 = n0;
-      m1 = n1;
     }
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      sc[n][0] = ex2(sc[n][0] - e0);
-      sc[n][1] = ex2(sc[n][1] - e0);
-      sc[n][2] = ex2(sc[n][2] - e1);
-      sc[n][3] = ex2(sc[n][3] - e1);
-      l0 += sc[n][0] + sc[n][1];
-      l1 += sc[n][2] + sc[n][3];
-    }
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          sc[mt][n][j] = ex2(sc[mt][n][j] - e[n][j & 1]);
+          l[n][j & 1] += sc[mt][n][j];
+        }
     // With several new tokens a masked key of this tile may be another row's
     // visible one, and 0 * (its infinity or NaN) would spoil this row: such a tile
     // is added element by element, masked keys left out.
     bool odd = false;
     if (!open && a.T > 1) {
+      constexpr uint32_t EX = DT == DT_BF16 ? 0x7F80u : 0x7C00u;
       for (int id = lane; id < TK * CH; id += 32) {
-        const uint4 u = *reinterpret_cast<const uint4*>(
-            smem + (vt - smem_u32(smem)) + (id / CH) * PITCH + (id % CH) * 16);
+        const uint4 u = *reinterpret_cast<const uint4*>(vtile + (id / CH) * PITCH + (id % CH) * 16);
         const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-        constexpr uint32_t EX = DT == DT_BF16 ? 0x7F80u : 0x7C00u;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          odd |= (w[j] & EX) == EX || ((w[j] >> 16) & EX) == EX;
+        for (int j = 0; j < 4; ++j) odd |= (w[j] & EX) == EX || ((w[j] >> 16) & EX) == EX;
       }
       odd = __any_sync(0xffffffffu, odd);
     }
     if (!odd) {
 #pragma unroll
-      for (int n = 0; n < NT; n += 2) {
+      for (int mt = 0; mt < MT; ++mt) {
         // P is held to 11 bits in float16; in bfloat16 (8 bits) a second product adds
         // what the rounding left, which brings it to 16.
-        uint32_t pf[4] = {pack2<DT>(sc[n][0], sc[n][1]), pack2<DT>(sc[n][2], sc[n][3]),
-                          pack2<DT>(sc[n + 1][0], sc[n + 1][1]), pack2<DT>(sc[n + 1][2], sc[n + 1][3])};
-        uint32_t pl[4];
-        if constexpr (DT == DT_BF16) {
-          const float x[8] = {sc[n][0], sc[n][1], sc[n][2], sc[n][3],
-                              sc[n + 1][0], sc[n + 1][1], sc[n + 1][2], sc[n + 1][3]};
+        uint32_t hi[NB][2], lo[NB][2];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 r = unpack2<DT>(pf[j]);
-            pl[j] = pack2<DT>(x[2 * j] - r.x, x[2 * j + 1] - r.y);
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const float p0 = sc[mt][n][2 * u], p1 = sc[mt][n][2 * u + 1];
+            hi[n][u] = pack2<DT>(p0, p1);
+            if constexpr (DT == DT_BF16) {
+              const float2 back = unpack2<DT>(hi[n][u]);
+              lo[n][u] = turn(pack2<DT>(p0 - back.x, p1 - back.y));
+            }
+            hi[n][u] = turn(hi[n][u]);
           }
-        }
 #pragma unroll
-        for (int d = 0; d < ON; d += 2) {
+        for (int k = 0; k < KS; ++k) {
           uint32_t vf[4];
-          ldsm4t(vt + (n * 8 + (lane & 7) + ((lane >> 3) & 1) * 8) * PITCH + (d + (lane >> 4)) * 16, vf);
-          mma<DT>(o[d], pf, vf[0], vf[1]);
-          mma<DT>(o[d + 1], pf, vf[2], vf[3]);
-          if constexpr (DT == DT_BF16) {
-            mma<DT>(o[d], pl, vf[0], vf[1]);
-            mma<DT>(o[d + 1], pl, vf[2], vf[3]);
+          ldsm4t(tile + v_at + mt * 16 * PITCH + k * 32, vf);
+#pragma unroll
+          for (int n = 0; n < NB; ++n) {
+            mma<DT>(o[n][k], vf, hi[n][0], hi[n][1]);
+            if constexpr (DT == DT_BF16) mma<DT>(o[n][k], vf, lo[n][0], lo[n][1]);
           }
         }
       }
     } else {
+#pragma unroll 1
+      for (int kk = 0; kk < TK; ++kk) {
+        const int key = key0 + kk, from = (kk & 7) * 4 + c;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
+        for (int n = 0; n < NB; ++n)
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk) {
-          const int from = (lane & ~3) | (kk >> 1);
-          const float w0 = __shfl_sync(0xffffffffu, sc[n][kk & 1], from);
-          const float w1 = __shfl_sync(0xffffffffu, sc[n][2 + (kk & 1)], from);
-          const int key = key0 + n * 8 + kk;
-          const bool s0 = key <= p0 && (a.window == 0 || key < a.sinks || key > p0 - a.window);
-          const bool s1 = key <= p1 && (a.window == 0 || key < a.sinks || key > p1 - a.window);
-          const unsigned char* vrow = smem + (vt - smem_u32(smem)) + (n * 8 + kk) * PITCH;
+          for (int j = 0; j < 2; ++j) {
+            float mine = 0.f;
 #pragma unroll
-          for (int d = 0; d < ON; ++d) {
-            const float2 v = unpack2<DT>(*reinterpret_cast<const uint32_t*>(vrow + d * 16 + c * 4));
-            if (s0) {
-              o[d][0] = fmaf(w0, v.x, o[d][0]);
-              o[d][1] = fmaf(w0, v.y, o[d][1]);
-            }
-            if (s1) {
-              o[d][2] = fmaf(w1, v.x, o[d][2]);
-              o[d][3] = fmaf(w1, v.y, o[d][3]);
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+              for (int u = 0; u < 2; ++u)
+                if (kk / 8 == mt * 2 + u) mine = sc[mt][n][2 * u + j];
+            const float w = __shfl_sync(0xffffffffu, mine, from);
+            const int p = p_first + tq[n][j];
+            if (!(key <= p && (a.window == 0 || key < a.sinks || key > p - a.window))) continue;
+            const T* vrow = reinterpret_cast<const T*>(vtile + kk * PITCH);
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+              o[n][k][j] = fmaf(w, Elem<DT>::to_f(vrow[k * 16 + g]), o[n][k][j]);
+              o[n][k][j + 2] = fmaf(w, Elem<DT>::to_f(vrow[k * 16 + g + 8]), o[n][k][j + 2]);
             }
           }
-        }
       }
     }
     ++t;
     if (t == s.tiles || i + 1 == count) {
-      // the segment ends: its sums over the quad's columns, then out or to the workspace
-      l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-      l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-      l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-      l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-      if (seg0 == 0 && t == s.tiles) {
+      // the segment ends: its sums over the lanes' keys, then out or to the workspace
+      const bool done = seg0 == 0 && t == s.tiles;
+      const int64_t piece = (part * 2 + (first ? 0 : 1)) * cols + col;
+      float2* ml = reinterpret_cast<float2*>(a.workspace) + piece * (8 * NB);
+      float* po = reinterpret_cast<float*>(reinterpret_cast<float2*>(a.workspace) +
+                                           (int64_t)parts * 2 * cols * (8 * NB)) + piece * (8 * NB) * D;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int r = k ? r1 : r0;
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+          for (int w = 4; w < 32; w <<= 1) l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], w);
+          const int lr = n * 8 + c * 2 + j, r = rbase + lr;
           if (r >= R) continue;
-          const float l = k ? l1 : l0, inv = l > 0.f || l != l ? 1.f / l : 0.f;
-          const int tq = r / a.G;
-          const int64_t row = ((int64_t)b * a.T + tq) * a.Hq + h * a.G + r - tq * a.G;
-          T* dst = reinterpret_cast<T*>(a.out) + row * D + c * 2;
+          const float sum = l[n][j];
+          if (done) {
+            const bool any = sum > 0.f || sum != sum;
+            const float inv = any ? 1.f / sum : 0.f;
+            const int64_t row = ((int64_t)b * a.T + tq[n][j]) * a.Hq + h * a.G + r - tq[n][j] * a.G;
+            T* dst = reinterpret_cast<T*>(a.out) + row * D + g;
 #pragma unroll
-          for (int n = 0; n < ON; ++n)
-            *reinterpret_cast<uint32_t*>(dst + n * 8) = pack2<DT>(o[n][2 * k] * inv, o[n][2 * k + 1] * inv);
-          if (a.lse != nullptr && c == 0) a.lse[row] = l > 0.f || l != l ? (k ? m1 : m0) * kLn2 + logf(l) : -INFINITY;
+            for (int k = 0; k < KS; ++k) {
+              dst[k * 16] = Elem<DT>::from_f(o[n][k][j] * inv);
+              dst[k * 16 + 8] = Elem<DT>::from_f(o[n][k][j + 2] * inv);
+            }
+            if (a.lse != nullptr && g == 0) a.lse[row] = any ? m[n][j] * kLn2 + logf(sum) : -INFINITY;
+          } else {
+            if (g == 0) ml[lr] = make_float2(m[n][j], sum);
+            float* dst = po + lr * D + g;
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+              dst[k * 16] = o[n][k][j];
+              dst[k * 16 + 8] = o[n][k][j + 2];
+            }
+          }
         }
-      } else {
-        const int64_t slot = (part * 2 + (first ? 0 : 1)) * cols + col;
-        float2* ml = reinterpret_cast<float2*>(a.workspace) + slot * 16;
-        float* po = reinterpret_cast<float*>(reinterpret_cast<float2*>(a.workspace) + (int64_t)parts * 2 * cols * 16) +
-                    slot * 16 * D;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int r = k ? r1 : r0, lr = g + 8 * k;
-          if (r >= R) continue;
-          if (c == 0) ml[lr] = k ? make_float2(m1, l1) : make_float2(m0, l0);
-#pragma unroll
-          for (int n = 0; n < ON; ++n)
-            *reinterpret_cast<float2*>(po + lr * D + n * 8 + c * 2) = make_float2(o[n][2 * k], o[n][2 * k + 1]);
-        }
-      }
       first = false;
       if (i + 1 < count) {
         do {
@@ -480,7 +544,8 @@ __global__ void __launch_bounds__(256) decode_join_kernel(const DecodeArgs a, in
   const int64_t row = live ? row_raw : rows - 1;
   const int hq = (int)(row % a.Hq), tq = (int)(row / a.Hq % a.T), b = (int)(row / a.Hq / a.T);
   const int h = hq / a.G, r = tq * a.G + hq - h * a.G;
-  const int rbs = row_blocks(a.G, a.T), cols = a.Hkv * rbs, col = h * rbs + r / 16;
+  const int R = a.G * a.T, per = 8 * blocks_of(R, D), groups = row_groups(R, D);
+  const int cols = a.Hkv * groups, col = h * groups + r / per;
   int64_t before, total;
   scan_to<TK>(a, lane, b, before, total);
   const int64_t chunk = max((int64_t)1, part_tiles(total, parts));
@@ -489,12 +554,12 @@ __global__ void __launch_bounds__(256) decode_join_kernel(const DecodeArgs a, in
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (n > 0 && p0 == p1) return;   // finished by its warp (the same for all warps of a row)
   const float2* ml = reinterpret_cast<const float2*>(a.workspace);
-  const float* po = reinterpret_cast<const float*>(ml + (int64_t)parts * 2 * cols * 16);
+  const float* po = reinterpret_cast<const float*>(ml + (int64_t)parts * 2 * cols * per);
   const int count = n > 0 ? (int)(p1 - p0 + 1) : 0;
   auto slot_row = [&](int i) {   // the piece of part p0 + i: a part's first segment is in its slot 0
     const int64_t p = p0 + i;
     const int64_t s = p * 2 + (i == 0 && before > p * chunk ? 1 : 0);
-    return (s * cols + col) * 16 + r % 16;
+    return (s * cols + col) * per + r % per;
   };
   float m = -INFINITY;
   for (int i = lane; i < count; i += 32) m = fmaxf(m, ml[slot_row(i)].x);
@@ -542,8 +607,9 @@ template <int D> int parts_for(int cols) {
   return warps / cols > 0 ? warps / cols : 1;
 }
 
-template <int D> size_t workspace_for(int cols) {
-  return (size_t)parts_for<D>(cols) * 2 * cols * 16 * (D + 2) * sizeof(float);
+template <int D> size_t workspace_for(int rows, int Hkv) {
+  const int cols = Hkv * row_groups(rows, D);
+  return (size_t)parts_for<D>(cols) * 2 * cols * 8 * blocks_of(rows, D) * (D + 2) * sizeof(float);
 }
 
 template <int DT, int D, int WPR>
@@ -565,19 +631,29 @@ cudaError_t launch_join(const DecodeArgs& a, int parts, cudaStream_t stream) {
   return e;
 }
 
-template <int DT, int D> cudaError_t launch_dim(const DecodeArgs& a, cudaStream_t stream) {
+template <int DT, int D, int NB> cudaError_t launch_blocks(const DecodeArgs& a, cudaStream_t stream) {
   constexpr int NW = Shape<D>::NW, SMEM = NW * Shape<D>::ST * kStageBytes<D>;
-  const int cols = a.Hkv * row_blocks(a.G, a.T), parts = parts_for<D>(cols);
-  cudaError_t e = cudaFuncSetAttribute(decode_kernel<DT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+  const int cols = a.Hkv * row_groups(a.G * a.T, D), parts = parts_for<D>(cols);
+  cudaError_t e = cudaFuncSetAttribute(decode_kernel<DT, D, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
   if (e != cudaSuccess) return e;
   const int64_t blocks = ((int64_t)parts * cols + NW - 1) / NW;
   if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  decode_kernel<DT, D><<<(unsigned)blocks, NW * 32, SMEM, stream>>>(a, parts);
+  decode_kernel<DT, D, NB><<<(unsigned)blocks, NW * 32, SMEM, stream>>>(a, parts);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   count_launch();
   // few rows with many pieces each: a CTA a row; else a warp a row
   return parts / a.B >= 16 ? launch_join<DT, D, 8>(a, parts, stream) : launch_join<DT, D, 1>(a, parts, stream);
+}
+
+template <int DT, int D> cudaError_t launch_dim(const DecodeArgs& a, cudaStream_t stream) {
+  switch (blocks_of(a.G * a.T, D)) {
+    case 1: return launch_blocks<DT, D, 1>(a, stream);
+    case 2: return launch_blocks<DT, D, 2>(a, stream);
+    default:
+      if constexpr (D != 256) return launch_blocks<DT, D, 4>(a, stream);
+      return cudaErrorInvalidValue;
+  }
 }
 
 template <int DT> cudaError_t launch_dt(const DecodeArgs& a, cudaStream_t stream) {
@@ -594,9 +670,9 @@ template <int DT> cudaError_t launch_dt(const DecodeArgs& a, cudaStream_t stream
 bool decode_supported(int D) { return D == 64 || D == 96 || D == 128 || D == 256; }
 
 size_t decode_workspace_bytes(int T, int Hq, int Hkv, int D) {
-  const int cols = Hkv * row_blocks(Hq / Hkv, T);
-  return D == 64 ? workspace_for<64>(cols) : D == 96 ? workspace_for<96>(cols)
-       : D == 128 ? workspace_for<128>(cols) : workspace_for<256>(cols);
+  const int rows = Hq / Hkv * T;
+  return D == 64 ? workspace_for<64>(rows, Hkv) : D == 96 ? workspace_for<96>(rows, Hkv)
+       : D == 128 ? workspace_for<128>(rows, Hkv) : workspace_for<256>(rows, Hkv);
 }
 
 cudaError_t launch_decode(const DecodeArgs& a, int dt, cudaStream_t stream) {

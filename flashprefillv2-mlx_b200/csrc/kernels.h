@@ -208,6 +208,7 @@ struct DecodeArgs {
   const int32_t* lengths;     // [B], the new tokens included
   int64_t table_stride;
   int B, T, Hq, Hkv, G, D, num_pages, page_size, table_width;
+  int page_shift;             // log2(page_size), -1 when it is no power of two
   int window, sinks;          // window 0: every key up to the query is seen
   float scale_log2;
   void* out;                  // [B, T, Hq, D]

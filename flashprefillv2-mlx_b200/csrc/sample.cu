@@ -10,17 +10,19 @@
 // of the maximum. A row without a logit above -inf gives -1.
 //
 // A row is read from DRAM once, into the shared memory of a cluster of 1 to 8 CTAs,
-// and noise is read only where a token is still in the running, so the logits' bytes
-// bound large batches and the chain of cluster-wide steps bounds single rows.
+// and noise is read only where a token is still in the running, so the bytes of the
+// two bound large batches and the chain of cluster-wide steps bounds single rows.
 //
 // Nothing is sorted but short lists. Top-k: every thread knows the largest logit of
-// its share; the (k / CTAs)-th largest of a CTA's 1024 such values is a bound that at
+// its share; the (k / CTAs)-th largest of a CTA's 512 such values is a bound that at
 // least k logits reach, and hardly more, so the few logits past it are gathered and
-// sorted. Otherwise (top-p alone, k too large, too many equal logits) the threshold is
-// found by counting: 1024 bins linear in x over the 32 T below the maximum, where all
-// the weight is, then bins over the ordered bit patterns inside the crossing bin until
-// it holds one value. Bin counts are integers and sums run in a fixed order, so a call
-// repeats bit for bit.
+// sorted. Top-p alone: logits are counted in 1024 bins linear in x over the 32 T below
+// the maximum, where all the weight is; the bin where the weight crosses p of it is
+// gathered and sorted, and the weight above it summed. Where such a list would not
+// hold the candidates (very large k, very many equal logits) the threshold is found by
+// counting alone, over the ordered bit patterns inside the crossing bin until it holds
+// one value. Counts are integers and sums run in a fixed order, so a call repeats bit
+// for bit.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -31,21 +33,46 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 1024;
-constexpr int kBins = 1024;
-constexpr int kList = 4096;                  // gathered candidates of a row
-constexpr int kSliceBytes = 160 * 1024;      // logits a CTA holds
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+constexpr int kBins = 2 * kThreads;          // of the linear histogram, two a thread
+constexpr int kKeyBits = 9;                  // bins over bit patterns, one a thread
+constexpr int kList = 2048;                  // gathered candidates of a row
+constexpr int kFew = kThreads / 2;           // of them that one CTA looks through by itself
+constexpr int kListBytes = kList * 12;       // keys with indices, and weights
+constexpr int kSliceTwo = 80 * 1024;         // logits a CTA holds when two share an SM,
+constexpr int kSliceOne = 176 * 1024;        // and when it has the SM to itself
 constexpr int kMaxCluster = 8;
+constexpr float kSpan = 32.f;                // of z in the bins: e^-32 of the weight is past them
+constexpr float kFloatMax = 3.402823466e+38f;
 constexpr uint32_t kLowest = 0x00800000u;    // order() of -FLT_MAX
+constexpr int kAnyIndex = 0x7fffffff;
 
-// Bit patterns in the order of the floats they hold.
+// Bit patterns in the order of the floats they hold (both zeros the same).
 __device__ __forceinline__ uint32_t order(float x) {
-  const uint32_t b = __float_as_uint(x);
+  const uint32_t b = __float_as_uint(x + 0.f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float unorder(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
+
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Larger of two packed pairs; of a number and a NaN the number.
+template <int DT> __device__ __forceinline__ uint32_t max_pair(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (DT == DT_BF16)
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else
+    asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <int DT> constexpr uint32_t kMinusInfPair = DT == DT_BF16 ? 0xFF80FF80u : 0xFC00FC00u;
 
 // One row's slice in a CTA: chunks of 16 bytes, aligned in memory, so the first and
 // the last chunk of a row may be partly outside it (filled with -inf).
@@ -56,6 +83,7 @@ template <int DT> struct Slice {
   const uint4* held;   // shared memory, null when the slice is read from global each time
   int64_t first;       // index of the first element of chunk 0 (may be negative)
   int chunks, vocab;
+  bool infinite;       // the row's maximum is +inf: such logits count as 0, others as -inf
 
   __device__ __forceinline__ int64_t index(int j) const { return first + (int64_t)j * VE; }
   __device__ __forceinline__ bool inside(int j) const {
@@ -71,103 +99,153 @@ template <int DT> struct Slice {
       e[i] = at + i >= 0 && at + i < vocab ? row[at + i] : Elem<DT>::from_f(-INFINITY);
     return u;
   }
-  // the chunk as floats: NaN as -inf, -0 as +0
+  // the chunk as floats, NaN as -inf
   __device__ __forceinline__ void get(int j, float (&x)[VE]) const {
     const uint4 u = held != nullptr ? held[j] : load(j);
     const uint32_t r[4] = {u.x, u.y, u.z, u.w};
     if constexpr (DT == DT_F32) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(r[i]);
+      for (int i = 0; i < 4; ++i) x[i] = fmaxf(__uint_as_float(r[i]), -INFINITY);
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float2 f = unpack2<DT>(r[i]);
+        const float2 f = unpack2<DT>(max_pair<DT>(r[i], kMinusInfPair<DT>));
         x[2 * i] = f.x;
         x[2 * i + 1] = f.y;
       }
     }
+    if (infinite) {
 #pragma unroll
-    for (int i = 0; i < VE; ++i) x[i] = fmaxf(x[i], -INFINITY) + 0.f;
+      for (int i = 0; i < VE; ++i) x[i] = x[i] == INFINITY ? 0.f : -INFINITY;
+    }
+  }
+  // the largest logit of a chunk (NaN and a row with infinities aside: it may be too large)
+  __device__ __forceinline__ float highest(int j) const {
+    const uint4 u = held != nullptr ? held[j] : load(j);
+    if constexpr (DT == DT_F32) {
+      return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)),
+                   fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+    } else {
+      const float2 f = unpack2<DT>(max_pair<DT>(max_pair<DT>(u.x, u.y), max_pair<DT>(u.z, u.w)));
+      return fmaxf(f.x, f.y);
+    }
+  }
+  // the largest logit of this thread's chunks
+  __device__ __forceinline__ float largest() const {
+    float mx = -INFINITY;
+    if constexpr (DT == DT_F32) {
+      for (int j = threadIdx.x; j < chunks; j += kThreads) {
+        float x[VE];
+        get(j, x);
+        mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), mx);
+      }
+    } else {
+      uint32_t best = kMinusInfPair<DT>;
+      for (int j = threadIdx.x; j < chunks; j += kThreads) {
+        const uint4 u = held != nullptr ? held[j] : load(j);
+        best = max_pair<DT>(max_pair<DT>(max_pair<DT>(u.x, u.y), max_pair<DT>(u.z, u.w)), best);
+      }
+      const float2 f = unpack2<DT>(best);
+      mx = fmaxf(f.x, f.y);
+    }
+    return mx;
+  }
+};
+
+// A threshold: what is above x, and of what equals it the indices up to `last`.
+struct Cut {
+  float x;
+  int last;
+  __device__ __forceinline__ bool keeps(float v, int at) const {
+    return v > x || (v == x && at <= last);
   }
 };
 
 struct Shared {
   unsigned hist[kBins];
-  unsigned long long best[32];
-  double sums[32][4];
+  unsigned long long warp_best[kWarps];
+  double sums[kWarps][4];
+  double scan[kWarps];
   // written by this CTA, read by the cluster
-  unsigned long long row_best, row_race;
+  unsigned long long race;
   double row_sums[4];
-  unsigned count, bound, ties;
+  unsigned row_top, bound, count, ties;
+  float part_weight;
   // broadcast inside the CTA
   unsigned long long out_best;
   double out_sums[4];
-  double scan[32];
-  unsigned found_bin, found_count;
   double found_above;
+  unsigned found_bin, found_count, out_u[2];
+  int part_start[kMaxCluster + 1];     // of each CTA's candidates in a merged list
+  float part_total[kMaxCluster];       // and their weight
   int tie_last;
 };
 
-__device__ __forceinline__ unsigned long long warp_max(unsigned long long v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const unsigned long long u = __shfl_xor_sync(0xffffffffu, v, o);
-    v = u > v ? u : v;
-  }
+__device__ __forceinline__ unsigned long long pack(uint32_t key, int64_t at) {
+  return (unsigned long long)key << 32 | (uint32_t)~(uint32_t)at;
+}
+
+__device__ __forceinline__ unsigned long long warp_best(unsigned long long v) {
+  const unsigned key = __reduce_max_sync(0xffffffffu, (unsigned)(v >> 32));
+  const unsigned low = __reduce_max_sync(0xffffffffu, (unsigned)(v >> 32) == key ? (unsigned)v : 0u);
+  return (unsigned long long)key << 32 | low;
+}
+
+// Largest of `v` over the CTA, valid in warp 0.
+__device__ unsigned long long block_best(Shared& sh, unsigned long long v) {
+  v = warp_best(v);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) sh.warp_best[threadIdx.x >> 5] = v;
+  __syncthreads();
+  if (threadIdx.x < 32) v = warp_best(threadIdx.x < kWarps ? sh.warp_best[threadIdx.x] : 0ull);
   return v;
 }
 
-// Largest of `v` over the cluster, in every thread.
-__device__ unsigned long long cluster_max(cg::cluster_group& cl, Shared& sh, unsigned long long v,
-                                          unsigned long long Shared::*slot) {
-  v = warp_max(v);
-  if ((threadIdx.x & 31) == 0) sh.best[threadIdx.x >> 5] = v;
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    v = warp_max(sh.best[threadIdx.x]);
-    if (threadIdx.x == 0) sh.*slot = v;
-  }
-  cl.sync();
-  if (threadIdx.x == 0) {
-    v = 0;
-    for (unsigned r = 0; r < cl.num_blocks(); ++r) {
-      const unsigned long long u = *cl.map_shared_rank(&(sh.*slot), r);
-      v = u > v ? u : v;
-    }
-    sh.out_best = v;
-  }
-  __syncthreads();
-  return sh.out_best;
-}
-
-// Sums of N values over the cluster, in a fixed order, in every thread.
-template <int N> __device__ void cluster_sum(cg::cluster_group& cl, Shared& sh, double (&v)[N]) {
+// Sums of N values over the CTA into row_sums, in a fixed order (no barrier after).
+template <int N> __device__ void block_sum(Shared& sh, const float (&x)[N]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < N; ++i) {
+    double v = x[i];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
-    if (lane == 0) sh.sums[warp][i] = v[i];
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (lane == 0) sh.sums[warp][i] = v;
   }
-  cl.sync();   // also: the last read of row_sums is over
+  __syncthreads();
   if (warp == 0) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      double s = sh.sums[lane][i];
+      double v = lane < kWarps ? sh.sums[lane][i] : 0.0;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      if (lane == 0) sh.row_sums[i] = s;
+      for (int o = kWarps / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      if (lane == 0) sh.row_sums[i] = v;
     }
   }
-  cl.sync();
-  if (threadIdx.x < N) {
-    double s = 0;
-    for (unsigned r = 0; r < cl.num_blocks(); ++r) s += cl.map_shared_rank(&sh, r)->row_sums[threadIdx.x];
-    sh.out_sums[threadIdx.x] = s;
-  }
-  __syncthreads();
+}
+
+// Adds up row_sums[i] of the cluster's CTAs, in a fixed order; a warp calls it.
+__device__ __forceinline__ double all_sums(cg::cluster_group& cl, Shared& sh, int i) {
+  const unsigned lane = threadIdx.x & 31;
+  double s = lane < cl.num_blocks() ? cl.map_shared_rank(&sh, lane)->row_sums[i] : 0.0;
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = sh.out_sums[i];
+  for (int o = 1; o < kMaxCluster; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return __shfl_sync(0xffffffffu, s, 0);
+}
+
+// The best `race` of the cluster's CTAs; a warp calls it.
+__device__ __forceinline__ unsigned long long all_best(cg::cluster_group& cl, Shared& sh) {
+  const unsigned lane = threadIdx.x & 31;
+  return warp_best(lane < cl.num_blocks() ? cl.map_shared_rank(&sh, lane)->race : 0ull);
+}
+
+// Sums of N values over the cluster, in every thread.
+template <int N> __device__ void cluster_sum(cg::cluster_group& cl, Shared& sh, const float (&x)[N], double (&v)[N]) {
+  cl.sync();   // the last read of row_sums is over
+  block_sum(sh, x);
+  cl.sync();
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = all_sums(cl, sh, i);
 }
 
 // Exclusive prefix of `v` over the CTA's threads.
@@ -183,78 +261,201 @@ __device__ double block_before(Shared& sh, double v) {
   if (lane == 31) sh.scan[warp] = incl;
   __syncthreads();
   if (warp == 0) {
-    const double mine = sh.scan[lane];
+    const double mine = lane < kWarps ? sh.scan[lane] : 0.0;
     double s = mine;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
+    for (int o = 1; o < kWarps; o <<= 1) {
       const double u = __shfl_up_sync(0xffffffffu, s, o);
       if (lane >= o) s += u;
     }
-    sh.scan[lane] = s - mine;
+    if (lane < kWarps) sh.scan[lane] = s - mine;
   }
   __syncthreads();
   return sh.scan[warp] + (incl - v);
 }
 
-// Descending bitonic sort of n (a power of two, at least 2) values in shared memory.
-template <typename K> __device__ void sort_down(K* v, int n) {
-  for (int size = 2; size <= n; size <<= 1)
-    for (int step = size >> 1; step > 0; step >>= 1) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < n / 2; i += kThreads) {
-        const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
-        const bool down = (lo & size) == 0;
-        const K x = v[lo], y = v[hi];
-        if ((x < y) == down) {
-          v[lo] = y;
-          v[hi] = x;
-        }
-      }
-    }
-  __syncthreads();
-}
-
-// The settings of one row and what its logits give.
+// The settings of one row and its largest logit.
 struct RowState {
-  float heat, inv_heat, top, scale;   // T, 1/T, the largest logit, bins per logit
+  float heat, inv_heat, to_log2, top, scale;   // T, 1/T, log2(e)/T, bins per logit
   float top_p, min_p;
 
-  __device__ __forceinline__ float z(float x) const { return x == top ? 0.f : __fdiv_rn(x - top, heat); }
-  __device__ __forceinline__ float z_near(float x) const { return x == top ? 0.f : (x - top) * inv_heat; }
-  __device__ __forceinline__ float weight(float x) const { return ex2(z_near(x) * kLog2e); }
-  __device__ __forceinline__ int bin(float x) const {
-    return x == top ? 0 : (int)fminf((top - x) * scale, (float)(kBins - 1));
+  __device__ __forceinline__ float z(float x) const { return __fdiv_rn(x - top, heat); }
+  __device__ __forceinline__ float weight(float x) const { return ex2((x - top) * to_log2); }
+  // bins as the floats 2^23 + bin (the addition rounds to whole bins); monotone in x
+  __device__ __forceinline__ float place(float x) const {
+    return fminf((top - x) * scale, (float)(kBins - 1)) + 8388608.f;
+  }
+  // 512 bins of the search by counting
+  __device__ __forceinline__ int coarse(float x) const {
+    return x == top ? 0 : (int)fminf((top - x) * scale * 0.5f, (float)(kThreads - 1));
   }
 };
 
-// A threshold: keys above `key`, and of those equal to it the ones up to index `last`.
-struct Cut {
-  uint32_t key;
-  int last;
-  __device__ __forceinline__ bool keeps(uint32_t k, int64_t at) const {
-    return k > key || (k == key && at <= last);
+// Descending bitonic sort of the n <= kList values of `v` (shared memory) by the first
+// warps of the CTA, four values a thread in registers: steps of 1 and 2 inside a
+// thread, up to 64 by shuffles, above through shared memory. Past n there are zeros up
+// to a whole number of threads. The whole CTA calls it; on return thread i holds the
+// values 4 i to 4 i + 3 (0 past the warps that sorted).
+__device__ void sort_down(unsigned long long* v, int n, unsigned long long (&x)[4]) {
+  int n2 = 128;   // a warp
+  while (n2 < n) n2 <<= 1;
+  const int tid = threadIdx.x, threads = n2 / 4;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = 0;
+  __syncthreads();
+  if (tid >= threads) return;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (4 * tid + i < n) x[i] = v[4 * tid + i];
+  auto swap = [](unsigned long long& p, unsigned long long& q, bool down) {
+    const bool change = (p < q) == down;
+    const unsigned long long u = change ? q : p, w = change ? p : q;
+    p = u;
+    q = w;
+  };
+  swap(x[0], x[1], true);
+  swap(x[2], x[3], false);
+  for (int size = 4; size <= n2; size <<= 1) {
+    const bool down = (4 * tid & size) == 0;
+    for (int step = size >> 1; step >= 128; step >>= 1) {
+      if (threads > 32) named_bar_sync(1, threads);   // the last round's reads are over
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[4 * tid + i] = x[i];
+      named_bar_sync(1, threads);
+      const bool keep_large = ((4 * tid & step) == 0) == down;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const unsigned long long y = v[(4 * tid + i) ^ step];
+        x[i] = (x[i] > y) == keep_large ? x[i] : y;
+      }
+    }
+    for (int step = min(size >> 1, 64); step >= 4; step >>= 1) {
+      const bool keep_large = ((4 * tid & step) == 0) == down;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const unsigned long long y = __shfl_xor_sync(0xffffffffu, x[i], step >> 2);
+        x[i] = (x[i] > y) == keep_large ? x[i] : y;
+      }
+    }
+    swap(x[0], x[2], down);
+    swap(x[1], x[3], down);
+    swap(x[0], x[1], down);
+    swap(x[2], x[3], down);
   }
-};
+}
 
-// Adds up the bins of the cluster's CTAs; thread i gets bin i.
+// Where each CTA's candidates start in a list of all of them, into part_start; returns
+// their number, the same in every thread of the cluster.
+__device__ int place_parts(cg::cluster_group& cl, Shared& sh) {
+  const int lane = threadIdx.x & 31, nblocks = (int)cl.num_blocks();
+  const int c = lane < nblocks ? (int)cl.map_shared_rank(&sh, lane)->count : 0;
+  int upto = c;
+#pragma unroll
+  for (int o = 1; o < kMaxCluster; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += u;
+  }
+  if (threadIdx.x < kMaxCluster) sh.part_start[lane + 1] = upto;   // past the last CTA: the end
+  if (threadIdx.x == 0) sh.part_start[0] = 0;
+  return __shfl_sync(0xffffffffu, upto, kMaxCluster - 1);
+}
+
+// Sorts a CTA's candidates and finds their places among the whole cluster's (descending,
+// ties by index ascending): on return thread i has the CTA's candidates 4 i to 4 i + 3 in
+// v, their weights in w, the number of larger candidates in rank and their weight in
+// before. Every CTA sorts its own and copies the others' sorted ones with their running
+// weights, where a binary search gives a candidate's place. All CTAs call it, after
+// place_parts().
+__device__ void merge_lists(cg::cluster_group& cl, Shared& sh, const RowState& row, unsigned long long* list,
+                            float* ahead, unsigned long long (&v)[4], float (&w)[4], int (&rank)[4],
+                            float (&before)[4]) {
+  const int tid = threadIdx.x, me = (int)cl.block_rank(), nblocks = (int)cl.num_blocks();
+  __syncthreads();
+  const int start = sh.part_start[me], own = sh.part_start[me + 1] - start;
+  sort_down(list, own, v);
+  double mine = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    w[i] = 4 * tid + i < own ? row.weight(unorder((uint32_t)(v[i] >> 32))) : 0.f;
+    mine += w[i];
+  }
+  double run = block_before(sh, mine);   // its barriers also end the reads of the unsorted list
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    rank[i] = 4 * tid + i;
+    before[i] = (float)run;
+    if (4 * tid + i < own) {
+      list[start + 4 * tid + i] = v[i];
+      ahead[start + 4 * tid + i] = (float)run;
+    }
+    run += w[i];
+  }
+  if (tid == kThreads - 1) sh.part_weight = (float)run;
+  cl.sync();
+  const int all = sh.part_start[nblocks];
+  for (int i = tid; i < all; i += kThreads) {
+    int c = 0;
+#pragma unroll
+    for (int q = 1; q < kMaxCluster; ++q) c += i >= sh.part_start[q];
+    const unsigned long long key = cl.map_shared_rank(list, c)[i];
+    const float f = cl.map_shared_rank(ahead, c)[i];
+    list[i] = key;   // its own ones with what they are
+    ahead[i] = f;
+  }
+  if (tid < nblocks) sh.part_total[tid] = cl.map_shared_rank(&sh, tid)->part_weight;
+  __syncthreads();
+  if (4 * tid >= own) return;
+  for (int c = 0; c < nblocks; ++c) {
+    if (c == me) continue;
+    const int s0 = sh.part_start[c], n = sh.part_start[c + 1] - s0;
+    if (n == 0) continue;
+    int lo[4] = {0, 0, 0, 0};   // known to be larger
+    for (int step = 1 << (31 - __clz(n)); step > 0; step >>= 1) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int to = lo[i] + step;
+        const bool larger = list[s0 + min(to, n) - 1] > v[i];
+        lo[i] = to <= n && larger ? to : lo[i];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      rank[i] += lo[i];
+      before[i] += lo[i] < n ? ahead[s0 + lo[i]] : sh.part_total[c];
+    }
+  }
+}
+
+__device__ __forceinline__ void gather(Shared& sh, unsigned long long* list, float x, int64_t at) {
+  const unsigned i = atomicAdd(&sh.count, 1u);
+  if (i < kList) list[i] = pack(order(x), at);
+}
+
+__device__ __forceinline__ void prefetch_l2(const void* p) {
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+}
+
+// Adds up bin threadIdx.x of the cluster's CTAs and clears it.
 __device__ unsigned gather_bin(cg::cluster_group& cl, Shared& sh) {
   cl.sync();
   unsigned c = 0;
-  for (unsigned r = 0; r < cl.num_blocks(); ++r) c += cl.map_shared_rank(&sh, r)->hist[threadIdx.x];
+#pragma unroll
+  for (unsigned r = 0; r < kMaxCluster; ++r)
+    if (r < cl.num_blocks()) c += cl.map_shared_rank(&sh, r)->hist[threadIdx.x];
   cl.sync();
   sh.hist[threadIdx.x] = 0;
   return c;
 }
 
-// Search for the value where the ordered logits reach `target` (a count, or a weight).
-// On return the crossing value is `key` with `count` logits equal to it and `above` of
-// the target used up by larger ones; or, when `count` logits in all are known to be
-// needed, `key` is a lower bound that just these reach.
+// Search by counting for the value where the ordered logits within `within` reach
+// `target` (a count, or a weight). On return the crossing value is `key` with `count`
+// logits equal to it and `above` of the target used up by larger ones; or, when not
+// `single`, `key` is a lower bound, and what reaches it is just what is needed.
 struct Found {
   uint32_t key;
   unsigned count;
   double above;
-  bool single;   // `key` is one value (else a bound with all `count` logits needed)
+  bool single;
 };
 
 template <int DT, bool WEIGHT>
@@ -268,17 +469,17 @@ __device__ Found search(cg::cluster_group& cl, Shared& sh, const Slice<DT>& sl, 
     sl.get(j, x);
 #pragma unroll
     for (int i = 0; i < VE; ++i) {
-      if (x[i] == -INFINITY || order(x[i]) < within.key) continue;
-      const int b = row.bin(x[i]);
+      if (x[i] == -INFINITY || x[i] < within.x) continue;
+      const int b = row.coarse(x[i]);
       // the last bin's weight is nothing next to the row's, and its count is what is left
-      if (!WEIGHT || b < kBins - 1) atomicAdd(&sh.hist[b], 1u);
+      if (!WEIGHT || b < kThreads - 1) atomicAdd(&sh.hist[b], 1u);
     }
   }
   unsigned c = gather_bin(cl, sh);
   double mass = (double)c;
-  if (WEIGHT) mass *= (double)ex2(-((float)tid + (tid == 0 ? 0.f : 0.5f)) / row.scale * row.inv_heat * kLog2e);
+  if (WEIGHT) mass *= (double)ex2(-((float)tid + (tid == 0 ? 0.f : 0.5f)) / (row.scale * 0.5f) * row.to_log2);
   double before = block_before(sh, mass);
-  if (tid == 0) sh.found_bin = kBins - 1;
+  if (tid == 0) sh.found_bin = kThreads - 1;
   __syncthreads();
   if (before + mass >= target) atomicMin(&sh.found_bin, (unsigned)tid);
   __syncthreads();
@@ -297,7 +498,7 @@ __device__ Found search(cg::cluster_group& cl, Shared& sh, const Slice<DT>& sl, 
     // The bins' weights were estimates: sum the weights above and in three bins around.
     int moved = 0;
     while (true) {
-      bin = min(max(bin, 1), kBins - 2);
+      bin = min(max(bin, 1), kThreads - 2);
       float s[4] = {0.f, 0.f, 0.f, 0.f};
       for (int j = tid; j < sl.chunks; j += kThreads) {
         float x[VE];
@@ -305,8 +506,8 @@ __device__ Found search(cg::cluster_group& cl, Shared& sh, const Slice<DT>& sl, 
         const int64_t at = sl.index(j);
 #pragma unroll
         for (int i = 0; i < VE; ++i) {
-          if (x[i] == -INFINITY || !within.keeps(order(x[i]), at + i)) continue;
-          const int b = row.bin(x[i]);
+          if (x[i] == -INFINITY || !within.keeps(x[i], (int)at + i)) continue;
+          const int b = row.coarse(x[i]);
           if (b > bin + 1) continue;
           const float w = row.weight(x[i]);
           s[0] += b < bin - 1 ? w : 0.f;
@@ -315,14 +516,14 @@ __device__ Found search(cg::cluster_group& cl, Shared& sh, const Slice<DT>& sl, 
           s[3] += b == bin + 1 ? w : 0.f;
         }
       }
-      double v[4] = {s[0], s[1], s[2], s[3]};
-      cluster_sum(cl, sh, v);
+      double v[4];
+      cluster_sum(cl, sh, s, v);
       if (v[0] >= target && bin > 1 && moved <= 0) {
         bin -= 3;
         moved = -1;
         continue;
       }
-      if (v[0] + v[1] + v[2] + v[3] < target && bin < kBins - 2 && moved >= 0) {
+      if (v[0] + v[1] + v[2] + v[3] < target && bin < kThreads - 2 && moved >= 0) {
         bin += 3;
         moved = 1;
         continue;
@@ -343,11 +544,11 @@ __device__ Found search(cg::cluster_group& cl, Shared& sh, const Slice<DT>& sl, 
   }
   // the keys of the bin: bin() falls as the key grows
   uint32_t lo = kLowest, hi = order(row.top);
-  if (bin < kBins - 1) {   // smallest key whose bin is <= bin
+  if (bin < kThreads - 1) {   // smallest key whose bin is <= bin
     uint32_t a = kLowest, b = hi;
     while (a < b) {
       const uint32_t mid = a + (b - a) / 2;
-      if (row.bin(unorder(mid)) <= bin) b = mid; else a = mid + 1;
+      if (row.coarse(unorder(mid)) <= bin) b = mid; else a = mid + 1;
     }
     lo = a;
   }
@@ -355,18 +556,18 @@ __device__ Found search(cg::cluster_group& cl, Shared& sh, const Slice<DT>& sl, 
     uint32_t a = lo, b = hi;
     while (a < b) {
       const uint32_t mid = a + (b - a + 1) / 2;
-      if (row.bin(unorder(mid)) >= bin) a = mid; else b = mid - 1;
+      if (row.coarse(unorder(mid)) >= bin) a = mid; else b = mid - 1;
     }
     hi = a;
   }
-  if (lo < within.key) lo = within.key;
+  if (within.x > -INFINITY && lo < order(within.x)) lo = order(within.x);
   if (hi < lo) return {lo, 0, above, false};   // the target is just past all there is
   while (true) {
     if (!WEIGHT && above + (double)count <= target) return {lo, count, above, false};
     if (count == 1) return {lo, 1, above, false};
     if (lo >= hi && count != 0xffffffffu) return {lo, count, above, true};
     const uint32_t width = hi - lo;   // keys less one
-    const int bits = 32 - __clz(width | 1), shift = bits > 10 ? bits - 10 : 0;
+    const int bits = 32 - __clz(width | 1), shift = bits > kKeyBits ? bits - kKeyBits : 0;
     for (int j = tid; j < sl.chunks; j += kThreads) {
       float x[VE];
       sl.get(j, x);
@@ -380,7 +581,7 @@ __device__ Found search(cg::cluster_group& cl, Shared& sh, const Slice<DT>& sl, 
     mass = (double)c;
     const uint32_t off = (uint32_t)tid << shift;
     if (WEIGHT && c != 0) {
-      // a bin of several values weighs as its middle one: it spans under 2^-15 of z
+      // a bin of several values weighs as its middle one: it spans under 2^-12 of z
       const uint32_t span = (1u << shift) - 1;
       const uint32_t mid = hi - off - min(span / 2, (hi - off - lo) / 2);
       mass *= (double)row.weight(unorder(mid));
@@ -413,9 +614,9 @@ __device__ Found search(cg::cluster_group& cl, Shared& sh, const Slice<DT>& sl, 
   }
 }
 
-// Index of the `need`-th logit (from 1) equal to `key`, in index order.
+// Index of the `need`-th logit (from 1) equal to `value`, in index order.
 template <int DT>
-__device__ int tie_index(cg::cluster_group& cl, Shared& sh, const Slice<DT>& sl, uint32_t key, unsigned need) {
+__device__ int tie_index(cg::cluster_group& cl, Shared& sh, const Slice<DT>& sl, float value, unsigned need) {
   constexpr int VE = Slice<DT>::VE;
   const int share = (sl.chunks + kThreads - 1) / kThreads;   // chunks a thread, consecutive
   const int j0 = min(sl.chunks, (int)threadIdx.x * share), j1 = min(sl.chunks, j0 + share);
@@ -424,7 +625,7 @@ __device__ int tie_index(cg::cluster_group& cl, Shared& sh, const Slice<DT>& sl,
     float x[VE];
     sl.get(j, x);
 #pragma unroll
-    for (int i = 0; i < VE; ++i) mine += order(x[i]) == key;
+    for (int i = 0; i < VE; ++i) mine += x[i] == value;
   }
   const unsigned before = (unsigned)block_before(sh, (double)mine);
   if (threadIdx.x == kThreads - 1) {
@@ -441,7 +642,7 @@ __device__ int tie_index(cg::cluster_group& cl, Shared& sh, const Slice<DT>& sl,
       float x[VE];
       sl.get(j, x);
       for (int i = 0; i < VE; ++i)
-        if (order(x[i]) == key && ++seen == need) {
+        if (x[i] == value && ++seen == need) {
           const int at = (int)(sl.index(j) + i);
           for (unsigned r = 0; r < cl.num_blocks(); ++r) cl.map_shared_rank(&sh, r)->tie_last = at;
         }
@@ -455,12 +656,226 @@ __device__ __forceinline__ float race_score(float z, float e) {
   return e > 0.f ? z - logf(e) : -3.402823466e+38f;   // noise has to be positive
 }
 
-__device__ __forceinline__ unsigned long long pack(uint32_t key, int64_t at) {
-  return (unsigned long long)key << 32 | (uint32_t)~(uint32_t)at;
+// The smallest logit whose weight reaches min_p in (0, 1]; every lane of a warp calls it.
+__device__ float min_p_logit(const RowState& row) {
+  const int lane = threadIdx.x & 31;
+  uint32_t lo = kLowest, hi = order(row.top);   // hi reaches it: its weight is 1
+  while (lo < hi) {
+    const uint32_t step = (hi - lo) / 32 + 1;
+    const uint64_t mine = (uint64_t)lo + (uint64_t)lane * step;
+    const bool reaches = mine >= hi || expf(row.z(unorder((uint32_t)mine))) >= row.min_p;
+    const int at = __ffs(__ballot_sync(0xffffffffu, reaches)) - 1;   // first lane that reaches it, -1: none
+    const uint32_t base = lo;
+    if (at != 0) lo = base + (uint32_t)(at < 0 ? 31 : at - 1) * step + 1;
+    if (at >= 0) hi = min(hi, base + (uint32_t)at * step);
+  }
+  return unorder(hi);
+}
+
+// Top-p over the whole row: cut after the shortest prefix with p of the weight.
+// Returns false (everywhere) when the crossing bin does not fit the list.
+template <int DT>
+__device__ bool nucleus(cg::cluster_group& cl, Shared& sh, const Slice<DT>& sl, const RowState& row,
+                        unsigned long long* list, float* ahead, double& whole, Cut& cut) {
+  constexpr int VE = Slice<DT>::VE;
+  const int tid = threadIdx.x;
+  float s[1] = {0.f};
+  for (int j = tid; j < sl.chunks; j += kThreads) {
+    float x[VE];
+    sl.get(j, x);
+#pragma unroll
+    for (int i = 0; i < VE; ++i) {
+      s[0] += row.weight(x[i]);
+      const int b = __float_as_int(row.place(x[i])) & (kBins - 1);
+      // past the last bin there is no weight to speak of
+      if (b < kBins - 1) atomicAdd(&sh.hist[b], 1u);
+    }
+  }
+  block_sum(sh, s);
+  cl.sync();
+  unsigned c0 = 0, c1 = 0;
+#pragma unroll
+  for (unsigned r = 0; r < kMaxCluster; ++r)
+    if (r < cl.num_blocks()) {
+      const uint2 u = reinterpret_cast<const uint2*>(cl.map_shared_rank(&sh, r)->hist)[tid];
+      c0 += u.x;
+      c1 += u.y;
+    }
+  whole = all_sums(cl, sh, 0);
+  if (tid == 0) sh.found_bin = kBins - 2;
+  // a bin weighs about its count times its middle's weight
+  const float per_bin = row.to_log2 / row.scale;
+  const double m0 = (double)c0 * ex2(-(tid == 0 ? 0.25f : 2.f * tid) * per_bin);
+  const double m1 = (double)c1 * ex2(-(2.f * tid + 1.f) * per_bin);
+  const double start = block_before(sh, m0 + m1);
+  const double target = (double)row.top_p * whole;
+  if (start + m0 >= target)
+    atomicMin(&sh.found_bin, min(2u * tid, (unsigned)kBins - 2u));
+  else if (start + m0 + m1 >= target)
+    atomicMin(&sh.found_bin, min(2u * tid + 1u, (unsigned)kBins - 2u));
+  __syncthreads();
+  int bin = (int)sh.found_bin, moved = 0;
+  for (int tries = 0; tries < 16; ++tries) {
+    // the weight above the bin, and the bin's logits
+    const float at_bin = 8388608.f + (float)bin;
+    float a[1] = {0.f};
+    for (int j = tid; j < sl.chunks; j += kThreads) {
+      float x[VE];
+      sl.get(j, x);
+#pragma unroll
+      for (int i = 0; i < VE; ++i) {
+        const float p = row.place(x[i]);
+        if (p < at_bin) a[0] += row.weight(x[i]);
+        if (p == at_bin) gather(sh, list, x[i], sl.index(j) + i);
+      }
+    }
+    cl.sync();   // row_sums, race and the lists of the last try were read
+    block_sum(sh, a);
+    cl.sync();
+    const int n = place_parts(cl, sh);
+    if (n > kList) return false;
+    const double above = all_sums(cl, sh, 0);
+    unsigned long long v[4];
+    float w[4], before[4];
+    int rank[4];
+    merge_lists(cl, sh, row, list, ahead, v, w, rank, before);
+    const int own = (int)sh.count;
+    // the last one that the prefix has to take: the smallest with less than the target before it
+    unsigned long long least = 0;   // inverted, so that the smallest is the best
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (4 * tid + i < own && above + before[i] < target) least = max(least, ~v[i]);
+    least = block_best(sh, least);
+    if (tid == 0) sh.race = least;
+    double total = above;
+    for (unsigned r = 0; r < cl.num_blocks(); ++r) total += sh.part_total[r];
+    cl.sync();
+    least = all_best(cl, sh);
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    // The estimate of the bin is off by a rounding at most, so a step that would turn back
+    // has met the crossing.
+    if (above >= target && bin > 0 && moved <= 0) {
+      bin += moved = -1;
+    } else if (total < target && bin < kBins - 2 && moved >= 0) {
+      bin += moved = 1;
+    } else {
+      if (least == 0) {   // nothing of the bin is needed
+        cut.x = row.top - ((float)bin - 0.5f) / row.scale;
+        cut.last = kAnyIndex;
+      } else {
+        cut.x = unorder((uint32_t)(~least >> 32));
+        cut.last = (int)(uint32_t)least;
+      }
+      return true;
+    }
+  }
+  return false;
+}
+
+// The race over a CTA's tokens that the cut keeps (all but -inf with ALL): its best
+// pack(order(score), index), thread by thread. With sum_here the weights of all tokens
+// are added to `sum`.
+//
+// A thread's noise is loaded 16 values ahead of their use. Scores are first taken to
+// about 1e-4, in powers of two, and a thread keeps its best chunk of them; then only
+// the chunks within a margin of the CTA's best are scored exactly.
+template <int DT, bool ALL>
+__device__ __forceinline__ unsigned long long race(Shared& sh, const Slice<DT>& sl, const RowState& row,
+                                                   const Cut cut, const float* noise, bool sum_here, float& sum) {
+  constexpr int VE = Slice<DT>::VE, DEPTH = 16 / VE;
+  const int tid = threadIdx.x;
+  const bool aligned = reinterpret_cast<uintptr_t>(noise + sl.first) % 16 == 0;
+  float e[DEPTH][VE];
+  auto fetch = [&](int j, float (&to)[VE]) {
+#pragma unroll
+    for (int i = 0; i < VE; ++i) to[i] = INFINITY;
+    if (j >= sl.chunks || (!ALL && !(sl.highest(j) >= cut.x))) return;
+    const int64_t at = sl.index(j);
+    if (aligned && sl.inside(j)) {
+#pragma unroll
+      for (int i = 0; i < VE; i += 4) {
+        const float4 f = __ldcs(reinterpret_cast<const float4*>(noise + at + i));
+        to[i] = f.x, to[i + 1] = f.y, to[i + 2] = f.z, to[i + 3] = f.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < VE; ++i)
+        if (at + i >= 0 && at + i < sl.vocab) to[i] = noise[at + i];
+    }
+  };
+#pragma unroll
+  for (int u = 0; u < DEPTH; ++u) fetch(tid + u * kThreads, e[u]);
+  float best = -INFINITY, second = -INFINITY;   // of the thread's chunks
+  int best_j = 0;
+  bool any = false, odd = false;
+  for (int jw = tid; jw < sl.chunks; jw += DEPTH * kThreads) {
+#pragma unroll
+    for (int u = 0; u < DEPTH; ++u) {
+      const int j = jw + u * kThreads;
+      if (j < sl.chunks) {
+        float x[VE], near = -INFINITY;
+        sl.get(j, x);
+        const int at = (int)sl.index(j);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) {
+          const float t = (x[i] - row.top) * row.to_log2;
+          if (sum_here) sum += ex2(t);
+          const float score = t - lg2(e[u][i]);
+          if (ALL) {
+            near = fmaxf(near, score);
+          } else if (cut.keeps(x[i], at + i)) {
+            near = fmaxf(near, score);
+            any = true;
+          }
+        }
+        // (a noise of 0 or below the normal range: an infinite score, which says nothing)
+        odd |= near == INFINITY;
+        if (near > best) {
+          second = best;
+          best = near;
+          best_j = j;
+        } else {
+          second = fmaxf(second, near);
+        }
+        fetch(j + DEPTH * kThreads, e[u]);
+      }
+    }
+  }
+  const unsigned high = __reduce_max_sync(0xffffffffu, order(best));
+  any |= ALL && sl.chunks > 0;
+  __syncthreads();
+  if ((tid & 31) == 0) sh.warp_best[tid >> 5] = high;
+  odd = __syncthreads_or(odd);
+  any = __syncthreads_or(any);
+  const unsigned cta =
+      __reduce_max_sync(0xffffffffu, (unsigned)sh.warp_best[tid & (kWarps - 1)]);
+  const float bar = unorder(cta) - 3e-3f;
+  // nothing within reach of a number: noise out of contract, all of it is scored
+  odd |= any && !(bar > -INFINITY);
+  unsigned long long best_key = 0;
+  if (odd || best >= bar) {
+    const bool every = odd || second >= bar;
+    for (int j = every ? tid : best_j; j < sl.chunks; j += every ? kThreads : 0x40000000) {
+      float x[VE];
+      sl.get(j, x);
+#pragma unroll 1
+      for (int i = 0; i < VE; ++i) {
+        float mine = x[0];
+#pragma unroll
+        for (int q = 1; q < VE; ++q) mine = i == q ? x[q] : mine;
+        const int64_t at = sl.index(j) + i;
+        if (!cut.keeps(mine, (int)at)) continue;
+        const float z = row.z(mine);
+        if (z > -INFINITY) best_key = max(best_key, pack(order(race_score(z, noise[at])), at));
+      }
+    }
+  }
+  return best_key;
 }
 
 template <int DT>
-__global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a, int per) {
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a, int per) {
   using T = typename Elem<DT>::T;
   constexpr int VE = Slice<DT>::VE;
   extern __shared__ __align__(16) unsigned char dyn[];
@@ -469,11 +884,13 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a,
   const int tid = threadIdx.x, rank = (int)cl.block_rank(), nblocks = (int)cl.num_blocks();
   const int r = blockIdx.x / nblocks;
   unsigned long long* list = reinterpret_cast<unsigned long long*>(dyn);
-  uint4* held = reinterpret_cast<uint4*>(dyn + kList * 8);
+  float* ahead = reinterpret_cast<float*>(dyn + kList * 8);
+  uint4* held = reinterpret_cast<uint4*>(dyn + kListBytes);
 
   Slice<DT> sl;
   sl.row = reinterpret_cast<const T*>(a.logits) + r * a.logits_stride;
   sl.vocab = a.vocab;
+  sl.infinite = false;
   const int mis = (int)(reinterpret_cast<uintptr_t>(sl.row) % 16 / sizeof(T));
   const int all = (int)(((int64_t)mis + a.vocab + VE - 1) / VE);
   const int share = (all + nblocks - 1) / nblocks;   // <= per when slices are held
@@ -490,13 +907,9 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a,
       else
         held[j] = sl.load(j);
     }
-    asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
+    asm volatile("cp.async.commit_group;" ::: "memory");
     sl.held = held;
   }
-  sh.hist[tid] = 0;
-  if (tid == 0) sh.count = 0;
-  __syncthreads();
-
   // settings
   RowState row;
   const float heat = a.temperature != nullptr ? a.temperature[r] : a.temperature_s;
@@ -504,26 +917,70 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a,
   row.min_p = a.min_p != nullptr ? a.min_p[r] : a.min_p_s;
   const int k_set = a.top_k != nullptr ? a.top_k[r] : a.top_k_s;
   const bool greedy = !(heat > 0.f);
-  row.heat = greedy ? 1.f : heat;
+  row.heat = greedy ? 1.f : fmaxf(heat, 1e-30f);   // its reciprocal stays finite
   row.inv_heat = 1.f / row.heat;
-  row.scale = (float)kBins / 32.f * row.inv_heat;
+  row.to_log2 = row.inv_heat * kLog2e;
+  row.scale = (float)kBins / kSpan * row.inv_heat;
+  const bool use_k = k_set > 0 && k_set < a.vocab;
+  const bool use_p = !(row.top_p >= 1.f);
+  const bool single = greedy || k_set == 1 || !(row.top_p > 0.f) || !(row.min_p <= 1.f);
+  const int need = (k_set + nblocks - 1) / nblocks;
+  const bool use_list = !single && use_k && need <= kThreads;
+  sh.hist[tid] = sh.hist[tid + kThreads] = 0;
+  if (tid == 0) sh.count = 0;
+  // A thread reads back its own chunks only, here and below, but for tie_index().
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
 
-  // the largest logit and its lowest index
-  float mx = -INFINITY;
-  int64_t mx_at = 0;
-  for (int j = tid; j < sl.chunks; j += kThreads) {
-    float x[VE];
-    sl.get(j, x);
+  // the largest logit, and for top-k the CTA's bound: bit by bit from the top, 16 bits
+  // bound it closely enough
+  uint32_t* maxima = reinterpret_cast<uint32_t*>(list);
+  maxima[tid] = order(sl.largest());
+  __syncthreads();
+  if (tid < 32) {
+    uint32_t m[kWarps], v = 0, low = 0;
 #pragma unroll
-    for (int i = 0; i < VE; ++i)
-      if (x[i] > mx) {
-        mx = x[i];
-        mx_at = sl.index(j) + i;
+    for (int i = 0; i < kWarps; ++i) {
+      m[i] = maxima[tid + 32 * i];
+      v = max(v, m[i]);
+    }
+    if (use_list && need <= 8) {
+      // few are needed: the need-th of these 32 lanes' maxima bounds them as well
+      int larger = 0;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const uint32_t u = __shfl_sync(0xffffffffu, v, i);
+        larger += u > v || (u == v && i < tid);
       }
+      low = __reduce_max_sync(0xffffffffu, larger == need - 1 ? v : 0u);
+    }
+    v = __reduce_max_sync(0xffffffffu, v);
+    if (use_list && need > 8)
+      for (int bit = 31; bit >= 16; --bit) {
+        const uint32_t trial = low | 1u << bit;
+        if (trial > v) continue;
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) c += m[i] >= trial;
+        if (__reduce_add_sync(0xffffffffu, c) >= need) low = trial;
+      }
+    if (tid == 0) {
+      sh.row_top = v;
+      sh.bound = low & 0xFFFF0000u;
+    }
   }
-  const unsigned long long top = cluster_max(cl, sh, pack(order(mx), mx_at), &Shared::row_best);
-  row.top = unorder((uint32_t)(top >> 32));
-  const int first = (int)~(uint32_t)top;
+  cl.sync();
+  if (tid < 32) {
+    const bool peer = tid < nblocks;
+    const unsigned top = __reduce_max_sync(0xffffffffu, peer ? cl.map_shared_rank(&sh, tid)->row_top : 0u);
+    const unsigned low = __reduce_min_sync(0xffffffffu, peer ? cl.map_shared_rank(&sh, tid)->bound : 0xffffffffu);
+    if (tid == 0) {
+      sh.out_u[0] = top;
+      sh.out_u[1] = low;
+    }
+  }
+  __syncthreads();
+  row.top = unorder(sh.out_u[0]);
+  float bound = unorder(max(sh.out_u[1], kLowest));
   if (row.top == -INFINITY) {
     if (rank == 0 && tid == 0) {
       a.tokens[r] = -1;
@@ -532,177 +989,214 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a,
     cl.sync();   // no CTA leaves while another may read its shared memory
     return;
   }
-  const bool use_k = k_set > 0 && k_set < a.vocab;
-  const bool use_p = !(row.top_p >= 1.f);
-  const bool single = greedy || k_set == 1 || !(row.top_p > 0.f) || !(row.min_p <= 1.f);
+  if (row.top == INFINITY) {
+    sl.infinite = true;
+    row.top = bound = 0.f;
+  }
 
-  double whole = 0;   // sum of all weights
-  if (a.logprobs != nullptr || (!single && use_p && !use_k)) {
-    float s = 0.f;
+  int token = -1;      // in thread 0 of CTA 0
+  double whole = 0;    // sum of all weights, there too
+  const bool want_sum = a.logprobs != nullptr;
+  bool done = false;
+  if (single) {
+    unsigned at = 0xffffffffu;
+    float s[1] = {0.f};
     for (int j = tid; j < sl.chunks; j += kThreads) {
       float x[VE];
       sl.get(j, x);
 #pragma unroll
-      for (int i = 0; i < VE; ++i) s += x[i] == -INFINITY ? 0.f : row.weight(x[i]);
+      for (int i = 0; i < VE; ++i) {
+        if (x[i] == row.top) at = min(at, (unsigned)(sl.index(j) + i));
+        if (want_sum) s[0] += row.weight(x[i]);
+      }
     }
-    double v[1] = {s};
-    cluster_sum(cl, sh, v);
-    whole = v[0];
-  }
-
-  int token = first;
-  if (!single) {
+    const unsigned long long best = block_best(sh, at == 0xffffffffu ? 0ull : pack(1u, at));
+    if (tid == 0) sh.race = best;
+    if (want_sum) block_sum(sh, s);
+    cl.sync();
+    if (rank == 0 && tid < 32) {
+      token = (int)~(uint32_t)all_best(cl, sh);
+      if (want_sum) whole = all_sums(cl, sh, 0);
+    }
+    done = true;
+  } else if (use_list) {
     const float* noise = a.noise + r * a.noise_stride;
-    bool done = false;
-    Cut cut = {0, 0};
-    if (use_k && (k_set + nblocks - 1) / nblocks <= kThreads) {
-      // bound that at least k logits reach
-      uint32_t* maxima = reinterpret_cast<uint32_t*>(list);
-      maxima[tid] = order(mx);
-      sort_down(maxima, kThreads);
-      if (tid == 0) sh.bound = maxima[(k_set + nblocks - 1) / nblocks - 1];
-      cl.sync();
-      uint32_t bound = 0xffffffffu;
-      for (int q = 0; q < nblocks; ++q) bound = min(bound, cl.map_shared_rank(&sh, q)->bound);
-      for (int j = tid; j < sl.chunks; j += kThreads) {
-        float x[VE];
-        sl.get(j, x);
+    float s[1] = {0.f};
+    for (int j = tid; j < sl.chunks; j += kThreads) {
+      if (!want_sum && !(sl.highest(j) >= bound)) continue;
+      float x[VE];
+      sl.get(j, x);
 #pragma unroll
-        for (int i = 0; i < VE; ++i)
-          if (x[i] > -INFINITY && order(x[i]) >= bound) {
-            const unsigned at = atomicAdd(&sh.count, 1u);
-            if (at < kList) list[at] = pack(order(x[i]), sl.index(j) + i);
-          }
-      }
-      cl.sync();
-      unsigned n = 0, before = 0;
-      for (int q = 0; q < nblocks; ++q) {
-        const unsigned c = cl.map_shared_rank(&sh, q)->count;
-        if (q < rank) before += c;
-        n += c;
-      }
-      if (n <= kList) {
-        done = true;
-        if (rank != 0) {   // hand the candidates to CTA 0
-          unsigned long long* to = cl.map_shared_rank(list, 0);
-          for (unsigned i = tid; i < sh.count; i += kThreads) to[before + i] = list[i];
-        }
-        cl.sync();
-        if (rank == 0) {
-          int n2 = 2;
-          while (n2 < (int)n) n2 <<= 1;
-          for (int i = (int)n + tid; i < n2; i += kThreads) list[i] = 0;
-          sort_down(list, n2);
-          const int kept = min((int)n, k_set);
-          constexpr int EACH = kList / kThreads;
-          float w[EACH];
-          double mine = 0;
-#pragma unroll
-          for (int i = 0; i < EACH; ++i) {
-            const int at = tid * EACH + i;
-            w[i] = at < kept ? expf(row.z(unorder((uint32_t)(list[at] >> 32)))) : 0.f;
-            mine += w[i];
-          }
-          double run = block_before(sh, mine);
-          if (tid == kThreads - 1) sh.found_above = run + mine;
-          __syncthreads();
-          const double target = use_p ? (double)row.top_p * sh.found_above : INFINITY;
-          unsigned long long best = 0;
-#pragma unroll
-          for (int i = 0; i < EACH; ++i) {
-            const int at = tid * EACH + i;
-            if (at < kept && (at == 0 || (run < target && w[i] >= row.min_p))) {
-              const float z = row.z(unorder((uint32_t)(list[at] >> 32)));
-              const int id = (int)~(uint32_t)list[at];
-              if (z > -INFINITY) {
-                const unsigned long long v = pack(order(race_score(z, noise[id])), id);
-                best = v > best ? v : best;
-              }
-            }
-            run += w[i];
-          }
-          best = warp_max(best);
-          if ((tid & 31) == 0) sh.best[tid >> 5] = best;
-          __syncthreads();
-          if (tid < 32) {
-            best = warp_max(sh.best[tid]);
-            token = (int)~(uint32_t)best;
-          }
+      for (int i = 0; i < VE; ++i) {
+        if (want_sum) s[0] += row.weight(x[i]);
+        if (x[i] >= bound) {
+          gather(sh, list, x[i], sl.index(j) + i);
+          prefetch_l2(noise + sl.index(j) + i);
         }
       }
     }
-    if (!done) {
-      if (use_k) {
-        const Found f = search<DT, false>(cl, sh, sl, row, (double)k_set, Cut{0, 0});
-        cut.key = f.key;
-        cut.last = 0x7fffffff;
-        if (f.single && f.above + (double)f.count > (double)k_set)
-          cut.last = tie_index(cl, sh, sl, f.key, (unsigned)((double)k_set - f.above));
-      }
-      if (use_p) {
-        double weight = whole;
-        if (use_k) {
-          float s = 0.f;
-          for (int j = tid; j < sl.chunks; j += kThreads) {
-            float x[VE];
-            sl.get(j, x);
+    if (want_sum) block_sum(sh, s);
+    cl.sync();
+    const int n = place_parts(cl, sh);
+    if (n <= kFew) {
+      // CTA 0 counts for each candidate the larger ones and their weight, two threads a
+      // candidate. Weights are whole numbers here, as the candidates come in any order.
+      done = true;
+      if (rank == 0) {
+        if (tid < 32 && want_sum) whole = all_sums(cl, sh, 0);
+        unsigned long long* weights = reinterpret_cast<unsigned long long*>(ahead);
+        __syncthreads();   // part_start
+        const int me = tid >> 1, side = tid & 1;
+        unsigned long long v = 0, w = 0, before = 0;
+        float e = 1.f;
+        if (me < n) {
+          int c = 0;
 #pragma unroll
-            for (int i = 0; i < VE; ++i)
-              if (x[i] > -INFINITY && cut.keeps(order(x[i]), sl.index(j) + i)) s += row.weight(x[i]);
+          for (int q = 1; q < kMaxCluster; ++q) c += me >= sh.part_start[q];
+          v = cl.map_shared_rank(list, c)[me - sh.part_start[c]];
+          w = (unsigned long long)(row.weight(unorder((uint32_t)(v >> 32))) * 0x1p40f);
+          e = noise[(int)~(uint32_t)v];
+          if (side == 0) {
+            list[kFew + me] = v;
+            weights[me] = w;
           }
-          double v[1] = {s};
-          cluster_sum(cl, sh, v);
-          weight = v[0];
-        } else {
-          cut.last = 0x7fffffff;
         }
-        const double target = (double)row.top_p * weight;
+        __syncthreads();
+        int place = 0;
+        if (me < n)
+#pragma unroll 4
+          for (int i = side; i < n; i += 2) {
+            const bool larger = list[kFew + i] > v;
+            place += larger;
+            before += larger ? weights[i] : 0ull;
+          }
+        place += __shfl_xor_sync(0xffffffffu, place, 1);
+        before += __shfl_xor_sync(0xffffffffu, before, 1);
+        const bool in = me < n && place < k_set;
+        bool kept = in;
+        if (use_p) {
+          // all weights of the first k: what is before the last of them, and its own
+          const int last = min(n, k_set) - 1;
+          if (in && place == last && side == 0) sh.out_best = before + w;
+          __syncthreads();
+          kept = in && (double)before < (double)row.top_p * (double)sh.out_best;
+        }
+        const float x = unorder((uint32_t)(v >> 32));
+        if (row.min_p > 0.f) kept = kept && expf(row.z(x)) >= row.min_p;
+        kept = in && (kept || place == 0);
+        unsigned long long best = 0;
+        if (kept && row.z(x) > -INFINITY)
+          best = (unsigned long long)order(race_score(row.z(x), e)) << 32 | (uint32_t)v;
+        token = (int)~(uint32_t)block_best(sh, best);
+      }
+    } else if (n <= kList) {
+      done = true;
+      if (rank == 0 && tid < 32 && want_sum) whole = all_sums(cl, sh, 0);
+      unsigned long long v[4];
+      float w[4], before[4], e[4];
+      int place[4];
+      merge_lists(cl, sh, row, list, ahead, v, w, place, before);
+      const int own = (int)sh.count;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)   // a place past k: not kept
+        e[i] = 4 * tid + i < own && place[i] < k_set ? noise[(int)~(uint32_t)v[i]] : 1.f;
+      float target = INFINITY;
+      if (use_p) {
+        // the weight of the first k: up to the k-th, or all of them
+        float s2[1] = {0.f};
+        double kept[1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s2[0] += 4 * tid + i < own && place[i] < k_set ? w[i] : 0.f;
+        cluster_sum(cl, sh, s2, kept);
+        target = (float)((double)row.top_p * kept[0]);
+      }
+      unsigned long long best = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (4 * tid + i >= own || place[i] >= k_set) continue;
+        if (place[i] > 0 && !(before[i] < target && w[i] >= row.min_p)) continue;
+        const float z = row.z(unorder((uint32_t)(v[i] >> 32)));
+        if (z > -INFINITY)
+          best = max(best, (unsigned long long)order(race_score(z, e[i])) << 32 | (uint32_t)v[i]);
+      }
+      best = block_best(sh, best);
+      if (tid == 0) sh.race = best;
+      cl.sync();
+      if (rank == 0 && tid < 32) token = (int)~(uint32_t)all_best(cl, sh);
+    } else {
+      cl.sync();   // the counts were read
+      if (tid == 0) sh.count = 0;
+      __syncthreads();
+    }
+  }
+  if (!done) {
+    Cut cut = {-kFloatMax, kAnyIndex};
+    bool have_sum = false;
+    if (use_k) {
+      const Found f = search<DT, false>(cl, sh, sl, row, (double)k_set, cut);
+      cut.x = unorder(f.key);
+      if (f.single && f.above + (double)f.count > (double)k_set)
+        cut.last = tie_index(cl, sh, sl, cut.x, (unsigned)((double)k_set - f.above));
+    }
+    if (use_p) {
+      have_sum = !use_k;
+      if (use_k || !nucleus(cl, sh, sl, row, list, ahead, whole, cut)) {
+        // the weight of what is left, by counting
+        cl.sync();
+        sh.hist[tid] = sh.hist[tid + kThreads] = 0;
+        float s[1] = {0.f};
+        for (int j = tid; j < sl.chunks; j += kThreads) {
+          float x[VE];
+          sl.get(j, x);
+#pragma unroll
+          for (int i = 0; i < VE; ++i)
+            if (cut.keeps(x[i], (int)sl.index(j) + i)) s[0] += row.weight(x[i]);
+        }
+        double left[1];
+        cluster_sum(cl, sh, s, left);
+        const double target = (double)row.top_p * left[0];
         const Found f = search<DT, true>(cl, sh, sl, row, target, cut);
-        int last = f.key > cut.key ? 0x7fffffff : cut.last;
-        if (f.single) {
-          const double need = ceil((target - f.above) / (double)row.weight(unorder(f.key)));
-          if (need < (double)f.count) {
-            const int at = tie_index(cl, sh, sl, f.key, (unsigned)max(1.0, need));
-            last = min(last, at);
-          }
+        const float x = fmaxf(unorder(f.key), cut.x);
+        int last = x > cut.x ? kAnyIndex : cut.last;
+        if (f.single && f.count > 0) {
+          const double part = ceil((target - f.above) / (double)row.weight(x));
+          if (part < (double)f.count) last = min(last, tie_index(cl, sh, sl, x, (unsigned)max(1.0, part)));
         }
-        cut.key = f.key;
+        cut.x = x;
         cut.last = last;
       }
-      // the race over what is left
-      const bool all_kept = !use_k && !use_p;
-      float best = -INFINITY;
-      unsigned long long best_key = 0;
-      for (int j = tid; j < sl.chunks; j += kThreads) {
-        float x[VE];
-        sl.get(j, x);
-        const int64_t at = sl.index(j);
-#pragma unroll
-        for (int i = 0; i < VE; ++i) {
-          if (!(x[i] > -INFINITY)) continue;
-          if (!all_kept && !cut.keeps(order(x[i]), at + i)) continue;
-          if (row.min_p > 0.f && at + i != first && !(expf(row.z(x[i])) >= row.min_p)) continue;
-          const float e = noise[at + i];
-          // the exact score only where a near one could win
-          if (row.z_near(x[i]) - __logf(e) < best - 2e-3f) continue;
-          const float z = row.z(x[i]);
-          if (!(z > -INFINITY)) continue;
-          const float s = race_score(z, e);
-          const unsigned long long v = pack(order(s), at + i);
-          if (v > best_key) {
-            best_key = v;
-            best = s;
-          }
-        }
+    }
+    if (row.min_p > 0.f) {
+      const float x = min_p_logit(row);
+      if (x > cut.x) {
+        cut.x = x;
+        cut.last = kAnyIndex;
       }
-      token = (int)~(uint32_t)cluster_max(cl, sh, best_key, &Shared::row_race);
+    }
+    const bool sum_here = want_sum && !have_sum;
+    float s[1] = {0.f};
+    const float* noise = a.noise + r * a.noise_stride;
+    const unsigned long long best_key =
+        cut.x == -kFloatMax && cut.last == kAnyIndex
+            ? race<DT, true>(sh, sl, row, cut, noise, sum_here, s[0])
+            : race<DT, false>(sh, sl, row, cut, noise, sum_here, s[0]);
+    const unsigned long long v = block_best(sh, best_key);
+    if (tid == 0) sh.race = v;
+    if (sum_here) {
+      cl.sync();   // row_sums were read
+      block_sum(sh, s);
+    }
+    cl.sync();
+    if (rank == 0 && tid < 32) {
+      token = (int)~(uint32_t)all_best(cl, sh);
+      if (sum_here) whole = all_sums(cl, sh, 0);
     }
   }
   if (rank == 0 && tid == 0) {
     a.tokens[r] = token;
     if (a.logprobs != nullptr) {
-      const float x = fmaxf(Elem<DT>::to_f(sl.row[token]), -INFINITY) + 0.f;
-      a.logprobs[r] = row.z(x) - (float)log(whole);
+      const float x = sl.infinite ? 0.f : Elem<DT>::to_f(sl.row[token]);
+      a.logprobs[r] = (float)((double)row.z(x) - log(whole));
     }
   }
   cl.sync();
@@ -711,15 +1205,17 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a,
 template <int DT> cudaError_t launch_dt(const SampleArgs& a, int num_sms, cudaStream_t stream) {
   constexpr int VE = Slice<DT>::VE;
   const int64_t chunks = ((int64_t)a.vocab + 2 * VE - 2) / VE;   // of a row at any alignment
-  // the smallest cluster that holds a row, larger while the GPU has CTAs to spare
+  // The smallest cluster that holds a row with two CTAs an SM (one computes while the
+  // other loads), larger while the GPU has room for more CTAs; a row past that is held
+  // by one CTA an SM, or read again each time.
   int n = 1;
-  while (n < kMaxCluster && (chunks + n - 1) / n * 16 > kSliceBytes) n *= 2;
+  while (n < kMaxCluster && (chunks + n - 1) / n * 16 > kSliceTwo) n *= 2;
   while (n < kMaxCluster && (int64_t)a.rows * n * 2 <= num_sms) n *= 2;
   const int64_t per = (chunks + n - 1) / n;
-  const bool held = per * 16 <= kSliceBytes;
-  const int smem = kList * 8 + (held ? (int)per * 16 : 0);
+  const bool held = per * 16 <= kSliceOne;
+  const int smem = kListBytes + (held ? (int)per * 16 : 0);
   cudaError_t e = cudaFuncSetAttribute(sample_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       kList * 8 + kSliceBytes);
+                                       kListBytes + kSliceOne);
   if (e != cudaSuccess) return e;
   if ((int64_t)a.rows * n > 0x7fffffff) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg = {};

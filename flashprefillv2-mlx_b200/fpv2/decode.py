@@ -10,7 +10,8 @@ backward: inputs that require grad are refused while grad mode is on.
 
 from __future__ import annotations
 
-import ctypes
+import functools
+import struct
 
 import torch
 
@@ -20,24 +21,32 @@ DECODE_HEAD_DIMS = (64, 96, 128, 256)
 _HALF = (torch.float16, torch.bfloat16)
 _INT32_MAX = 2**31 - 1
 
+# Stride arrays go to the library as packed bytes. These calls are short on the GPU,
+# so their host side avoids what costs a microsecond: views, ctypes arrays, Stream
+# objects.
+_pack4 = struct.Struct("4q").pack
+_pack6 = struct.Struct("6q").pack
+_pack9 = struct.Struct("9q").pack
 
-def _no_grad(what: str, *tensors: torch.Tensor | None) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError(f"{what} has no backward; call it under torch.no_grad()")
+
+def _refuse_grad(what: str) -> None:
+    raise ValueError(f"{what} has no backward; call it under torch.no_grad()")
 
 
-def _call(name: str, on: torch.Tensor, *args) -> None:
+def _call(fn, on: torch.Tensor, *args) -> None:
     """One library call on ``on``'s device and its current stream."""
-    fn = getattr(_lib.lib(), name)
-    if on.device.index == torch.cuda.current_device():
-        _lib.check(fn(*args, _lib.stream_of(on)))
+    if on.get_device() == torch.cuda.current_device():
+        rc = fn(*args, _lib.stream_of(on))
     else:
         with torch.cuda.device(on.device):
-            _lib.check(fn(*args, _lib.stream_of(on)))
+            rc = fn(*args, _lib.stream_of(on))
+    if rc:
+        _lib.check(rc)
 
 
-def _strides(*values: int):
-    return (ctypes.c_int64 * len(values))(*values)
+@functools.lru_cache(maxsize=None)
+def _workspace_bytes(new: int, q_heads: int, kv_heads: int, dim: int) -> int:
+    return int(_lib.lib().fpv2_decode_workspace_bytes(new, q_heads, kv_heads, dim))
 
 
 def rope_table(positions: int, rotary_dim: int, *, theta: float = 10000.0,
@@ -86,11 +95,12 @@ def qk_norm_rope(
     not written) k and v go into the cache and the returned k is None. Slots must
     not repeat.
     """
-    if q.ndim != 3 or k.ndim != 3:
+    qshape, kshape = q.shape, k.shape
+    if len(qshape) != 3 or len(kshape) != 3:
         raise ValueError("q and k must have shape [tokens, heads, dim]")
-    tokens, q_heads, dim = q.shape
-    kv_heads = k.shape[1]
-    if k.shape[0] != tokens or k.shape[2] != dim:
+    tokens, q_heads, dim = qshape
+    kv_heads = kshape[1]
+    if kshape[0] != tokens or kshape[2] != dim:
         raise ValueError("q and k must have the same tokens and head dimension")
     if not q_heads or not kv_heads:
         raise ValueError("q and k must have heads")
@@ -100,65 +110,75 @@ def qk_norm_rope(
     code = _lib.dtype_code(dtype)
     if k.dtype != dtype:
         raise ValueError("q and k must share their dtype")
-    if positions.ndim != 1 or positions.shape[0] != tokens or positions.dtype not in (torch.int32, torch.int64):
+    wide = positions.dtype == torch.int64
+    if positions.shape != (tokens,) or not (wide or positions.dtype == torch.int32):
         raise ValueError("positions must be an int32 or int64 tensor [tokens]")
     if table.ndim != 2 or table.dtype != torch.float32 or not table.shape[0]:
         raise ValueError("table must be a float32 tensor [positions, rotary_dim]")
-    rotary = table.shape[1]
+    span, rotary = table.shape
     if not rotary or rotary % 2 or rotary > dim:
         raise ValueError("rotary_dim must be even and in [2, head_dim]")
+    tensors = [q, k, positions, table]
     weight_code = code
-    weights = [w for w in (q_weight, k_weight) if w is not None]
-    for w in weights:
-        if w.ndim != 1 or w.shape[0] != dim or w.dtype != weights[0].dtype:
-            raise ValueError("norm weights must share one dtype and have shape [head_dim]")
-        weight_code = _lib.dtype_code(w.dtype)
-    cache = (v, k_cache, v_cache, slots)
+    if q_weight is not None or k_weight is not None:
+        weights = [w for w in (q_weight, k_weight) if w is not None]
+        for w in weights:
+            if w.shape != (dim,) or w.dtype != weights[0].dtype:
+                raise ValueError("norm weights must share one dtype and have shape [head_dim]")
+        weight_code = _lib.dtype_code(weights[0].dtype)
+        tensors += weights
     paged = k_cache is not None
-    if any((x is not None) != paged for x in cache):
+    if (v is not None) != paged or (v_cache is not None) != paged or (slots is not None) != paged:
         raise ValueError("v, k_cache, v_cache and slots go together")
     if paged:
-        if v.shape != k.shape or v.dtype != dtype:
+        if v.shape != kshape or v.dtype != dtype:
             raise ValueError("v must have the shape and dtype of k")
-        for c in (k_cache, v_cache):
-            if c.ndim != 4 or c.shape[2] != kv_heads or c.shape[3] != dim or c.dtype != dtype:
-                raise ValueError("caches must have shape [pages, page_size, kv_heads, dim] and k's dtype")
-            if c.stride(3) != 1 and dim > 1:
-                raise ValueError("a cache's head dimension must be contiguous")
-        if k_cache.shape != v_cache.shape or not k_cache.shape[0] or not k_cache.shape[1]:
+        cshape = k_cache.shape
+        if len(cshape) != 4 or cshape[2] != kv_heads or cshape[3] != dim or k_cache.dtype != dtype \
+                or v_cache.dtype != dtype:
+            raise ValueError("caches must have shape [pages, page_size, kv_heads, dim] and k's dtype")
+        if v_cache.shape != cshape or not cshape[0] or not cshape[1]:
             raise ValueError("k_cache and v_cache must have identical non-empty shapes")
-        if slots.ndim != 1 or slots.shape[0] != tokens or slots.dtype != torch.int64:
+        kc, vc = k_cache.stride(), v_cache.stride()
+        if dim > 1 and (kc[3] != 1 or vc[3] != 1):
+            raise ValueError("a cache's head dimension must be contiguous")
+        if slots.shape != (tokens,) or slots.dtype != torch.int64:
             raise ValueError("slots must be an int64 tensor [tokens]")
-    _no_grad("qk_norm_rope", q, k, table, q_weight, k_weight, *cache)
-    _lib.require_cuda(q, k, positions, table, q_weight, k_weight, *cache)
+        tensors += (v, k_cache, v_cache, slots)
+    if torch.is_grad_enabled() and any([t.requires_grad for t in tensors]):
+        _refuse_grad("qk_norm_rope")
+    device = q.get_device()
+    if device < 0 or any([t.get_device() != device for t in tensors]):
+        _lib.require_cuda(*tensors)
     q, k = _rows(q), _rows(k)
     positions, table = positions.contiguous(), table.contiguous()
     if q_weight is not None:
         q_weight = q_weight.contiguous()
     if k_weight is not None:
         k_weight = k_weight.contiguous()
-    k_out = None
+    qs, ks, vs = q.stride(), k.stride(), (0, 0)
+    k_out = v_ptr = kc_ptr = vc_ptr = slots_ptr = cache_strides = None
+    pages = page_size = 0
     if heads_first:
-        q_out = torch.empty((q_heads, tokens, dim), dtype=dtype, device=q.device)
-        out = [dim, tokens * dim, dim, tokens * dim]
+        q_out = q.new_empty((q_heads, tokens, dim))
+        out = _pack4(dim, tokens * dim, dim, tokens * dim)
     else:
-        q_out = torch.empty((tokens, q_heads, dim), dtype=dtype, device=q.device)
-        out = [q_heads * dim, dim, kv_heads * dim, dim]
-    inn = [q.stride(0), q.stride(1), k.stride(0), k.stride(1), 0, 0]
-    cache_strides, pages, page_size = None, 0, 0
+        q_out = q.new_empty(qshape)
+        out = _pack4(q_heads * dim, dim, kv_heads * dim, dim)
     if paged:
         v, slots = _rows(v), slots.contiguous()
-        inn[4:] = v.stride(0), v.stride(1)
-        pages, page_size = k_cache.shape[:2]
-        cache_strides = _strides(*k_cache.stride()[:3], *v_cache.stride()[:3])
+        vs = v.stride()
+        pages, page_size = cshape[0], cshape[1]
+        cache_strides = _pack6(kc[0], kc[1], kc[2], vc[0], vc[1], vc[2])
+        v_ptr, slots_ptr = v.data_ptr(), slots.data_ptr()
+        kc_ptr, vc_ptr = k_cache.data_ptr(), v_cache.data_ptr()
     else:
-        k_out = torch.empty((kv_heads, tokens, dim) if heads_first else (tokens, kv_heads, dim),
-                            dtype=dtype, device=q.device)
-    _call("fpv2_qk_norm_rope", q, q.data_ptr(), k.data_ptr(), _lib.ptr(v), code, tokens, q_heads, kv_heads,
-          dim, _strides(*inn), positions.data_ptr(), positions.dtype == torch.int64, table.data_ptr(),
-          table.shape[0], rotary, bool(interleaved), _lib.ptr(q_weight), _lib.ptr(k_weight), weight_code,
-          float(eps), q_out.data_ptr(), _lib.ptr(k_out), _strides(*out), _lib.ptr(k_cache),
-          _lib.ptr(v_cache), cache_strides, _lib.ptr(slots), pages, page_size)
+        k_out = q.new_empty((kv_heads, tokens, dim) if heads_first else kshape)
+    _call(_lib.lib().fpv2_qk_norm_rope, q, q.data_ptr(), k.data_ptr(), v_ptr, code, tokens, q_heads,
+          kv_heads, dim, _pack6(qs[0], qs[1], ks[0], ks[1], vs[0], vs[1]), positions.data_ptr(), wide,
+          table.data_ptr(), span, rotary, bool(interleaved), _lib.ptr(q_weight), _lib.ptr(k_weight),
+          weight_code, eps, q_out.data_ptr(), _lib.ptr(k_out), out, kc_ptr, vc_ptr, cache_strides,
+          slots_ptr, pages, page_size)
     return q_out, k_out
 
 
@@ -192,12 +212,13 @@ def decode_attention(
     256, any page size. Returns the output in ``q``'s shape, and with ``return_lse``
     the float32 log-sum-exp of the scaled scores (without the last dimension).
     """
-    if q.ndim not in (3, 4):
+    shape, kshape = q.shape, k_cache.shape
+    if len(shape) == 3:
+        (batch, q_heads, dim), new = shape, 1
+    elif len(shape) == 4:
+        batch, new, q_heads, dim = shape
+    else:
         raise ValueError("q must have shape [batch, heads, dim] or [batch, new, heads, dim]")
-    shape = q.shape
-    q4 = q if q.ndim == 4 else q.unsqueeze(1)
-    batch, new, q_heads, dim = q4.shape
-    kshape = k_cache.shape
     if len(kshape) != 4:
         raise ValueError("k_cache must have shape [pages, page_size, kv_heads, dim]")
     dtype = q.dtype
@@ -214,44 +235,49 @@ def decode_attention(
         raise ValueError("q must hold at least one new token a sequence")
     if not pages or not page_size:
         raise ValueError("the caches are empty")
-    if block_tables.ndim != 2 or block_tables.dtype != torch.int32 or block_tables.shape[0] != batch:
+    tshape = block_tables.shape
+    if len(tshape) != 2 or block_tables.dtype != torch.int32 or tshape[0] != batch:
         raise ValueError("block_tables must be an int32 tensor [batch, max_pages]")
-    if lengths.ndim != 1 or lengths.dtype != torch.int32 or lengths.shape[0] != batch:
+    if lengths.shape != (batch,) or lengths.dtype != torch.int32:
         raise ValueError("lengths must be an int32 tensor [batch]")
-    width = block_tables.shape[1]
+    width = tshape[1]
     if not width:
         raise ValueError("block_tables holds no pages")
     if not (0 <= window <= _INT32_MAX and 0 <= sinks <= _INT32_MAX):
         raise ValueError("window and sinks must be non-negative 32-bit integers")
-    _no_grad("decode_attention", q, k_cache, v_cache)
-    _lib.require_cuda(q, k_cache, v_cache, block_tables, lengths)
-    out = torch.empty((batch, new, q_heads, dim), dtype=dtype, device=q.device)
-    lse = torch.empty((batch, new, q_heads), dtype=torch.float32, device=q.device) if return_lse else None
+    if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
+        _refuse_grad("decode_attention")
+    device = q.get_device()
+    if device < 0 or k_cache.get_device() != device or v_cache.get_device() != device \
+            or block_tables.get_device() != device or lengths.get_device() != device:
+        _lib.require_cuda(q, k_cache, v_cache, block_tables, lengths)
+    out = q.new_empty(shape)
+    lse = q.new_empty(shape[:-1], dtype=torch.float32) if return_lse else None
     if batch:
-        qs, ks, vs = q4.stride(), k_cache.stride(), v_cache.stride()
-        if qs[3] != 1 or (qs[0] | qs[1] | qs[2]) & 1 or q4.data_ptr() & 3:
-            q4 = q4.clone(memory_format=torch.contiguous_format)
-            qs = q4.stride()
+        qs, ks, vs = q.stride(), k_cache.stride(), v_cache.stride()
+        if qs[-1] != 1 or any([x & 1 for x in qs[:-1]]) or q.data_ptr() & 3:
+            q = q.clone(memory_format=torch.contiguous_format)
+            qs = q.stride()
         if ks[3] != 1 or vs[3] != 1:
             raise ValueError("a cache's head dimension must be contiguous")
         if block_tables.stride(1) != 1:
             block_tables = block_tables.contiguous()
         lengths = lengths.contiguous()
-        nbytes = _lib.lib().fpv2_decode_workspace_bytes(new, q_heads, kv_heads, dim)
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-        _call("fpv2_decode_attention", q4, q4.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+        nbytes = _workspace_bytes(new, q_heads, kv_heads, dim)
+        workspace = q.new_empty(nbytes, dtype=torch.uint8)
+        token_stride = qs[1] if len(shape) == 4 else 0
+        _call(_lib.lib().fpv2_decode_attention, q, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
               _lib.dtype_code(dtype), batch, new, q_heads, kv_heads, dim,
-              _strides(*qs[:3], *ks[:3], *vs[:3]), block_tables.data_ptr(), block_tables.stride(0), width,
-              lengths.data_ptr(), pages, page_size, float(scale), window, sinks, out.data_ptr(), _lib.ptr(lse),
-              workspace.data_ptr(), nbytes)
-    out = out.view(shape)
-    return (out, lse.view(shape[:-1])) if return_lse else out
+              _pack9(qs[0], token_stride, qs[-2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2]),
+              block_tables.data_ptr(), block_tables.stride(0), width, lengths.data_ptr(), pages, page_size,
+              scale, window, sinks, out.data_ptr(), _lib.ptr(lse), workspace.data_ptr(), nbytes)
+    return (out, lse) if return_lse else out
 
 
 def _setting(value, name: str, dtype: torch.dtype, rows: int, plain: float):
     """(tensor, scalar) of a per-row or common setting."""
     if isinstance(value, torch.Tensor):
-        if value.ndim != 1 or value.shape[0] != rows or value.dtype != dtype:
+        if value.shape != (rows,) or value.dtype != dtype:
             raise ValueError(f"{name} must be a number or a {dtype} tensor [rows]")
         return value.contiguous(), plain
     return None, value
@@ -282,7 +308,7 @@ def sample_tokens(
     ``return_logprobs`` also float32 ``[rows]``: the token's log-probability under
     ``softmax(x / T)`` over the whole row (``T = 1`` where ``T <= 0``).
     """
-    if logits.ndim != 2 or noise.ndim != 2 or logits.shape != noise.shape:
+    if logits.ndim != 2 or logits.shape != noise.shape:
         raise ValueError("logits and noise must have the same shape [rows, vocab]")
     rows, vocab = logits.shape
     if not vocab:
@@ -296,12 +322,16 @@ def sample_tokens(
     least, least_all = _setting(min_p, "min_p", torch.float32, rows, 0.0)
     if not -_INT32_MAX <= k_all <= _INT32_MAX:
         raise ValueError("top_k must be a 32-bit integer")
-    _no_grad("sample_tokens", logits)
-    _lib.require_cuda(logits, noise, heat, k, p, least)
+    if logits.requires_grad and torch.is_grad_enabled():
+        _refuse_grad("sample_tokens")
+    device = logits.get_device()
+    if device < 0 or any([t is not None and t.get_device() != device for t in (noise, heat, k, p, least)]):
+        _lib.require_cuda(logits, noise, heat, k, p, least)
     logits, noise = _rows(logits), _rows(noise)
-    tokens = torch.empty(rows, dtype=torch.int64, device=logits.device)
-    logprobs = torch.empty(rows, dtype=torch.float32, device=logits.device) if return_logprobs else None
-    _call("fpv2_sample_tokens", logits, logits.data_ptr(), code, rows, vocab, logits.stride(0),
-          noise.data_ptr(), noise.stride(0), _lib.ptr(heat), float(heat_all), _lib.ptr(k), int(k_all),
-          _lib.ptr(p), float(p_all), _lib.ptr(least), float(least_all), tokens.data_ptr(), _lib.ptr(logprobs))
+    tokens = logits.new_empty(rows, dtype=torch.int64)
+    logprobs = logits.new_empty(rows, dtype=torch.float32) if return_logprobs else None
+    ptr = _lib.ptr
+    _call(_lib.lib().fpv2_sample_tokens, logits, logits.data_ptr(), code, rows, vocab, logits.stride(0),
+          noise.data_ptr(), noise.stride(0), ptr(heat), heat_all, ptr(k), int(k_all), ptr(p), p_all,
+          ptr(least), least_all, tokens.data_ptr(), ptr(logprobs))
     return (tokens, logprobs) if return_logprobs else tokens
