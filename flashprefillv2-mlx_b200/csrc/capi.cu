@@ -113,6 +113,17 @@ size_t dt_size(int dt) { return dt == DT_F32 ? 4 : 2; }
 
 }  // namespace
 
+cudaError_t allow_shared(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = 1ull << (dev & (kMaxDevices - 1));
+  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
+
 int current_launch(TcLaunch* out) {
   DeviceInfo* d = nullptr;
   const int rc = device_info(&d);

@@ -634,7 +634,8 @@ cudaError_t launch_join(const DecodeArgs& a, int parts, cudaStream_t stream) {
 template <int DT, int D, int NB> cudaError_t launch_blocks(const DecodeArgs& a, cudaStream_t stream) {
   constexpr int NW = Shape<D>::NW, SMEM = NW * Shape<D>::ST * kStageBytes<D>;
   const int cols = a.Hkv * row_groups(a.G * a.T, D), parts = parts_for<D>(cols);
-  cudaError_t e = cudaFuncSetAttribute(decode_kernel<DT, D, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+  static std::atomic<uint64_t> allowed{0};
+  cudaError_t e = allow_shared(reinterpret_cast<const void*>(decode_kernel<DT, D, NB>), SMEM, allowed);
   if (e != cudaSuccess) return e;
   const int64_t blocks = ((int64_t)parts * cols + NW - 1) / NW;
   if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;

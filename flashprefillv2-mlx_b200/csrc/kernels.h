@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace fpv2 {
 
 // ---- pooling (pool.cu) ----------------------------------------------------
@@ -236,6 +238,10 @@ struct SampleArgs {
   float* logprobs;            // nullable [rows]
 };
 cudaError_t launch_sample(const SampleArgs& a, int dt, int num_sms, cudaStream_t stream);
+
+// Lets `kernel` use `bytes` of dynamic shared memory on the current device; `done` is
+// the caller's record (one bit a device) of where that was set before.
+cudaError_t allow_shared(const void* kernel, int bytes, std::atomic<uint64_t>& done);
 
 // The current device's launch record, or an FPV2_ERR_* code (capi.cu).
 int current_launch(TcLaunch* out);

@@ -166,16 +166,24 @@ struct Shared {
   unsigned long long warp_best[kWarps];
   double sums[kWarps][4];
   double scan[kWarps];
+  unsigned count;
   // written by this CTA, read by the cluster
-  unsigned long long race;
   double row_sums[4];
-  unsigned row_top, bound, count, ties;
+  unsigned ties;
   float part_weight;
+  // written by each CTA of the cluster, in its place
+  unsigned long long least_of[kMaxCluster];
+  unsigned top_of[kMaxCluster], bound_of[kMaxCluster], count_of[kMaxCluster];
+  // in CTA 0: the best token and the sum of each CTA of the cluster
+  unsigned long long best_of[kMaxCluster];
+  double sum_of[kMaxCluster];
+  // written by one CTA for all
+  double share;
   // broadcast inside the CTA
   unsigned long long out_best;
   double out_sums[4];
   double found_above;
-  unsigned found_bin, found_count, out_u[2];
+  unsigned found_bin, found_count;
   int part_start[kMaxCluster + 1];     // of each CTA's candidates in a merged list
   float part_total[kMaxCluster];       // and their weight
   int tie_last;
@@ -201,8 +209,9 @@ __device__ unsigned long long block_best(Shared& sh, unsigned long long v) {
   return v;
 }
 
-// Sums of N values over the CTA into row_sums, in a fixed order (no barrier after).
-template <int N> __device__ void block_sum(Shared& sh, const float (&x)[N]) {
+// Sums of N values over the CTA into row_sums from `slot`, in a fixed order (no barrier
+// after; thread 0 may use them).
+template <int N> __device__ void block_sum(Shared& sh, const float (&x)[N], int slot = 0) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   __syncthreads();
 #pragma unroll
@@ -219,7 +228,7 @@ template <int N> __device__ void block_sum(Shared& sh, const float (&x)[N]) {
       double v = lane < kWarps ? sh.sums[lane][i] : 0.0;
 #pragma unroll
       for (int o = kWarps / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      if (lane == 0) sh.row_sums[i] = v;
+      if (lane == 0) sh.row_sums[slot + i] = v;
     }
   }
 }
@@ -231,12 +240,6 @@ __device__ __forceinline__ double all_sums(cg::cluster_group& cl, Shared& sh, in
 #pragma unroll
   for (int o = 1; o < kMaxCluster; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   return __shfl_sync(0xffffffffu, s, 0);
-}
-
-// The best `race` of the cluster's CTAs; a warp calls it.
-__device__ __forceinline__ unsigned long long all_best(cg::cluster_group& cl, Shared& sh) {
-  const unsigned lane = threadIdx.x & 31;
-  return warp_best(lane < cl.num_blocks() ? cl.map_shared_rank(&sh, lane)->race : 0ull);
 }
 
 // Sums of N values over the cluster, in every thread.
@@ -344,11 +347,15 @@ __device__ void sort_down(unsigned long long* v, int n, unsigned long long (&x)[
   }
 }
 
-// Where each CTA's candidates start in a list of all of them, into part_start; returns
-// their number, the same in every thread of the cluster.
+// Once a CTA's candidates are gathered: tells the others their number and waits for
+// the cluster, then sets part_start to where each CTA's start in a list of all of them;
+// returns the number of all, the same in every thread of the cluster.
 __device__ int place_parts(cg::cluster_group& cl, Shared& sh) {
   const int lane = threadIdx.x & 31, nblocks = (int)cl.num_blocks();
-  const int c = lane < nblocks ? (int)cl.map_shared_rank(&sh, lane)->count : 0;
+  __syncthreads();
+  if ((int)threadIdx.x < nblocks) cl.map_shared_rank(&sh, threadIdx.x)->count_of[cl.block_rank()] = sh.count;
+  cl.sync();
+  const int c = lane < nblocks ? (int)sh.count_of[lane] : 0;
   int upto = c;
 #pragma unroll
   for (int o = 1; o < kMaxCluster; o <<= 1) {
@@ -360,34 +367,47 @@ __device__ int place_parts(cg::cluster_group& cl, Shared& sh) {
   return __shfl_sync(0xffffffffu, upto, kMaxCluster - 1);
 }
 
-// Sorts a CTA's candidates and finds their places among the whole cluster's (descending,
-// ties by index ascending): on return thread i has the CTA's candidates 4 i to 4 i + 3 in
-// v, their weights in w, the number of larger candidates in rank and their weight in
-// before. Every CTA sorts its own and copies the others' sorted ones with their running
-// weights, where a binary search gives a candidate's place. All CTAs call it, after
-// place_parts().
+// Sorts the cluster's candidates: afterwards every CTA has all of them, each CTA's part
+// (from part_start) sorted (descending, ties by index ascending) with the running weight
+// of the part before each. All CTAs call it, after place_parts().
 __device__ void merge_lists(cg::cluster_group& cl, Shared& sh, const RowState& row, unsigned long long* list,
-                            float* ahead, unsigned long long (&v)[4], float (&w)[4], int (&rank)[4],
-                            float (&before)[4]) {
+                            float* ahead) {
   const int tid = threadIdx.x, me = (int)cl.block_rank(), nblocks = (int)cl.num_blocks();
   __syncthreads();
   const int start = sh.part_start[me], own = sh.part_start[me + 1] - start;
-  sort_down(list, own, v);
+  unsigned long long v[4];
+  if (own <= kFew / 2) {   // four threads a candidate count the larger ones
+    const int i = tid >> 2;
+    v[0] = i < own ? list[i] : 0;
+    int place = 0;
+    if (i < own)
+      for (int j = tid & 3; j < own; j += 4) place += list[j] > v[0];
+    place += __shfl_xor_sync(0xffffffffu, place, 1);
+    place += __shfl_xor_sync(0xffffffffu, place, 2);
+    __syncthreads();
+    if (i < own && (tid & 3) == 0) list[start + place] = v[0];
+  } else {
+    sort_down(list, own, v);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (4 * tid + i < own) list[start + 4 * tid + i] = v[i];
+  }
+  __syncthreads();
+  const int each = (own + kThreads - 1) / kThreads;   // at most 4
+  float w[4];
   double mine = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    w[i] = 4 * tid + i < own ? row.weight(unorder((uint32_t)(v[i] >> 32))) : 0.f;
+    const int at = each * tid + i;
+    w[i] = i < each && at < own ? row.weight(unorder((uint32_t)(list[start + at] >> 32))) : 0.f;
     mine += w[i];
   }
-  double run = block_before(sh, mine);   // its barriers also end the reads of the unsorted list
+  double run = block_before(sh, mine);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    rank[i] = 4 * tid + i;
-    before[i] = (float)run;
-    if (4 * tid + i < own) {
-      list[start + 4 * tid + i] = v[i];
-      ahead[start + 4 * tid + i] = (float)run;
-    }
+    const int at = each * tid + i;
+    if (i < each && at < own) ahead[start + at] = (float)run;
     run += w[i];
   }
   if (tid == kThreads - 1) sh.part_weight = (float)run;
@@ -404,31 +424,43 @@ __device__ void merge_lists(cg::cluster_group& cl, Shared& sh, const RowState& r
   }
   if (tid < nblocks) sh.part_total[tid] = cl.map_shared_rank(&sh, tid)->part_weight;
   __syncthreads();
-  if (4 * tid >= own) return;
-  for (int c = 0; c < nblocks; ++c) {
-    if (c == me) continue;
-    const int s0 = sh.part_start[c], n = sh.part_start[c + 1] - s0;
-    if (n == 0) continue;
-    int lo[4] = {0, 0, 0, 0};   // known to be larger
-    for (int step = 1 << (31 - __clz(n)); step > 0; step >>= 1) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int to = lo[i] + step;
-        const bool larger = list[s0 + min(to, n) - 1] > v[i];
-        lo[i] = to <= n && larger ? to : lo[i];
-      }
+}
+
+// Calls each(place in this CTA's part, candidate, number of larger ones, their weight) for
+// this CTA's candidates after merge_lists(), each by one thread: as many lanes as the
+// cluster has CTAs share a candidate and search a part each.
+template <typename F>
+__device__ __forceinline__ void for_places(Shared& sh, const unsigned long long* list, const float* ahead, int me,
+                                           int nblocks, const F& each) {
+  const int start = sh.part_start[me], own = sh.part_start[me + 1] - start;
+  const int c = threadIdx.x & (nblocks - 1);   // a power of two
+  const int s0 = sh.part_start[c], n = sh.part_start[c + 1] - s0;
+  const int per = kThreads / nblocks;
+  for (int i0 = 0; i0 < own; i0 += per) {
+    const int i = i0 + (int)threadIdx.x / nblocks;
+    const unsigned long long v = i < own ? list[start + i] : ~0ull;
+    int lo = 0;   // known to be larger
+    for (int step = n > 0 ? 1 << (31 - __clz(n)) : 0; step > 0; step >>= 1) {
+      const int to = lo + step;
+      lo = to <= n && list[s0 + min(to, n) - 1] > v ? to : lo;
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      rank[i] += lo[i];
-      before[i] += lo[i] < n ? ahead[s0 + lo[i]] : sh.part_total[c];
+    float before = n == 0 ? 0.f : lo < n ? ahead[s0 + lo] : sh.part_total[c];
+    for (int o = 1; o < nblocks; o <<= 1) {
+      lo += __shfl_xor_sync(0xffffffffu, lo, o);
+      before += __shfl_xor_sync(0xffffffffu, before, o);
     }
+    if (c == 0 && i < own) each(i, v, lo, before);
   }
 }
 
 __device__ __forceinline__ void gather(Shared& sh, unsigned long long* list, float x, int64_t at) {
   const unsigned i = atomicAdd(&sh.count, 1u);
   if (i < kList) list[i] = pack(order(x), at);
+}
+
+// Starts bringing `bytes` from p (both multiples of 16) into L2.
+__device__ __forceinline__ void prefetch_l2_bulk(const void* p, unsigned bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
 }
 
 __device__ __forceinline__ void prefetch_l2(const void* p) {
@@ -729,28 +761,23 @@ __device__ bool nucleus(cg::cluster_group& cl, Shared& sh, const Slice<DT>& sl, 
         if (p == at_bin) gather(sh, list, x[i], sl.index(j) + i);
       }
     }
-    cl.sync();   // row_sums, race and the lists of the last try were read
-    block_sum(sh, a);
-    cl.sync();
+    const int slot = 1 + (tries & 1);   // the other one may still be read
+    block_sum(sh, a, slot);
     const int n = place_parts(cl, sh);
     if (n > kList) return false;
-    const double above = all_sums(cl, sh, 0);
-    unsigned long long v[4];
-    float w[4], before[4];
-    int rank[4];
-    merge_lists(cl, sh, row, list, ahead, v, w, rank, before);
-    const int own = (int)sh.count;
+    const double above = all_sums(cl, sh, slot);
+    merge_lists(cl, sh, row, list, ahead);
     // the last one that the prefix has to take: the smallest with less than the target before it
     unsigned long long least = 0;   // inverted, so that the smallest is the best
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (4 * tid + i < own && above + before[i] < target) least = max(least, ~v[i]);
-    least = block_best(sh, least);
-    if (tid == 0) sh.race = least;
+    for_places(sh, list, ahead, (int)cl.block_rank(), (int)cl.num_blocks(), [&](int, unsigned long long v, int, float before) {
+      if (above + before < target) least = max(least, ~v);
+    });
+    least = __shfl_sync(0xffffffffu, block_best(sh, least), 0);
+    if (tid < (int)cl.num_blocks()) cl.map_shared_rank(&sh, tid)->least_of[cl.block_rank()] = least;
     double total = above;
     for (unsigned r = 0; r < cl.num_blocks(); ++r) total += sh.part_total[r];
     cl.sync();
-    least = all_best(cl, sh);
+    least = warp_best((tid & 31) < (int)cl.num_blocks() ? sh.least_of[tid & 31] : 0ull);
     if (tid == 0) sh.count = 0;
     __syncthreads();
     // The estimate of the bin is off by a rounding at most, so a step that would turn back
@@ -874,6 +901,20 @@ __device__ __forceinline__ unsigned long long race(Shared& sh, const Slice<DT>& 
   return best_key;
 }
 
+// Hands a CTA's best token and its part of the sum (thread 0's) to CTA 0. True for the
+// other CTAs, which have arrived and may leave: nothing of theirs is read after this.
+__device__ __forceinline__ bool leave(cg::cluster_group& cl, Shared& sh, unsigned long long best, double part) {
+  if (threadIdx.x == 0) {
+    Shared* to = cl.map_shared_rank(&sh, 0);
+    to->best_of[cl.block_rank()] = best;
+    to->sum_of[cl.block_rank()] = part;
+  }
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  if (cl.block_rank() != 0) return true;
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+  return false;
+}
+
 template <int DT>
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a, int per) {
   using T = typename Elem<DT>::T;
@@ -886,6 +927,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a,
   unsigned long long* list = reinterpret_cast<unsigned long long*>(dyn);
   float* ahead = reinterpret_cast<float*>(dyn + kList * 8);
   uint4* held = reinterpret_cast<uint4*>(dyn + kListBytes);
+
+  // (with the wait below: every CTA of the cluster runs before its shared memory is written)
+  asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
 
   Slice<DT> sl;
   sl.row = reinterpret_cast<const T*>(a.logits) + r * a.logits_stride;
@@ -926,6 +970,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a,
   const bool single = greedy || k_set == 1 || !(row.top_p > 0.f) || !(row.min_p <= 1.f);
   const int need = (k_set + nblocks - 1) / nblocks;
   const bool use_list = !single && use_k && need <= kThreads;
+  const float* noise = a.noise + r * a.noise_stride;
+  if (!single && !use_k) {
+    // much or all of the noise is going to be read, after the logits were looked at
+    const int64_t n0 = max((int64_t)0, sl.first), n1 = min((int64_t)a.vocab, sl.index(sl.chunks));
+    const uintptr_t p0 = (reinterpret_cast<uintptr_t>(noise + n0) + 15) / 16 * 16;
+    const uintptr_t p1 = reinterpret_cast<uintptr_t>(noise + n1) / 16 * 16;
+    const uintptr_t p = p0 + (uintptr_t)tid * 2048;
+    if (p < p1) prefetch_l2_bulk(reinterpret_cast<const void*>(p), (unsigned)min((uintptr_t)2048, p1 - p));
+  }
   sh.hist[tid] = sh.hist[tid + kThreads] = 0;
   if (tid == 0) sh.count = 0;
   // A thread reads back its own chunks only, here and below, but for tie_index().
@@ -933,6 +986,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a,
 
   // the largest logit, and for top-k the CTA's bound: bit by bit from the top, 16 bits
   // bound it closely enough
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
   uint32_t* maxima = reinterpret_cast<uint32_t*>(list);
   maxima[tid] = order(sl.largest());
   __syncthreads();
@@ -963,30 +1017,25 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a,
         for (int i = 0; i < kWarps; ++i) c += m[i] >= trial;
         if (__reduce_add_sync(0xffffffffu, c) >= need) low = trial;
       }
-    if (tid == 0) {
-      sh.row_top = v;
-      sh.bound = low & 0xFFFF0000u;
+    if (tid < nblocks) {
+      Shared* to = cl.map_shared_rank(&sh, tid);
+      to->top_of[rank] = v;
+      to->bound_of[rank] = low & 0xFFFF0000u;
     }
   }
   cl.sync();
-  if (tid < 32) {
-    const bool peer = tid < nblocks;
-    const unsigned top = __reduce_max_sync(0xffffffffu, peer ? cl.map_shared_rank(&sh, tid)->row_top : 0u);
-    const unsigned low = __reduce_min_sync(0xffffffffu, peer ? cl.map_shared_rank(&sh, tid)->bound : 0xffffffffu);
-    if (tid == 0) {
-      sh.out_u[0] = top;
-      sh.out_u[1] = low;
-    }
+  uint32_t top = 0, low = 0xffffffffu;
+  for (int q = 0; q < nblocks; ++q) {
+    top = max(top, sh.top_of[q]);
+    low = min(low, sh.bound_of[q]);
   }
-  __syncthreads();
-  row.top = unorder(sh.out_u[0]);
-  float bound = unorder(max(sh.out_u[1], kLowest));
+  row.top = unorder(top);
+  float bound = unorder(max(low, kLowest));
   if (row.top == -INFINITY) {
     if (rank == 0 && tid == 0) {
       a.tokens[r] = -1;
       if (a.logprobs != nullptr) a.logprobs[r] = -INFINITY;
     }
-    cl.sync();   // no CTA leaves while another may read its shared memory
     return;
   }
   if (row.top == INFINITY) {
@@ -994,8 +1043,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a,
     row.top = bound = 0.f;
   }
 
-  int token = -1;      // in thread 0 of CTA 0
-  double whole = 0;    // sum of all weights, there too
+  // Each path leaves the CTA's best token (as pack() has it) and its part of the sum of
+  // all weights in thread 0.
+  unsigned long long best = 0;
+  double part = 0;
   const bool want_sum = a.logprobs != nullptr;
   bool done = false;
   if (single) {
@@ -1010,17 +1061,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a,
         if (want_sum) s[0] += row.weight(x[i]);
       }
     }
-    const unsigned long long best = block_best(sh, at == 0xffffffffu ? 0ull : pack(1u, at));
-    if (tid == 0) sh.race = best;
+    best = block_best(sh, at == 0xffffffffu ? 0ull : pack(1u, at));
     if (want_sum) block_sum(sh, s);
-    cl.sync();
-    if (rank == 0 && tid < 32) {
-      token = (int)~(uint32_t)all_best(cl, sh);
-      if (want_sum) whole = all_sums(cl, sh, 0);
-    }
+    part = sh.row_sums[0];
     done = true;
   } else if (use_list) {
-    const float* noise = a.noise + r * a.noise_stride;
     float s[1] = {0.f};
     for (int j = tid; j < sl.chunks; j += kThreads) {
       if (!want_sum && !(sl.highest(j) >= bound)) continue;
@@ -1036,93 +1081,85 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a,
       }
     }
     if (want_sum) block_sum(sh, s);
-    cl.sync();
+    part = sh.row_sums[0];
     const int n = place_parts(cl, sh);
     if (n <= kFew) {
-      // CTA 0 counts for each candidate the larger ones and their weight, two threads a
-      // candidate. Weights are whole numbers here, as the candidates come in any order.
+      // CTA 0 alone: it gets the candidates and counts for each the larger ones and their
+      // weight, two threads a candidate. Weights are whole numbers here, as the
+      // candidates come in any order.
       done = true;
-      if (rank == 0) {
-        if (tid < 32 && want_sum) whole = all_sums(cl, sh, 0);
-        unsigned long long* weights = reinterpret_cast<unsigned long long*>(ahead);
-        __syncthreads();   // part_start
-        const int me = tid >> 1, side = tid & 1;
-        unsigned long long v = 0, w = 0, before = 0;
-        float e = 1.f;
-        if (me < n) {
-          int c = 0;
-#pragma unroll
-          for (int q = 1; q < kMaxCluster; ++q) c += me >= sh.part_start[q];
-          v = cl.map_shared_rank(list, c)[me - sh.part_start[c]];
-          w = (unsigned long long)(row.weight(unorder((uint32_t)(v >> 32))) * 0x1p40f);
-          e = noise[(int)~(uint32_t)v];
-          if (side == 0) {
-            list[kFew + me] = v;
-            weights[me] = w;
-          }
-        }
-        __syncthreads();
-        int place = 0;
-        if (me < n)
-#pragma unroll 4
-          for (int i = side; i < n; i += 2) {
-            const bool larger = list[kFew + i] > v;
-            place += larger;
-            before += larger ? weights[i] : 0ull;
-          }
-        place += __shfl_xor_sync(0xffffffffu, place, 1);
-        before += __shfl_xor_sync(0xffffffffu, before, 1);
-        const bool in = me < n && place < k_set;
-        bool kept = in;
-        if (use_p) {
-          // all weights of the first k: what is before the last of them, and its own
-          const int last = min(n, k_set) - 1;
-          if (in && place == last && side == 0) sh.out_best = before + w;
-          __syncthreads();
-          kept = in && (double)before < (double)row.top_p * (double)sh.out_best;
-        }
-        const float x = unorder((uint32_t)(v >> 32));
-        if (row.min_p > 0.f) kept = kept && expf(row.z(x)) >= row.min_p;
-        kept = in && (kept || place == 0);
-        unsigned long long best = 0;
-        if (kept && row.z(x) > -INFINITY)
-          best = (unsigned long long)order(race_score(row.z(x), e)) << 32 | (uint32_t)v;
-        token = (int)~(uint32_t)block_best(sh, best);
+      __syncthreads();   // part_start
+      unsigned long long* to = cl.map_shared_rank(list + kFew, 0);
+      for (int i = tid; i < (int)sh.count; i += kThreads) to[sh.part_start[rank] + i] = list[i];
+      if (leave(cl, sh, 0, part)) return;
+      unsigned long long* weights = reinterpret_cast<unsigned long long*>(ahead);
+      const int me = tid >> 1, side = tid & 1;
+      unsigned long long v = 0, w = 0, before = 0;
+      float e = 1.f;
+      if (me < n) {
+        v = list[kFew + me];
+        w = (unsigned long long)(row.weight(unorder((uint32_t)(v >> 32))) * 0x1p40f);
+        e = noise[(int)~(uint32_t)v];
+        if (side == 0) weights[me] = w;
       }
+      __syncthreads();
+      int place = 0;
+      if (me < n)
+#pragma unroll 4
+        for (int i = side; i < n; i += 2) {
+          const bool larger = list[kFew + i] > v;
+          place += larger;
+          before += larger ? weights[i] : 0ull;
+        }
+      place += __shfl_xor_sync(0xffffffffu, place, 1);
+      before += __shfl_xor_sync(0xffffffffu, before, 1);
+      const bool in = me < n && place < k_set;
+      bool kept = in;
+      if (use_p) {
+        // the weight of the first k: what is before the last of them, and its own
+        const int last = min(n, k_set) - 1;
+        if (in && place == last && side == 0) sh.out_best = before + w;
+        __syncthreads();
+        kept = in && (double)before < (double)row.top_p * (double)sh.out_best;
+      }
+      const float z = row.z(unorder((uint32_t)(v >> 32)));
+      if (row.min_p > 0.f) kept = kept && expf(z) >= row.min_p;
+      kept = in && (kept || place == 0);
+      best = block_best(sh, kept && z > -INFINITY ? (unsigned long long)order(race_score(z, e)) << 32 | (uint32_t)v
+                                                  : 0ull);
+      if (tid == 0) sh.best_of[0] = best;
     } else if (n <= kList) {
       done = true;
-      if (rank == 0 && tid < 32 && want_sum) whole = all_sums(cl, sh, 0);
-      unsigned long long v[4];
-      float w[4], before[4], e[4];
-      int place[4];
-      merge_lists(cl, sh, row, list, ahead, v, w, place, before);
-      const int own = (int)sh.count;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)   // a place past k: not kept
-        e[i] = 4 * tid + i < own && place[i] < k_set ? noise[(int)~(uint32_t)v[i]] : 1.f;
+      merge_lists(cl, sh, row, list, ahead);
       float target = INFINITY;
       if (use_p) {
-        // the weight of the first k: up to the k-th, or all of them
-        float s2[1] = {0.f};
-        double kept[1];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s2[0] += 4 * tid + i < own && place[i] < k_set ? w[i] : 0.f;
-        cluster_sum(cl, sh, s2, kept);
-        target = (float)((double)row.top_p * kept[0]);
+        // the weight of the first k: what is before the last of them, and its own
+        const int last = min(n, k_set) - 1;
+        for_places(sh, list, ahead, rank, nblocks, [&](int, unsigned long long v, int place, float before) {
+          if (place != last) return;
+          const double share = (double)before + (double)row.weight(unorder((uint32_t)(v >> 32)));
+          for (int q = 0; q < nblocks; ++q) cl.map_shared_rank(&sh, q)->share = share;
+        });
+        cl.sync();
+        target = (float)((double)row.top_p * sh.share);
       }
-      unsigned long long best = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (4 * tid + i >= own || place[i] >= k_set) continue;
-        if (place[i] > 0 && !(before[i] < target && w[i] >= row.min_p)) continue;
-        const float z = row.z(unorder((uint32_t)(v[i] >> 32)));
-        if (z > -INFINITY)
-          best = max(best, (unsigned long long)order(race_score(z, e[i])) << 32 | (uint32_t)v[i]);
+      // which are kept, then their race with all noise loads in flight at once
+      unsigned char* kept = reinterpret_cast<unsigned char*>(sh.hist);
+      for_places(sh, list, ahead, rank, nblocks, [&](int i, unsigned long long v, int place, float before) {
+        const float z = row.z(unorder((uint32_t)(v >> 32)));
+        kept[i] = place < k_set && z > -INFINITY && (place == 0 || (before < target && expf(z) >= row.min_p));
+      });
+      __syncthreads();
+      const int start = sh.part_start[rank], own = sh.part_start[rank + 1] - start;
+      for (int i = tid; i < own; i += kThreads) {
+        if (!kept[i]) continue;
+        const unsigned long long v = list[start + i];
+        const float score = race_score(row.z(unorder((uint32_t)(v >> 32))), noise[(int)~(uint32_t)v]);
+        best = max(best, (unsigned long long)order(score) << 32 | (uint32_t)v);
       }
       best = block_best(sh, best);
-      if (tid == 0) sh.race = best;
-      cl.sync();
-      if (rank == 0 && tid < 32) token = (int)~(uint32_t)all_best(cl, sh);
+      cl.sync();   // the lists and part weights were read
+      if (leave(cl, sh, best, part)) return;
     } else {
       cl.sync();   // the counts were read
       if (tid == 0) sh.count = 0;
@@ -1132,6 +1169,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a,
   if (!done) {
     Cut cut = {-kFloatMax, kAnyIndex};
     bool have_sum = false;
+    double whole = 0;
     if (use_k) {
       const Found f = search<DT, false>(cl, sh, sl, row, (double)k_set, cut);
       cut.x = unorder(f.key);
@@ -1175,31 +1213,30 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a,
     }
     const bool sum_here = want_sum && !have_sum;
     float s[1] = {0.f};
-    const float* noise = a.noise + r * a.noise_stride;
-    const unsigned long long best_key =
-        cut.x == -kFloatMax && cut.last == kAnyIndex
-            ? race<DT, true>(sh, sl, row, cut, noise, sum_here, s[0])
-            : race<DT, false>(sh, sl, row, cut, noise, sum_here, s[0]);
-    const unsigned long long v = block_best(sh, best_key);
-    if (tid == 0) sh.race = v;
-    if (sum_here) {
-      cl.sync();   // row_sums were read
-      block_sum(sh, s);
-    }
-    cl.sync();
-    if (rank == 0 && tid < 32) {
-      token = (int)~(uint32_t)all_best(cl, sh);
-      if (sum_here) whole = all_sums(cl, sh, 0);
+    best = block_best(sh, cut.x == -kFloatMax && cut.last == kAnyIndex
+                              ? race<DT, true>(sh, sl, row, cut, noise, sum_here, s[0])
+                              : race<DT, false>(sh, sl, row, cut, noise, sum_here, s[0]));
+    if (sum_here) block_sum(sh, s, 3);
+    part = sum_here ? sh.row_sums[3] : rank == 0 ? whole : 0.0;
+    if (leave(cl, sh, best, part)) return;
+  } else if (single) {
+    if (leave(cl, sh, best, part)) return;
+  }
+  __syncthreads();
+  if (tid < 32) {
+    const unsigned long long v = warp_best(tid < nblocks ? sh.best_of[tid] : 0ull);
+    double sum = tid < nblocks ? sh.sum_of[tid] : 0.0;
+#pragma unroll
+    for (int o = 1; o < kMaxCluster; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (tid == 0) {
+      const int token = (int)~(uint32_t)v;
+      a.tokens[r] = token;
+      if (want_sum) {
+        const float x = sl.infinite ? 0.f : Elem<DT>::to_f(sl.row[token]);
+        a.logprobs[r] = (float)((double)row.z(x) - log(sum));
+      }
     }
   }
-  if (rank == 0 && tid == 0) {
-    a.tokens[r] = token;
-    if (a.logprobs != nullptr) {
-      const float x = sl.infinite ? 0.f : Elem<DT>::to_f(sl.row[token]);
-      a.logprobs[r] = (float)((double)row.z(x) - log(whole));
-    }
-  }
-  cl.sync();
 }
 
 template <int DT> cudaError_t launch_dt(const SampleArgs& a, int num_sms, cudaStream_t stream) {
@@ -1214,8 +1251,8 @@ template <int DT> cudaError_t launch_dt(const SampleArgs& a, int num_sms, cudaSt
   const int64_t per = (chunks + n - 1) / n;
   const bool held = per * 16 <= kSliceOne;
   const int smem = kListBytes + (held ? (int)per * 16 : 0);
-  cudaError_t e = cudaFuncSetAttribute(sample_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       kListBytes + kSliceOne);
+  static std::atomic<uint64_t> allowed{0};
+  cudaError_t e = allow_shared(reinterpret_cast<const void*>(sample_kernel<DT>), kListBytes + kSliceOne, allowed);
   if (e != cudaSuccess) return e;
   if ((int64_t)a.rows * n > 0x7fffffff) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg = {};

@@ -116,34 +116,14 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
          ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_float,
          ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p],
     ),
-    "fpv2_qk_norm_rope": (
-        ctypes.c_int,
-        [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64,
-         ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p,
-         ctypes.c_int32, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32,
-         ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_void_p,
-         ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
-         ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p],
-    ),
-    "fpv2_decode_attention": (
-        ctypes.c_int,
-        [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int32,
-         ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p,
-         ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p, ctypes.c_int32,
-         ctypes.c_int32, ctypes.c_float, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p,
-         ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p],
-    ),
+    # parameters as one packed structure (fpv2.decode packs them)
+    "fpv2_qk_norm_rope": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
+    "fpv2_decode_attention": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
     "fpv2_decode_workspace_bytes": (
         ctypes.c_int64,
         [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32],
     ),
-    "fpv2_sample_tokens": (
-        ctypes.c_int,
-        [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int32, ctypes.c_int64,
-         ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_float, ctypes.c_void_p,
-         ctypes.c_int32, ctypes.c_void_p, ctypes.c_float, ctypes.c_void_p, ctypes.c_float,
-         ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p],
-    ),
+    "fpv2_sample_tokens": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
     "fpv2_fast_path_mask": (
         ctypes.c_int,
         [ctypes.c_int, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,

@@ -21,25 +21,25 @@ DECODE_HEAD_DIMS = (64, 96, 128, 256)
 _HALF = (torch.float16, torch.bfloat16)
 _INT32_MAX = 2**31 - 1
 
-# Stride arrays go to the library as packed bytes. These calls are short on the GPU,
-# so their host side avoids what costs a microsecond: views, ctypes arrays, Stream
-# objects.
-_pack4 = struct.Struct("4q").pack
-_pack6 = struct.Struct("6q").pack
-_pack9 = struct.Struct("9q").pack
+# The parameter structures of include/fpv2_b200.h, field by field (null pointers are 0).
+# These calls are short on the GPU, so their host side avoids what costs microseconds:
+# many ctypes arguments, views, Stream objects.
+_pack_rope = struct.Struct("@3q 5q 6q 2q 3q 1q 2q 1q 1d 2q 4q 2q 6q 3q").pack
+_pack_decode = struct.Struct("@3q 1q 5q 3q 6q 3q 1q 4q 1d 3q 1q").pack
+_pack_sample = struct.Struct("@5q 2q 1q1d 2q 1q1d 1q1d 2q").pack
 
 
 def _refuse_grad(what: str) -> None:
     raise ValueError(f"{what} has no backward; call it under torch.no_grad()")
 
 
-def _call(fn, on: torch.Tensor, *args) -> None:
+def _call(fn, on: torch.Tensor, params: bytes) -> None:
     """One library call on ``on``'s device and its current stream."""
     if on.get_device() == torch.cuda.current_device():
-        rc = fn(*args, _lib.stream_of(on))
+        rc = fn(params, _lib.stream_of(on))
     else:
         with torch.cuda.device(on.device):
-            rc = fn(*args, _lib.stream_of(on))
+            rc = fn(params, _lib.stream_of(on))
     if rc:
         _lib.check(rc)
 
@@ -128,6 +128,7 @@ def qk_norm_rope(
         weight_code = _lib.dtype_code(weights[0].dtype)
         tensors += weights
     paged = k_cache is not None
+    kc = vc = (0, 0, 0)
     if (v is not None) != paged or (v_cache is not None) != paged or (slots is not None) != paged:
         raise ValueError("v, k_cache, v_cache and slots go together")
     if paged:
@@ -157,29 +158,32 @@ def qk_norm_rope(
     if k_weight is not None:
         k_weight = k_weight.contiguous()
     qs, ks, vs = q.stride(), k.stride(), (0, 0)
-    k_out = v_ptr = kc_ptr = vc_ptr = slots_ptr = cache_strides = None
-    pages = page_size = 0
+    k_out = None
+    v_ptr = kc_ptr = vc_ptr = slots_ptr = pages = page_size = 0
     if heads_first:
         q_out = q.new_empty((q_heads, tokens, dim))
-        out = _pack4(dim, tokens * dim, dim, tokens * dim)
+        out = (dim, tokens * dim, dim, tokens * dim)
     else:
         q_out = q.new_empty(qshape)
-        out = _pack4(q_heads * dim, dim, kv_heads * dim, dim)
+        out = (q_heads * dim, dim, kv_heads * dim, dim)
     if paged:
         v, slots = _rows(v), slots.contiguous()
         vs = v.stride()
         pages, page_size = cshape[0], cshape[1]
-        cache_strides = _pack6(kc[0], kc[1], kc[2], vc[0], vc[1], vc[2])
         v_ptr, slots_ptr = v.data_ptr(), slots.data_ptr()
         kc_ptr, vc_ptr = k_cache.data_ptr(), v_cache.data_ptr()
     else:
         k_out = q.new_empty((kv_heads, tokens, dim) if heads_first else kshape)
-    _call(_lib.lib().fpv2_qk_norm_rope, q, q.data_ptr(), k.data_ptr(), v_ptr, code, tokens, q_heads,
-          kv_heads, dim, _pack6(qs[0], qs[1], ks[0], ks[1], vs[0], vs[1]), positions.data_ptr(), wide,
-          table.data_ptr(), span, rotary, bool(interleaved), _lib.ptr(q_weight), _lib.ptr(k_weight),
-          weight_code, eps, q_out.data_ptr(), _lib.ptr(k_out), out, kc_ptr, vc_ptr, cache_strides,
-          slots_ptr, pages, page_size)
+    _call(_lib.lib().fpv2_qk_norm_rope, q, _pack_rope(
+        q.data_ptr(), k.data_ptr(), v_ptr, code, tokens, q_heads, kv_heads, dim, qs[0], qs[1], ks[0], ks[1],
+        vs[0], vs[1], positions.data_ptr(), wide, table.data_ptr(), span, rotary, bool(interleaved),
+        _address(q_weight), _address(k_weight), weight_code, eps, q_out.data_ptr(), _address(k_out), *out,
+        kc_ptr, vc_ptr, kc[0], kc[1], kc[2], vc[0], vc[1], vc[2], slots_ptr, pages, page_size))
     return q_out, k_out
+
+
+def _address(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -251,7 +255,7 @@ def decode_attention(
     if device < 0 or k_cache.get_device() != device or v_cache.get_device() != device \
             or block_tables.get_device() != device or lengths.get_device() != device:
         _lib.require_cuda(q, k_cache, v_cache, block_tables, lengths)
-    out = q.new_empty(shape)
+    out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
     lse = q.new_empty(shape[:-1], dtype=torch.float32) if return_lse else None
     if batch:
         qs, ks, vs = q.stride(), k_cache.stride(), v_cache.stride()
@@ -266,11 +270,11 @@ def decode_attention(
         nbytes = _workspace_bytes(new, q_heads, kv_heads, dim)
         workspace = q.new_empty(nbytes, dtype=torch.uint8)
         token_stride = qs[1] if len(shape) == 4 else 0
-        _call(_lib.lib().fpv2_decode_attention, q, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-              _lib.dtype_code(dtype), batch, new, q_heads, kv_heads, dim,
-              _pack9(qs[0], token_stride, qs[-2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2]),
-              block_tables.data_ptr(), block_tables.stride(0), width, lengths.data_ptr(), pages, page_size,
-              scale, window, sinks, out.data_ptr(), _lib.ptr(lse), workspace.data_ptr(), nbytes)
+        _call(_lib.lib().fpv2_decode_attention, q, _pack_decode(
+            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _lib.dtype_code(dtype), batch, new, q_heads,
+            kv_heads, dim, qs[0], token_stride, qs[-2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
+            block_tables.data_ptr(), block_tables.stride(0), width, lengths.data_ptr(), pages, page_size,
+            window, sinks, scale, out.data_ptr(), _address(lse), workspace.data_ptr(), nbytes))
     return (out, lse) if return_lse else out
 
 
@@ -330,8 +334,8 @@ def sample_tokens(
     logits, noise = _rows(logits), _rows(noise)
     tokens = logits.new_empty(rows, dtype=torch.int64)
     logprobs = logits.new_empty(rows, dtype=torch.float32) if return_logprobs else None
-    ptr = _lib.ptr
-    _call(_lib.lib().fpv2_sample_tokens, logits, logits.data_ptr(), code, rows, vocab, logits.stride(0),
-          noise.data_ptr(), noise.stride(0), ptr(heat), heat_all, ptr(k), int(k_all), ptr(p), p_all,
-          ptr(least), least_all, tokens.data_ptr(), ptr(logprobs))
+    _call(_lib.lib().fpv2_sample_tokens, logits, _pack_sample(
+        logits.data_ptr(), code, rows, vocab, logits.stride(0), noise.data_ptr(), noise.stride(0),
+        _address(heat), heat_all, _address(k), int(k_all), _address(p), p_all, _address(least), least_all,
+        tokens.data_ptr(), _address(logprobs)))
     return (tokens, logprobs) if return_logprobs else tokens

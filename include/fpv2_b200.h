@@ -290,86 +290,99 @@ FPV2_API int fpv2_pool_pages(const void* pages, const int32_t* block_table, int3
                              void* out, int out_dtype, void* stream);
 
 /*
- * Decode step (no counterpart in the reference, whose model library runs it).
+ * Decode step (no counterpart in the reference, whose model library runs it). The
+ * calls are short, so each takes one structure of 8-byte fields; sizes and strides
+ * (in elements) are int64_t, pointers are device pointers. The head dimension is
+ * contiguous everywhere.
  *
- * RMS norm of every query and key head, rotary embedding, and the write of the
- * results: y = x / sqrt(mean(x^2) + eps) * weight, then pair (a, b) of the first
- * rotary_dim dimensions becomes (a c - b s, b c + a s), in float32, rounded once.
- *   q [tokens, q_heads, head_dim], k and v [tokens, kv_heads, head_dim], `dtype`;
- *   in_strides: token and head strides of q, k, v (six, in elements; the head
- *     dimension is contiguous everywhere)
- *   positions [tokens] int32 (int64 with positions_int64), clamped into the table
- *   table float32 [table_positions, rotary_dim]: cosines of the rotary_dim / 2
- *     pairs, then their sines
- *   interleaved 0: pair i is dimensions (i, i + rotary_dim / 2); 1: (2i, 2i + 1)
- *   q_weight, k_weight (nullable) [head_dim], `weight_dtype`
- *   q_out, k_out: out_strides holds their token and head strides (four)
- * With k_cache and v_cache (page pools [num_pages, page_size, kv_heads, head_dim],
- * cache_strides: page, row and head strides of each) k is written to the cache
- * instead of k_out and v is copied: token i goes to row slots[i] % page_size of
- * page slots[i] / page_size; a slot out of range is not written. Without a cache
- * v is not used.
+ * fpv2_qk_norm_rope: RMS norm of every query and key head, rotary embedding, and the
+ * write of the results: y = x / sqrt(mean(x^2) + eps) * weight, then pair (a, b) of the
+ * first rotary_dim dimensions becomes (a c - b s, b c + a s), in float32, rounded once.
+ * With k_cache and v_cache k is written to the cache instead of k_out and v is copied:
+ * token i goes to row slots[i] % page_size of page slots[i] / page_size; a slot out of
+ * range is not written. Without a cache v is not used.
  */
-FPV2_API int fpv2_qk_norm_rope(const void* q, const void* k, const void* v, int dtype, int64_t tokens,
-                      int32_t q_heads, int32_t kv_heads, int32_t head_dim,
-                      const int64_t* in_strides, const void* positions, int32_t positions_int64,
-                      const float* table, int64_t table_positions, int32_t rotary_dim,
-                      int32_t interleaved, const void* q_weight, const void* k_weight,
-                      int weight_dtype, float eps, void* q_out, void* k_out,
-                      const int64_t* out_strides, void* k_cache, void* v_cache,
-                      const int64_t* cache_strides, const int64_t* slots, int64_t num_pages,
-                      int32_t page_size, void* stream);
+typedef struct {
+  const void *q, *k, *v;           /* [tokens, q_heads | kv_heads, head_dim] */
+  int64_t dtype, tokens, q_heads, kv_heads, head_dim;
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  const void* positions;           /* [tokens] int32, or int64; clamped into the table */
+  int64_t positions_int64;
+  const float* table;              /* [table_positions, rotary_dim]: cosines of the pairs, then sines */
+  int64_t table_positions, rotary_dim;
+  int64_t interleaved;             /* 0: pair i is (i, i + rotary_dim / 2); 1: (2 i, 2 i + 1) */
+  const void *q_weight, *k_weight; /* nullable [head_dim] */
+  int64_t weight_dtype;
+  double eps;
+  void *q_out, *k_out;
+  int64_t q_out_token_stride, q_out_head_stride, k_out_token_stride, k_out_head_stride;
+  void *k_cache, *v_cache;         /* nullable page pools [num_pages, page_size, kv_heads, head_dim] */
+  int64_t k_page_stride, k_row_stride, k_cache_head_stride, v_page_stride, v_row_stride, v_cache_head_stride;
+  const int64_t* slots;            /* [tokens] */
+  int64_t num_pages, page_size;
+} fpv2_qk_norm_rope_params;
+FPV2_API int fpv2_qk_norm_rope(const fpv2_qk_norm_rope_params* params, void* stream);
 
 /*
- * Attention of the newest new_tokens tokens of each sequence over its paged K/V,
- * the keys of all sequences split evenly over the GPU and joined.
- *   q [batch, new_tokens, q_heads, head_dim]; k_pages, v_pages [num_pages,
- *     page_size, kv_heads, head_dim]; head_dim 64, 96, 128 or 256
- *   strides (nine, in elements): batch, token, head of q (multiples of 2); page,
- *     row, head of k_pages and of v_pages (multiples of 8)
- *   block_tables int32 [batch, table_width], rows table_stride apart; entries past
- *     a sequence's pages are not read, the others are clamped to the pool
- *   lengths int32 [batch]: keys of each sequence, the new tokens included
- *     (clamped to [0, table_width * page_size])
- * Query t of sequence b is at position p = lengths[b] - new_tokens + t and sees the
- * keys j <= p with j < sinks or j > p - window (window 0: all j <= p). out
- * [batch, new_tokens, q_heads, head_dim] and lse (nullable) float32 [batch,
- * new_tokens, q_heads] (natural log) are contiguous; a query that sees no key gets
- * zeros and -inf. `workspace`: fpv2_decode_workspace_bytes(...), 16-byte aligned,
- * written before it is read by each call.
+ * Attention of the newest new_tokens tokens of each sequence over its paged K/V, the
+ * keys of all sequences split evenly over the GPU and joined. Query t of sequence b is
+ * at position p = lengths[b] - new_tokens + t and sees the keys j <= p with j < sinks or
+ * j > p - window (window 0: all j <= p). out and lse (natural log) are contiguous; a
+ * query that sees no key gets zeros and -inf. Table entries past a sequence's pages are
+ * not read, the others are clamped to the pool; lengths are clamped to [0, table_width *
+ * page_size]. The workspace is written before it is read by each call.
  */
-FPV2_API int fpv2_decode_attention(const void* q, const void* k_pages, const void* v_pages, int dtype,
-                          int32_t batch, int32_t new_tokens, int32_t q_heads, int32_t kv_heads,
-                          int32_t head_dim, const int64_t* strides, const int32_t* block_tables,
-                          int64_t table_stride, int32_t table_width, const int32_t* lengths,
-                          int32_t num_pages, int32_t page_size, float scale, int32_t window,
-                          int32_t sinks, void* out, float* lse, void* workspace,
-                          int64_t workspace_bytes, void* stream);
+typedef struct {
+  const void* q;                   /* [batch, new_tokens, q_heads, head_dim], 4-byte aligned */
+  const void *k_pages, *v_pages;   /* [num_pages, page_size, kv_heads, head_dim], 16-byte aligned */
+  int64_t dtype;                   /* FPV2_F16 or FPV2_BF16 */
+  int64_t batch, new_tokens, q_heads, kv_heads, head_dim;   /* head_dim 64, 96, 128 or 256 */
+  int64_t q_batch_stride, q_token_stride, q_head_stride;    /* multiples of 2 */
+  int64_t k_page_stride, k_row_stride, k_head_stride;       /* multiples of 8 */
+  int64_t v_page_stride, v_row_stride, v_head_stride;
+  const int32_t* block_tables;     /* [batch, table_width], rows table_stride apart */
+  int64_t table_stride, table_width;
+  const int32_t* lengths;          /* [batch]: keys, the new tokens included */
+  int64_t num_pages, page_size, window, sinks;
+  double scale;
+  void* out;                       /* [batch, new_tokens, q_heads, head_dim] */
+  float* lse;                      /* nullable [batch, new_tokens, q_heads] */
+  void* workspace;                 /* fpv2_decode_workspace_bytes(), 16-byte aligned */
+  int64_t workspace_bytes;
+} fpv2_decode_attention_params;
+FPV2_API int fpv2_decode_attention(const fpv2_decode_attention_params* params, void* stream);
 
 /* Workspace of fpv2_decode_attention (any batch and lengths); 0 for an unsupported shape. */
 FPV2_API int64_t fpv2_decode_workspace_bytes(int32_t new_tokens, int32_t q_heads, int32_t kv_heads,
                                     int32_t head_dim);
 
 /*
- * The next token of each row of logits [rows, vocab] (`dtype`, rows logits_stride
- * elements apart) from given random numbers: noise float32 [rows, vocab], positive,
- * exponentially distributed. With x the logits (NaN as -inf), z = (x - max) / T and
- * w = exp(z), tokens ordered by (x descending, index ascending):
- *   top_k > 0: the first top_k stay; top_p < 1: of those, the shortest prefix whose
- *   weight reaches top_p times their weight; min_p > 0: of those, w >= min_p; the
- *   first token always stays. tokens[r] = argmax of z - log(noise), ties to the
- *   lowest index. T <= 0: the lowest index of the maximum. A row without a logit
- *   above -inf gives -1.
- * temperature, top_k, top_p, min_p: [rows] on the device, or null to use the *_all
- * value for every row. logprobs (nullable) float32 [rows]: log of the token's share
- * of sum exp(x / T) over the whole row, before the filters (T = 1 where T <= 0).
+ * The next token of each row of logits from given random numbers. With x the logits
+ * (NaN as -inf), z = (x - max) / T and w = exp(z), tokens ordered by (x descending, index
+ * ascending): top_k > 0: the first top_k stay; top_p < 1: of those, the shortest prefix
+ * whose weight reaches top_p times their weight; min_p > 0: of those, w >= min_p; the
+ * first token always stays. tokens[r] = argmax of z - log(noise), ties to the lowest
+ * index. T <= 0: the lowest index of the maximum. A row without a logit above -inf
+ * gives -1. logprobs: log of the token's share of sum exp(x / T) over the whole row,
+ * before the filters (T = 1 where T <= 0).
  */
-FPV2_API int fpv2_sample_tokens(const void* logits, int dtype, int64_t rows, int32_t vocab,
-                       int64_t logits_stride, const float* noise, int64_t noise_stride,
-                       const float* temperature, float temperature_all, const int32_t* top_k,
-                       int32_t top_k_all, const float* top_p, float top_p_all,
-                       const float* min_p, float min_p_all, int64_t* tokens, float* logprobs,
-                       void* stream);
+typedef struct {
+  const void* logits;              /* [rows, vocab], rows logits_stride apart */
+  int64_t dtype, rows, vocab, logits_stride;
+  const float* noise;              /* [rows, vocab], positive, exponentially distributed */
+  int64_t noise_stride;
+  const float* temperature;        /* [rows], or null: temperature_all for every row */
+  double temperature_all;
+  const int32_t* top_k;
+  int64_t top_k_all;
+  const float* top_p;
+  double top_p_all;
+  const float* min_p;
+  double min_p_all;
+  int64_t* tokens;                 /* [rows] */
+  float* logprobs;                 /* nullable [rows] */
+} fpv2_sample_tokens_params;
+FPV2_API int fpv2_sample_tokens(const fpv2_sample_tokens_params* params, void* stream);
 
 /*
  * Which kernel family the two stages would use for this shape:

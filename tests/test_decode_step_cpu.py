@@ -8,12 +8,14 @@ status for scalars out of contract.
 from __future__ import annotations
 
 import ctypes
+import re
+from pathlib import Path
 
 import pytest
 import torch
 
 import fpv2
-from fpv2 import _lib
+from fpv2 import _lib, decode
 
 BF = torch.bfloat16
 
@@ -127,40 +129,80 @@ def test_rope_table_rows_and_refusals():
             fpv2.rope_table(*bad)
 
 
+def _structure(name: str) -> type[ctypes.Structure]:
+    """A parameter structure as include/fpv2_b200.h declares it."""
+    text = (Path(__file__).resolve().parents[1] / "include" / "fpv2_b200.h").read_text()
+    body = re.search(r"typedef struct \{([^}]*)\} " + name + ";", text).group(1)
+    fields = []
+    for line in re.sub(r"/\*.*?\*/", "", body, flags=re.S).split(";"):
+        line = line.strip()
+        if not line:
+            continue
+        kind = ctypes.c_double if line.startswith("double") else ctypes.c_int64
+        names = re.sub(r"^(const\s+)?\w+", "", line).replace("*", " ")
+        fields += [(f.strip(), kind) for f in names.split(",")]
+    return type(name, (ctypes.Structure,), {"_fields_": fields})
+
+
+@pytest.mark.parametrize("name,pack", [
+    ("fpv2_qk_norm_rope_params", decode._pack_rope),
+    ("fpv2_decode_attention_params", decode._pack_decode),
+    ("fpv2_sample_tokens_params", decode._pack_sample),
+])
+def test_packed_parameters_have_the_declared_layout(name, pack):
+    kind = _structure(name)
+    values = [float(i) if t is ctypes.c_double else i for i, (_, t) in enumerate(kind._fields_)]
+    assert pack(*values) == bytes(kind(*values))
+
+
 def test_entry_points_return_status_without_gpu():
     lib = _lib.lib()
     before = _lib.launch_count()
-    nine = (ctypes.c_int64 * 9)(*[64] * 9)
-    six = (ctypes.c_int64 * 6)(*[64] * 6)
+    some = 1 << 20   # a pointer that is never followed
 
-    def decode(batch=1, new=1, hq=4, hkv=2, dim=64, strides=nine, pages=2, page=16, width=2, scale=1.0,
-               window=0, dtype=1, ptr=1 << 20, nbytes=1 << 40):
-        return lib.fpv2_decode_attention(ptr, ptr, ptr, dtype, batch, new, hq, hkv, dim, strides, ptr, 2, width,
-                                         ptr, pages, page, scale, window, 0, ptr, None, ptr, nbytes, None)
+    def call(entry, good, **change):
+        kind = _structure(entry + "_params")
+        fields = {n: some if n not in good else good[n] for n, _ in kind._fields_}
+        fields.update(change)
+        return getattr(lib, entry)(bytes(kind(**{n: v or 0 for n, v in fields.items()})), None)
 
-    bad = [decode(dtype=2), decode(batch=-1), decode(new=0), decode(hq=3), decode(dim=80), decode(pages=0),
-           decode(width=1 << 30), decode(scale=float("nan")), decode(window=-1), decode(strides=None),
-           decode(ptr=None), decode(nbytes=8), decode(strides=(ctypes.c_int64 * 9)(*[4] * 9))]
+    def decode_call(**change):
+        good = dict(dtype=1, batch=1, new_tokens=1, q_heads=4, kv_heads=2, head_dim=64, table_width=2,
+                    num_pages=2, page_size=16, window=0, sinks=0, scale=1.0, workspace_bytes=1 << 40)
+        return call("fpv2_decode_attention", good, **change)
+
+    bad = [decode_call(**c) for c in (
+        dict(dtype=2), dict(batch=-1), dict(new_tokens=0), dict(q_heads=3), dict(q_heads=1 << 30),
+        dict(head_dim=80), dict(num_pages=0), dict(table_width=1 << 30), dict(scale=float("nan")),
+        dict(window=-1), dict(sinks=1 << 40), dict(q=None), dict(lengths=None), dict(workspace_bytes=8),
+        dict(k_row_stride=4), dict(q_head_stride=3), dict(k_pages=some + 2), dict(workspace=some + 8))]
     assert bad == [_lib.ERR_INVALID_ARGUMENT] * len(bad)
-    assert decode(batch=0) == _lib.OK
+    assert decode_call(batch=0) == _lib.OK
 
-    def rope(dtype=1, tokens=1, hq=1, dim=64, rot=64, table=8, eps=1e-6, ptr=1 << 20, k_cache=None, strides=six):
-        return lib.fpv2_qk_norm_rope(ptr, ptr, ptr, dtype, tokens, hq, 1, dim, strides, ptr, 0, ptr, table, rot, 0,
-                                     None, None, dtype, eps, ptr, ptr, strides, k_cache, None, None, None, 0, 0,
-                                     None)
+    def rope_call(**change):
+        good = dict(dtype=1, tokens=1, q_heads=1, kv_heads=1, head_dim=64, table_positions=8, rotary_dim=64,
+                    interleaved=0, positions_int64=0, weight_dtype=1, eps=1e-6, k_cache=0, v_cache=0)
+        return call("fpv2_qk_norm_rope", good, **change)
 
-    bad = [rope(dtype=7), rope(tokens=-1), rope(hq=0), rope(dim=257), rope(rot=63), rope(rot=66), rope(table=0),
-           rope(eps=-1.0), rope(ptr=None), rope(k_cache=1 << 20), rope(strides=None)]
+    bad = [rope_call(**c) for c in (
+        dict(dtype=7), dict(tokens=-1), dict(q_heads=0), dict(head_dim=257), dict(rotary_dim=63),
+        dict(rotary_dim=66), dict(table_positions=0), dict(eps=-1.0), dict(q=None), dict(weight_dtype=5),
+        dict(k_cache=some), dict(k_cache=some, v_cache=some, slots=None),
+        dict(k_cache=some, v_cache=some, page_size=0))]
     assert bad == [_lib.ERR_INVALID_ARGUMENT] * len(bad)
-    assert rope(tokens=0) == _lib.OK
+    assert rope_call(tokens=0) == _lib.OK
 
-    def sample(dtype=1, rows=1, vocab=8, ptr=1 << 20):
-        return lib.fpv2_sample_tokens(ptr, dtype, rows, vocab, vocab, ptr, vocab, None, 1.0, None, 0, None, 1.0,
-                                      None, 0.0, ptr, None, None)
+    def sample_call(**change):
+        good = dict(dtype=1, rows=1, vocab=8, temperature_all=1.0, top_k_all=0, top_p_all=1.0, min_p_all=0.0)
+        return call("fpv2_sample_tokens", good, **change)
 
-    bad = [sample(dtype=3), sample(rows=-1), sample(vocab=0), sample(ptr=None), sample(ptr=(1 << 20) + 1)]
+    bad = [sample_call(**c) for c in (
+        dict(dtype=3), dict(rows=-1), dict(vocab=0), dict(logits=None), dict(noise=None),
+        dict(logits=some + 1))]
     assert bad == [_lib.ERR_INVALID_ARGUMENT] * len(bad)
-    assert sample(rows=0) == _lib.OK
+    assert sample_call(rows=0) == _lib.OK
+    for entry in ("fpv2_qk_norm_rope", "fpv2_decode_attention", "fpv2_sample_tokens"):
+        assert getattr(lib, entry)(None, None) == _lib.ERR_INVALID_ARGUMENT
     assert lib.fpv2_decode_workspace_bytes(1, 3, 2, 64) == 0
     assert lib.fpv2_decode_workspace_bytes(1, 32, 8, 128) > 0
     assert _lib.launch_count() == before
