@@ -41,10 +41,12 @@ template <int D> constexpr int kPitch = D * 2 + 16;
 template <int D> constexpr int kStageBytes = 2 * Shape<D>::TK * kPitch<D>;
 
 // Blocks of eight query rows a warp takes, and the warps that share a KV head's rows.
-// More blocks reuse a tile in shared memory but need their own accumulators in
-// registers: 16 bytes of head_dim a block and lane, so two blocks at most for 256.
+// More blocks reuse a tile in shared memory but need their queries and accumulators in
+// registers, 3 D / 4 a block and lane with the addresses and scores beside them: four
+// blocks fit for head_dim 64 alone (at 128, 8 x 8000 keys of 32 rows a head take 203 us
+// with four blocks, which spill, and 100 us with two and the tiles fetched twice).
 __host__ __device__ inline int blocks_of(int rows, int D) {
-  return rows <= 8 ? 1 : rows <= 16 || D == 256 ? 2 : 4;
+  return rows <= 8 ? 1 : rows <= 16 || D > 64 ? 2 : 4;
 }
 __host__ __device__ inline int row_groups(int rows, int D) {
   const int per = 8 * blocks_of(rows, D);
@@ -86,20 +88,32 @@ __device__ __forceinline__ int warp_sum(int v) {
   return v;
 }
 
-// Tiles before sequence `want` and in total (warp-wide).
+// A sequence costs its tiles and about two more, for its queries' way in and its
+// results' way out; the stream that is cut into parts counts those first, ahead of the
+// tiles. (Without them a part of many short sequences took three times the average part's
+// time: 24 sequences of 3 to 20011 keys, 55 us against @@ us.)
+constexpr int kSeqCost = 2;
+__device__ __forceinline__ int cost_of(const Seq& s) { return s.tiles > 0 ? s.tiles + kSeqCost : 0; }
+
+// Stream units before sequence `want` and in total (warp-wide).
 template <int TK>
 __device__ __forceinline__ void scan_to(const DecodeArgs& a, int lane, int want, int64_t& before,
                                         int64_t& total) {
   before = total = 0;
   for (int b0 = 0; b0 < a.B; b0 += 32) {
-    const int n = seq_of<TK>(a, b0 + lane).tiles;
+    const int n = cost_of(seq_of<TK>(a, b0 + lane));
     before += warp_sum(b0 + lane < want ? n : 0);
     total += warp_sum(n);
   }
 }
 
+// a / b for non-negative a and positive b, mostly of 32 bits.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
 __device__ __forceinline__ int64_t part_tiles(int64_t total, int parts) {
-  return (total + parts - 1) / parts;
+  return quotient(total + parts - 1, parts);
 }
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
@@ -151,11 +165,33 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Walks the tiles of a part for the copies: sequence, tile in it, and this lane's
-// row of it: its page (loaded one tile before it is needed) and place in the page.
-template <int TK> struct Feed {
+// Walks the tiles of a part: sequence, tile in it, and the tile's place in the stream.
+template <int TK> struct Walk {
   int b, t;
   Seq s;
+  int64_t at;
+
+  __device__ __forceinline__ void next(const DecodeArgs& a, int64_t end) {
+    ++t;
+    ++at;
+    while (t >= s.tiles && at + kSeqCost < end) {   // a sequence with tiles ahead
+      ++b;
+      s = seq_of<TK>(a, b);
+      if (s.tiles > 0) {
+        t = 0;
+        at += kSeqCost;
+      }
+    }
+    if (t >= s.tiles) at = end;
+  }
+};
+
+// The walk for the copies, with this lane's row of the tile: its page (loaded one tile
+// before it is needed) and place in the page.
+template <int TK> struct Feed : Walk<TK> {
+  using Walk<TK>::b;
+  using Walk<TK>::t;
+  using Walk<TK>::s;
   int page, in_page;
 
   __device__ __forceinline__ int key0() const { return (t < s.head ? t : t + s.jump) * TK; }
@@ -165,15 +201,6 @@ template <int TK> struct Feed {
     const int at = a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size;
     in_page = key - at * a.page_size;
     page = a.tables[(int64_t)b * a.table_stride + at];
-  }
-  __device__ __forceinline__ void next(const DecodeArgs& a, int lane, bool whole) {
-    ++t;
-    while (t >= s.tiles) {   // a part that goes on has a sequence with tiles ahead
-      ++b;
-      t = 0;
-      s = seq_of<TK>(a, b);
-    }
-    fetch(a, lane, whole);
   }
 };
 
@@ -194,9 +221,8 @@ __global__ void __launch_bounds__(Shape<D>::NW * 32, 1) decode_kernel(const Deco
   const int g = lane >> 2, c = lane & 3;   // mma fragments: rows g and g + 8, column pair c
   const int R = a.G * a.T;                 // query rows of a KV head
   const int groups = row_groups(R, D), cols = a.Hkv * groups;
-  const int64_t wi = (int64_t)blockIdx.x * NW + warp;
-  const int64_t part = wi / cols;
-  const int col = (int)(wi - part * cols);
+  const unsigned wi = blockIdx.x * NW + warp;
+  const int part = (int)(wi / (unsigned)cols), col = (int)(wi - (unsigned)part * cols);
   const int h = col / groups, rbase = (col - h * groups) * 8 * NB;
   if (part >= parts) return;
 
@@ -204,16 +230,16 @@ __global__ void __launch_bounds__(Shape<D>::NW * 32, 1) decode_kernel(const Deco
   int64_t unused, total;
   scan_to<TK>(a, lane, 0, unused, total);
   const int64_t chunk = part_tiles(total, parts);
-  const int64_t begin = part * chunk, end = min(begin + chunk, total);
+  const int64_t begin = (int64_t)part * chunk, end = min(begin + chunk, total);
   if (begin >= end) return;
-  const int count = (int)(end - begin);
   const bool whole = a.page_size % TK == 0;
   Feed<TK> f;
+  bool started;   // the first sequence started in an earlier part
   {
     int64_t run = 0;
     int b0 = 0;
     while (true) {
-      const int n = seq_of<TK>(a, b0 + lane).tiles;
+      const int n = cost_of(seq_of<TK>(a, b0 + lane));
       int incl = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -224,7 +250,10 @@ __global__ void __launch_bounds__(Shape<D>::NW * 32, 1) decode_kernel(const Deco
       if (past) {
         const int at = __ffs(past) - 1;
         f.b = b0 + at;
-        f.t = (int)(begin - run - (__shfl_sync(0xffffffffu, incl, at) - __shfl_sync(0xffffffffu, n, at)));
+        run += __shfl_sync(0xffffffffu, incl - n, at);   // where the sequence starts
+        f.t = max((int)(begin - run) - kSeqCost, 0);
+        f.at = run + kSeqCost + f.t;
+        started = run < begin;
         break;
       }
       run += __shfl_sync(0xffffffffu, incl, 31);
@@ -232,10 +261,10 @@ __global__ void __launch_bounds__(Shape<D>::NW * 32, 1) decode_kernel(const Deco
     }
     f.s = seq_of<TK>(a, f.b);
   }
+  if (f.at >= end) return;   // nothing but the cost of a sequence whose tiles are the next part's
   f.fetch(a, lane, whole);
-  int b = f.b, t = f.t, seg0 = f.t;   // the consumer's sequence, tile, and the segment's first tile
-  Seq s = f.s;
-  bool first = true;
+  Walk<TK> w = f;    // the consumer's
+  int seg0 = f.t;    // its segment's first tile
 
   unsigned char* const ring_ptr = smem + warp * ST * kStageBytes<D>;
   const uint32_t ring = smem_u32(ring_ptr);
@@ -243,10 +272,10 @@ __global__ void __launch_bounds__(Shape<D>::NW * 32, 1) decode_kernel(const Deco
   const T* kh = reinterpret_cast<const T*>(a.k) + h * a.k_sh + lch * 8;
   const T* vh = reinterpret_cast<const T*>(a.v) + h * a.v_sh + lch * 8;
   const uint32_t ldst = lrow * PITCH + lch * 16;
-  int ahead = 0, fill = 0;   // tiles whose copies were issued, and the ring slot of the next
+  int fill = 0;   // the ring slot of the next copy
 
-  auto issue = [&]() {
-    if (ahead < count) {
+  auto issue = [&](const Feed<TK>& f) {
+    if (f.at < end) {
       const uint32_t dst = ring + fill * kStageBytes<D> + ldst;
       fill = fill + 1 == ST ? 0 : fill + 1;
       const int key0 = f.key0();
@@ -282,12 +311,23 @@ __global__ void __launch_bounds__(Shape<D>::NW * 32, 1) decode_kernel(const Deco
           }
         }
       }
-      if (++ahead < count) f.next(a, lane, whole);
     }
     cp_commit();
   };
+  auto advance = [&]() {
+    if (f.at < end) f.next(a, end);
+    if (f.at < end) f.fetch(a, lane, whole);
+  };
+  {
+    Feed<TK> early[ST - 1];   // their table entries are loaded side by side
 #pragma unroll
-  for (int i = 0; i < ST - 1; ++i) issue();
+    for (int i = 0; i < ST - 1; ++i) {
+      early[i] = f;
+      advance();
+    }
+#pragma unroll
+    for (int i = 0; i < ST - 1; ++i) issue(early[i]);
+  }
 
   uint32_t qf[NB][KS][2];
   float o[NB][KS][4];
@@ -301,7 +341,7 @@ __global__ void __launch_bounds__(Shape<D>::NW * 32, 1) decode_kernel(const Deco
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
       const int r = rbase + n * 8 + g, rt = r / a.G;
-      const T* q = reinterpret_cast<const T*>(a.q) + b * a.q_sb + rt * a.q_st +
+      const T* q = reinterpret_cast<const T*>(a.q) + w.b * a.q_sb + rt * a.q_st +
                    (int64_t)(h * a.G + r - rt * a.G) * a.q_sh + c * 2;
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
@@ -322,10 +362,11 @@ __global__ void __launch_bounds__(Shape<D>::NW * 32, 1) decode_kernel(const Deco
   const uint32_t k_at = ((lane & 7) + ((lane >> 3) & 1) * 8) * PITCH + (lane >> 4) * 16;
   const uint32_t v_at = (TK + (lane & 7) + (lane >> 4) * 8) * PITCH + ((lane >> 3) & 1) * 16;
   int slot = 0;
-  for (int i = 0; i < count; ++i) {
+  while (true) {
     cp_wait<ST - 2>();
     __syncwarp();
-    issue();
+    issue(f);
+    advance();
     const uint32_t tile = ring + slot * kStageBytes<D>;
     const unsigned char* vtile = ring_ptr + slot * kStageBytes<D> + TK * PITCH;
     slot = slot + 1 == ST ? 0 : slot + 1;
@@ -349,7 +390,8 @@ __global__ void __launch_bounds__(Shape<D>::NW * 32, 1) decode_kernel(const Deco
 #pragma unroll
         for (int j = 0; j < 4; ++j) sc[mt][n][j] = (sc[mt][n][j] + s2[n][j]) * a.scale_log2;
     }
-    const int key0 = (t < s.head ? t : t + s.jump) * TK;
+    const Seq& s = w.s;
+    const int key0 = (w.t < s.head ? w.t : w.t + s.jump) * TK;
     // a tile that every row sees whole needs no mask
     const int p_first = s.len - a.T;
     const bool open = key0 + TK <= p_first + 1 &&
@@ -477,11 +519,13 @@ __global__ void __launch_bounds__(Shape<D>::NW * 32, 1) decode_kernel(const Deco
           }
       }
     }
-    ++t;
-    if (t == s.tiles || i + 1 == count) {
+    const int was_b = w.b;
+    const bool whole_seq = seg0 == 0 && w.t + 1 == s.tiles;
+    w.next(a, end);
+    if (w.b != was_b || w.at >= end) {
       // the segment ends: its sums over the lanes' keys, then out or to the workspace
-      const bool done = seg0 == 0 && t == s.tiles;
-      const int64_t piece = (part * 2 + (first ? 0 : 1)) * cols + col;
+      const bool done = whole_seq;
+      const int64_t piece = ((int64_t)part * 2 + (started ? 0 : 1)) * cols + col;
       float2* ml = reinterpret_cast<float2*>(a.workspace) + piece * (8 * NB);
       float* po = reinterpret_cast<float*>(reinterpret_cast<float2*>(a.workspace) +
                                            (int64_t)parts * 2 * cols * (8 * NB)) + piece * (8 * NB) * D;
@@ -497,7 +541,7 @@ __global__ void __launch_bounds__(Shape<D>::NW * 32, 1) decode_kernel(const Deco
           if (done) {
             const bool any = sum > 0.f || sum != sum;
             const float inv = any ? 1.f / sum : 0.f;
-            const int64_t row = ((int64_t)b * a.T + tq[n][j]) * a.Hq + h * a.G + r - tq[n][j] * a.G;
+            const int64_t row = ((int64_t)was_b * a.T + tq[n][j]) * a.Hq + h * a.G + r - tq[n][j] * a.G;
             T* dst = reinterpret_cast<T*>(a.out) + row * D + g;
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
@@ -515,16 +559,10 @@ __global__ void __launch_bounds__(Shape<D>::NW * 32, 1) decode_kernel(const Deco
             }
           }
         }
-      first = false;
-      if (i + 1 < count) {
-        do {
-          ++b;
-          s = seq_of<TK>(a, b);
-        } while (s.tiles == 0);
-        t = 0;
-        seg0 = 0;
-        start_segment();
-      }
+      if (w.at >= end) break;
+      started = false;
+      seg0 = 0;
+      start_segment();
     }
   }
   cp_wait<0>();
@@ -532,53 +570,74 @@ __global__ void __launch_bounds__(Shape<D>::NW * 32, 1) decode_kernel(const Deco
 
 // Joins the pieces of the sequences that were cut:
 //   m = max m_i,  o = sum 2^(m_i - m) o_i / sum 2^(m_i - m) l_i,
-// and fills the rows of empty sequences. WPR warps take one query row.
-template <int DT, int D, int WPR>
-__global__ void __launch_bounds__(256) decode_join_kernel(const DecodeArgs a, int parts) {
-  constexpr int TK = Shape<D>::TK, NV = D / 32;
-  __shared__ float red[WPR > 1 ? WPR : 1][D + 2];
+// and fills the rows of empty sequences. A warp takes a row (ROW_CTA: a CTA, for few rows
+// of many pieces each).
+// It fits beside the first kernel's CTAs, so it is launched and has its part boundaries
+// when that one ends.
+
+template <int DT, int D, bool ROW_CTA>
+__global__ void __launch_bounds__(256, 4) decode_join_kernel(const DecodeArgs a, int parts) {
+  constexpr int TK = Shape<D>::TK, NV = D / 32, WARPS = 8, WPR = ROW_CTA ? WARPS : 1;
+  __shared__ float red[WPR][D + 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % WPR;
-  const int64_t rows = (int64_t)a.B * a.T * a.Hq;
-  const int64_t row_raw = (int64_t)blockIdx.x * (8 / WPR) + warp / WPR;
-  const bool live = row_raw < rows;
-  const int64_t row = live ? row_raw : rows - 1;
-  const int hq = (int)(row % a.Hq), tq = (int)(row / a.Hq % a.T), b = (int)(row / a.Hq / a.T);
-  const int h = hq / a.G, r = tq * a.G + hq - h * a.G;
-  const int R = a.G * a.T, per = 8 * blocks_of(R, D), groups = row_groups(R, D);
-  const int cols = a.Hkv * groups, col = h * groups + r / per;
+  const int R = a.G * a.T, per = 8 * blocks_of(R, D), groups = row_groups(R, D), cols = a.Hkv * groups;
+  const unsigned id = ROW_CTA ? blockIdx.x : blockIdx.x * WARPS + warp;   // (b * Hkv + h) * R + r
+  const unsigned head = id / (unsigned)R;
+  const int r = (int)(id - head * R), b = (int)(head / (unsigned)a.Hkv), h = (int)(head - (unsigned)b * a.Hkv);
+  if (b >= a.B) return;
   int64_t before, total;
   scan_to<TK>(a, lane, b, before, total);
   const int64_t chunk = max((int64_t)1, part_tiles(total, parts));
   const int n = seq_of<TK>(a, b).tiles;
-  const int64_t p0 = before / chunk, p1 = n > 0 ? (before + n - 1) / chunk : p0;
+  const int p0 = (int)quotient(before + kSeqCost, chunk);
+  const int p1 = n > 0 ? (int)quotient(before + kSeqCost + n - 1, chunk) : p0;
+  const bool late = before >= (int64_t)p0 * chunk;   // the sequence starts in its first part
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (n > 0 && p0 == p1) return;   // finished by its warp (the same for all warps of a row)
+  if (n > 0 && p0 == p1) return;   // finished by its warp
   const float2* ml = reinterpret_cast<const float2*>(a.workspace);
   const float* po = reinterpret_cast<const float*>(ml + (int64_t)parts * 2 * cols * per);
-  const int count = n > 0 ? (int)(p1 - p0 + 1) : 0;
-  auto slot_row = [&](int i) {   // the piece of part p0 + i: a part's first segment is in its slot 0
-    const int64_t p = p0 + i;
-    const int64_t s = p * 2 + (i == 0 && before > p * chunk ? 1 : 0);
-    return (s * cols + col) * per + r % per;
+  const int count = n > 0 ? p1 - p0 + 1 : 0;
+  const int col = h * groups + r / per, lr = r % per;
+  auto slot_row = [&](int i) {   // the piece of part p0 + i: slot 1 where the sequence starts
+    return ((int64_t)((p0 + i) * 2 + (i == 0 && late ? 1 : 0)) * cols + col) * per + lr;
   };
   float m = -INFINITY;
   for (int i = lane; i < count; i += 32) m = fmaxf(m, ml[slot_row(i)].x);
-#pragma unroll
-  for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
-  const float base = m == -INFINITY ? 0.f : m;
-  float acc[NV], l = 0.f;
+  float acc[NV], l = 0.f, base = 0.f;
 #pragma unroll
   for (int j = 0; j < NV; ++j) acc[j] = 0.f;
-#pragma unroll 4
-  for (int i = sub; i < count; i += WPR) {
-    const int64_t at = slot_row(i);
-    const float2 x = ml[at];
-    const float w = ex2(x.x - base);
-    l = fmaf(w, x.y, l);
+  constexpr int U = NV <= 2 ? 8 : NV <= 4 ? 4 : 2;   // pieces in flight a warp
+  for (int i0 = sub; i0 < count; i0 += U * WPR) {
+    float2 x[U];
+    float v[U][NV];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) acc[j] = fmaf(w, po[at * D + lane + 32 * j], acc[j]);
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * WPR;
+      x[u] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int j = 0; j < NV; ++j) v[u][j] = 0.f;
+      if (i < count) {
+        const int64_t at = slot_row(i);
+        x[u] = ml[at];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) v[u][j] = po[at * D + lane + 32 * j];
+      }
+    }
+    if (i0 == sub) {   // the maximum, while the first outputs are on their way
+#pragma unroll
+      for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
+      base = m == -INFINITY ? 0.f : m;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float w = ex2(x[u].x - base);
+      l = fmaf(w, x[u].y, l);
+#pragma unroll
+      for (int j = 0; j < NV; ++j) acc[j] = fmaf(w, v[u][j], acc[j]);
+    }
   }
-  if constexpr (WPR > 1) {
+  if constexpr (ROW_CTA) {
+    // (a warp without pieces did not reduce its maximum: the first has one and writes)
 #pragma unroll
     for (int j = 0; j < NV; ++j) red[sub][lane + 32 * j] = acc[j];
     if (lane == 0) red[sub][D] = l;
@@ -591,9 +650,10 @@ __global__ void __launch_bounds__(256) decode_join_kernel(const DecodeArgs a, in
       l += red[w][D];
     }
   }
-  if (!live) return;
   const bool any = l > 0.f || l != l;
   const float inv = any ? 1.f / l : 0.f;
+  const int tq = r / a.G;
+  const int64_t row = ((int64_t)b * a.T + tq) * a.Hq + h * a.G + r - tq * a.G;
   using E = Elem<DT>;
   typename E::T* dst = reinterpret_cast<typename E::T*>(a.out) + row * D;
 #pragma unroll
@@ -612,11 +672,11 @@ template <int D> size_t workspace_for(int rows, int Hkv) {
   return (size_t)parts_for<D>(cols) * 2 * cols * 8 * blocks_of(rows, D) * (D + 2) * sizeof(float);
 }
 
-template <int DT, int D, int WPR>
+
+template <int DT, int D, bool ROW_CTA>
 cudaError_t launch_join(const DecodeArgs& a, int parts, cudaStream_t stream) {
-  const int64_t rows = (int64_t)a.B * a.T * a.Hq;
-  const int64_t blocks = (rows * WPR + 7) / 8;
-  if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  const int64_t rows = (int64_t)a.B * a.Hq * a.T, blocks = ROW_CTA ? rows : (rows + 7) / 8;
+  if (rows > 0x7fffffff) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)blocks);
   cfg.blockDim = dim3(256);
@@ -626,7 +686,7 @@ cudaError_t launch_join(const DecodeArgs& a, int parts, cudaStream_t stream) {
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, decode_join_kernel<DT, D, WPR>, a, parts);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, decode_join_kernel<DT, D, ROW_CTA>, a, parts);
   if (e == cudaSuccess) count_launch();
   return e;
 }
@@ -644,17 +704,15 @@ template <int DT, int D, int NB> cudaError_t launch_blocks(const DecodeArgs& a, 
   if (e != cudaSuccess) return e;
   count_launch();
   // few rows with many pieces each: a CTA a row; else a warp a row
-  return parts / a.B >= 16 ? launch_join<DT, D, 8>(a, parts, stream) : launch_join<DT, D, 1>(a, parts, stream);
+  return parts / a.B >= 16 ? launch_join<DT, D, true>(a, parts, stream)
+                           : launch_join<DT, D, false>(a, parts, stream);
 }
 
 template <int DT, int D> cudaError_t launch_dim(const DecodeArgs& a, cudaStream_t stream) {
-  switch (blocks_of(a.G * a.T, D)) {
-    case 1: return launch_blocks<DT, D, 1>(a, stream);
-    case 2: return launch_blocks<DT, D, 2>(a, stream);
-    default:
-      if constexpr (D != 256) return launch_blocks<DT, D, 4>(a, stream);
-      return cudaErrorInvalidValue;
-  }
+  const int blocks = blocks_of(a.G * a.T, D);
+  if constexpr (D == 64)
+    if (blocks == 4) return launch_blocks<DT, D, 4>(a, stream);
+  return blocks == 1 ? launch_blocks<DT, D, 1>(a, stream) : launch_blocks<DT, D, 2>(a, stream);
 }
 
 template <int DT> cudaError_t launch_dt(const DecodeArgs& a, cudaStream_t stream) {

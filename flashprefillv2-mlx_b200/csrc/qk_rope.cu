@@ -59,57 +59,124 @@ __device__ __forceinline__ int64_t slot_of(const RopeArgs& a, int64_t t) {
   return s >= 0 && s < a.num_slots ? s : -1;
 }
 
-// Four values as they are in memory, and as floats.
-template <int DT> struct Four;
-template <> struct Four<DT_F32> {
-  float4 u;
-  __device__ __forceinline__ void to(float* x) const { x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w; }
-  static __device__ __forceinline__ Four of(const float* x) { return {make_float4(x[0], x[1], x[2], x[3])}; }
-};
-template <int DT> struct Four {
-  uint2 u;
-  __device__ __forceinline__ void to(float* x) const {
-    const float2 f = unpack2<DT>(u.x), g = unpack2<DT>(u.y);
-    x[0] = f.x, x[1] = f.y, x[2] = g.x, x[3] = g.y;
+__device__ __forceinline__ float2 mul_f32x2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rd;\n\t"
+      "mov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+      "mul.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 neg(float2 a) { return make_float2(-a.x, -a.y); }
+
+// BYTES (8 or 16) of values as they are in memory, and as pairs of floats.
+template <int DT, int BYTES> struct Pack {
+  static constexpr int N = BYTES / (DT == DT_F32 ? 4 : 2), WORDS = BYTES / 4;
+  uint32_t u[WORDS];
+  __device__ __forceinline__ void load(const void* p) {
+    if constexpr (BYTES == 16) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p);
+      u[0] = v.x, u[1] = v.y, u[2] = v.z, u[3] = v.w;
+    } else {
+      const uint2 v = *reinterpret_cast<const uint2*>(p);
+      u[0] = v.x, u[1] = v.y;
+    }
   }
-  static __device__ __forceinline__ Four of(const float* x) {
-    return {make_uint2(pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3]))};
+  __device__ __forceinline__ void store(void* p) const {
+    if constexpr (BYTES == 16)
+      *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
+    else
+      *reinterpret_cast<uint2*>(p) = make_uint2(u[0], u[1]);
+  }
+  __device__ __forceinline__ void to(float2* x) const {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      if constexpr (DT == DT_F32)
+        x[i] = make_float2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
+      else
+        x[i] = unpack2<DT>(u[i]);
+    }
+  }
+  __device__ __forceinline__ void from(const float2* x) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      if constexpr (DT == DT_F32) {
+        u[2 * i] = __float_as_uint(x[i].x);
+        u[2 * i + 1] = __float_as_uint(x[i].y);
+      } else {
+        u[i] = pack2<DT>(x[i].x, x[i].y);
+      }
+    }
   }
 };
-template <int DT> __device__ __forceinline__ void load4(const void* p, float* x) {
-  reinterpret_cast<const Four<DT>*>(p)->to(x);
+// N floats as pairs
+template <int N> __device__ __forceinline__ void load_floats(const float* p, float2* x) {
+  if constexpr (N == 2) {
+    x[0] = *reinterpret_cast<const float2*>(p);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(p + i);
+      x[i / 2] = make_float2(v.x, v.y);
+      x[i / 2 + 1] = make_float2(v.z, v.w);
+    }
+  }
+}
+template <int N> __device__ __forceinline__ void load_weights(const void* w, int dt, int at, float2* x) {
+  if (dt == DT_F32) {
+    load_floats<N>(reinterpret_cast<const float*>(w) + at, x);
+  } else if (dt == DT_BF16) {
+    Pack<DT_BF16, 2 * N> p;
+    p.load(reinterpret_cast<const uint16_t*>(w) + at);
+    p.to(x);
+  } else {
+    Pack<DT_F16, 2 * N> p;
+    p.load(reinterpret_cast<const uint16_t*>(w) + at);
+    p.to(x);
+  }
 }
 
-__device__ __forceinline__ void load4_weight(const void* w, int dt, int at, float* x) {
-  if (dt == DT_F32)
-    load4<DT_F32>(reinterpret_cast<const float*>(w) + at, x);
-  else if (dt == DT_BF16)
-    load4<DT_BF16>(reinterpret_cast<const uint16_t*>(w) + at, x);
-  else
-    load4<DT_F16>(reinterpret_cast<const uint16_t*>(w) + at, x);
-}
+// Vector form: LANES lanes hold one head vector, two packs of it a lane, so neighbouring
+// lanes read neighbouring packs: the two sides of N rotary pairs (or N interleaved
+// pairs), so the rotation needs no other lane. A group of LANES lanes takes heads of one
+// token, `apart` heads from one to the next, so neighbouring groups read neighbouring
+// heads, the token's table row and cache slot are looked up once and the norm weights
+// stay in registers from head to head; the next AHEAD heads are being loaded meanwhile.
+//
+// Bytes in flight against registers: a 16-bit type has 16 values of 8 bytes each in the
+// works a lane, and does best with two heads ahead and two CTAs an SM (2048 tokens of
+// 32 + 8 + 8 heads of 128: 16.7 us; one ahead and four CTAs 24.7 us, with spills), float32
+// has half the values and wants the CTAs (16384 tokens: 121 us; two ahead and two 151 us).
+template <int DT> constexpr int kAhead = DT == DT_F32 ? 1 : 2;
+template <int DT> constexpr int kCtas = DT == DT_F32 ? 4 : 2;
 
-// Vector form: LANES lanes hold one head vector, two fours of it a lane: the two
-// sides of four rotary pairs (or four interleaved pairs), so the rotation needs no
-// other lane and only four cosines and sines; past rotary_dim, eight in a row. A group
-// of LANES lanes takes HPT heads of one token, `apart` heads from one to the next, so
-// neighbouring groups read neighbouring heads, the token's table row and cache slot
-// are looked up once and HPT heads' loads are in flight.
-template <int DT, int LANES, int HPT, bool INTER>
-__global__ void __launch_bounds__(256) qk_rope_vec_kernel(const RopeArgs a, int apart) {
-  constexpr int ES = DT == DT_F32 ? 4 : 2;
+template <int DT, int BYTES, int LANES, bool INTER>
+__global__ void __launch_bounds__(256, kCtas<DT>) qk_rope_vec_kernel(const RopeArgs a, int apart) {
+  using P = Pack<DT, BYTES>;
+  constexpr int ES = DT == DT_F32 ? 4 : 2, N = P::N, H = N / 2, AHEAD = kAhead<DT>;
   const int heads = a.Hq + (a.k_cache != nullptr ? 2 : 1) * a.Hkv;
   const int c = threadIdx.x % LANES;
   const unsigned group = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
   const unsigned t_raw = group / (unsigned)apart;
   const int h0 = (int)(group - t_raw * apart);
   const bool in = t_raw < a.tokens;    // lanes past the end still take part in shuffles
-  const bool live = in && c * 8 < a.D;
+  const bool live = in && c * 2 * N < a.D;
   const int64_t t = in ? t_raw : 0;
-  const int half = a.rot / 2;
-  const bool turns = live && c * 8 < a.rot;
-  const int d0 = INTER || c * 8 >= a.rot ? c * 8 : c * 4;
-  const int d1 = INTER || c * 8 >= a.rot ? c * 8 + 4 : half + c * 4;
+  // the dimensions of the lane's two packs, and what of them is rotated
+  const int half = a.rot / 2, rest = a.D - a.rot;
+  int d0, d1;
+  bool turn0, turn1;
+  if (INTER) {
+    d0 = c * N;
+    d1 = a.D / 2 + c * N;
+    turn0 = live && d0 < a.rot;
+    turn1 = live && d1 < a.rot;
+  } else {
+    turn0 = turn1 = live && c * N < half;
+    d0 = c * N < half ? c * N : a.rot + c * N - half;
+    d1 = c * N < half ? half + c * N : d0 + rest / 2;
+  }
 
   // strides fit 32 bits here, so an address is one wide multiply-add
   const int kv0 = a.Hq, v0 = a.Hq + a.Hkv;
@@ -117,23 +184,35 @@ __global__ void __launch_bounds__(256) qk_rope_vec_kernel(const RopeArgs a, int 
   const char* ks = reinterpret_cast<const char*>(a.k) + t * (int)a.k_st * ES;
   const char* vs = reinterpret_cast<const char*>(a.v) + t * (int)a.v_st * ES;
   const int qsh = (int)a.q_sh * ES, ksh = (int)a.k_sh * ES, vsh = (int)a.v_sh * ES;
-  Four<DT> x[HPT][2];
+  auto load = [&](int h, P (&x)[2]) {
+    if (!live || h >= heads) return;
+    const char* src = h < kv0 ? qs + (int64_t)h * qsh
+                    : h < v0 ? ks + (int64_t)(h - kv0) * ksh : vs + (int64_t)(h - v0) * vsh;
+    x[0].load(src + d0 * ES);
+    x[1].load(src + d1 * ES);
+  };
+  P x[AHEAD + 1][2] = {};
 #pragma unroll
-  for (int i = 0; i < HPT; ++i) {
-    const int h = h0 + i * apart;
-    x[i][0] = x[i][1] = Four<DT>{};
-    if (live && h < heads) {
-      const char* src = h < kv0 ? qs + (int64_t)h * qsh
-                      : h < v0 ? ks + (int64_t)(h - kv0) * ksh : vs + (int64_t)(h - v0) * vsh;
-      x[i][0] = *reinterpret_cast<const Four<DT>*>(src + d0 * ES);
-      x[i][1] = *reinterpret_cast<const Four<DT>*>(src + d1 * ES);
-    }
+  for (int i = 0; i < AHEAD; ++i) load(h0 + i * apart, x[i]);
+  float2 co[H], si[H];   // interleaved: of the first pack's pairs, then of the second's
+#pragma unroll
+  for (int j = 0; j < H; ++j) {   // no rotation: by nothing
+    co[j] = make_float2(1.f, 1.f);
+    si[j] = make_float2(0.f, 0.f);
   }
-  float co[4], si[4];
-  if (turns) {
-    const float* row = table_row(a, t);
-    load4<DT_F32>(row + c * 4, co);
-    load4<DT_F32>(row + half + c * 4, si);
+  const float* row = table_row(a, t);
+  if constexpr (INTER) {
+    if (turn0) {
+      load_floats<H>(row + d0 / 2, co);
+      load_floats<H>(row + half + d0 / 2, si);
+    }
+    if (turn1) {
+      load_floats<H>(row + d1 / 2, co + H / 2);
+      load_floats<H>(row + half + d1 / 2, si + H / 2);
+    }
+  } else if (turn0) {
+    load_floats<N>(row + c * N, co);
+    load_floats<N>(row + half + c * N, si);
   }
   char* const qd = reinterpret_cast<char*>(a.q_out) + t * (int)a.qo_st * ES;
   char *kd, *vd = nullptr;   // null: a cache slot out of range, not written
@@ -144,54 +223,75 @@ __global__ void __launch_bounds__(256) qk_rope_vec_kernel(const RopeArgs a, int 
   } else {
     const int64_t slot = slot_of(a, t);
     const unsigned page = (unsigned)slot / (unsigned)a.page_size;
-    const int row = (int)slot - (int)(page * a.page_size);
-    kd = slot < 0 ? nullptr : reinterpret_cast<char*>(a.k_cache) + ((int64_t)page * (int)a.kc_sp + (int64_t)row * (int)a.kc_sr) * ES;
-    vd = slot < 0 ? nullptr : reinterpret_cast<char*>(a.v_cache) + ((int64_t)page * (int)a.vc_sp + (int64_t)row * (int)a.vc_sr) * ES;
+    const int in_page = (int)slot - (int)(page * a.page_size);
+    kd = slot < 0 ? nullptr : reinterpret_cast<char*>(a.k_cache) + ((int64_t)page * (int)a.kc_sp + (int64_t)in_page * (int)a.kc_sr) * ES;
+    vd = slot < 0 ? nullptr : reinterpret_cast<char*>(a.v_cache) + ((int64_t)page * (int)a.vc_sp + (int64_t)in_page * (int)a.vc_sr) * ES;
     ksd = (int)a.kc_sh * ES;
     vsd = (int)a.vc_sh * ES;
   }
   const int qsd = (int)a.qo_sh * ES;
   const float inv_d = 1.f / (float)a.D;
+  const void* have = nullptr;
+  float2 w[2 * H];
 #pragma unroll
-  for (int i = 0; i < HPT; ++i) {
-    const int h = h0 + i * apart;
-    float y[8];
-    x[i][0].to(y);
-    x[i][1].to(y + 4);
-    float ss = 0.f;
+  for (int j = 0; j < 2 * H; ++j) w[j] = make_float2(1.f, 1.f);
+  // every lane of a warp takes the same number of steps
+  const int steps = (heads + apart - 1) / apart;
+  for (int step = 0; step < steps; ++step) {
+    const int h = h0 + step * apart;
+    load(h + AHEAD * apart, x[AHEAD]);
+    float2 y[2 * H];
+    x[0][0].to(y);
+    x[0][1].to(y + H);
+    float2 s2 = mul_f32x2(y[0], y[0]);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) ss = fmaf(y[j], y[j], ss);
+    for (int j = 1; j < 2 * H; ++j) s2 = fma_f32x2(y[j], y[j], s2);
+    float ss = s2.x + s2.y;
 #pragma unroll
     for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (!live || h >= heads) continue;
-    if (h < a.Hq + a.Hkv) {
-      const float r = rsqrtf(fmaf(ss, inv_d, a.eps));
-#pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] *= r;
-      const void* weight = h < a.Hq ? a.q_weight : a.k_weight;
-      if (weight != nullptr) {
-        float w[8];
-        load4_weight(weight, a.weight_dt, d0, w);
-        load4_weight(weight, a.weight_dt, d1, w + 4);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] *= w[j];
-      }
-      if (turns) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int p = INTER ? 2 * j : j, q = INTER ? 2 * j + 1 : j + 4;
-          const float u = y[p], v = y[q];
-          y[p] = u * co[j] - v * si[j];
-          y[q] = v * co[j] + u * si[j];
-        }
-      }
-    }
     char* const to = h < kv0 ? qd : h < v0 ? kd : vd;
-    if (to != nullptr) {
+    if (live && h < heads && to != nullptr) {
       char* const dst = to + (h < kv0 ? (int64_t)h * qsd
                               : h < v0 ? (int64_t)(h - kv0) * ksd : (int64_t)(h - v0) * vsd);
-      *reinterpret_cast<Four<DT>*>(dst + d0 * ES) = Four<DT>::of(y);
-      *reinterpret_cast<Four<DT>*>(dst + d1 * ES) = Four<DT>::of(y + 4);
+      if (h < v0) {
+        const float r = rsqrtf(fmaf(ss, inv_d, a.eps));
+        const void* weight = h < kv0 ? a.q_weight : a.k_weight;
+        if (weight != have) {
+          have = weight;
+          if (weight != nullptr) {
+            load_weights<N>(weight, a.weight_dt, d0, w);
+            load_weights<N>(weight, a.weight_dt, d1, w + H);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 2 * H; ++j) w[j] = make_float2(1.f, 1.f);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 2 * H; ++j) y[j] = mul_f32x2(mul_f32x2(y[j], make_float2(r, r)), w[j]);
+        if constexpr (INTER) {
+#pragma unroll
+          for (int j = 0; j < 2 * H; ++j) {
+            const float cj = j & 1 ? co[j / 2].y : co[j / 2].x, sj = j & 1 ? si[j / 2].y : si[j / 2].x;
+            y[j] = fma_f32x2(y[j], make_float2(cj, cj), mul_f32x2(make_float2(-y[j].y, y[j].x), make_float2(sj, sj)));
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < H; ++j) {
+            const float2 u = y[j], v = y[j + H];
+            y[j] = fma_f32x2(u, co[j], neg(mul_f32x2(v, si[j])));
+            y[j + H] = fma_f32x2(v, co[j], mul_f32x2(u, si[j]));
+          }
+        }
+        x[0][0].from(y);
+        x[0][1].from(y + H);
+      }
+      x[0][0].store(dst + d0 * ES);
+      x[0][1].store(dst + d1 * ES);
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      x[i][0] = x[i + 1][0];
+      x[i][1] = x[i + 1][1];
     }
   }
 }
@@ -244,25 +344,28 @@ __global__ void __launch_bounds__(256) qk_rope_any_kernel(const RopeArgs a) {
   }
 }
 
-template <int DT, int LANES, int HPT>
-cudaError_t launch_vec(const RopeArgs& a, int heads, cudaStream_t stream) {
-  const int apart = (heads + HPT - 1) / HPT;
+template <int DT, int BYTES, int LANES>
+cudaError_t launch_lanes(const RopeArgs& a, int num_sms, cudaStream_t stream) {
+  const int heads = a.Hq + (a.k_cache != nullptr ? 2 : 1) * a.Hkv;
+  // as many heads a lane group, up to eight, as leave every SM its CTAs
+  const int64_t groups = (int64_t)kCtas<DT> * num_sms * (256 / LANES);
+  const int64_t most = std::min<int64_t>(8, std::max<int64_t>(1, a.tokens * heads / groups));
+  const int apart = (heads + (int)most - 1) / (int)most;
   const int64_t blocks = (a.tokens * apart * LANES + 255) / 256;
   if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
   if (a.interleaved)
-    qk_rope_vec_kernel<DT, LANES, HPT, true><<<(unsigned)blocks, 256, 0, stream>>>(a, apart);
+    qk_rope_vec_kernel<DT, BYTES, LANES, true><<<(unsigned)blocks, 256, 0, stream>>>(a, apart);
   else
-    qk_rope_vec_kernel<DT, LANES, HPT, false><<<(unsigned)blocks, 256, 0, stream>>>(a, apart);
+    qk_rope_vec_kernel<DT, BYTES, LANES, false><<<(unsigned)blocks, 256, 0, stream>>>(a, apart);
   count_launch();
   return cudaGetLastError();
 }
 
-template <int DT, int LANES>
-cudaError_t launch_vec_heads(const RopeArgs& a, int num_sms, cudaStream_t stream) {
-  const int heads = a.Hq + (a.k_cache != nullptr ? 2 : 1) * a.Hkv;
-  // four heads a lane group once that still gives every SM two CTAs
-  const bool many = a.tokens * heads * LANES / (256 * 4) >= 2 * num_sms;
-  return many ? launch_vec<DT, LANES, 4>(a, heads, stream) : launch_vec<DT, LANES, 1>(a, heads, stream);
+template <int DT, int BYTES> cudaError_t launch_vec(const RopeArgs& a, int num_sms, cudaStream_t stream) {
+  constexpr int PER = 2 * Pack<DT, BYTES>::N;   // values a lane
+  return a.D <= 64 ? launch_lanes<DT, BYTES, 64 / PER>(a, num_sms, stream)
+       : a.D <= 128 ? launch_lanes<DT, BYTES, 128 / PER>(a, num_sms, stream)
+                    : launch_lanes<DT, BYTES, 256 / PER>(a, num_sms, stream);
 }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -271,16 +374,18 @@ template <int DT> cudaError_t launch_dt(const RopeArgs& a, int num_sms, cudaStre
   constexpr int ES = DT == DT_F32 ? 4 : 2;
   const int64_t strides = a.q_st | a.q_sh | a.k_st | a.k_sh | a.v_st | a.v_sh | a.qo_st | a.qo_sh |
                           a.ko_st | a.ko_sh | a.kc_sp | a.kc_sr | a.kc_sh | a.vc_sp | a.vc_sr | a.vc_sh;
-  const bool vec = a.D % 8 == 0 && a.rot % 8 == 0 && (strides * ES) % 16 == 0 &&
-                   aligned16(a.q) && aligned16(a.k) && aligned16(a.v) && aligned16(a.q_out) &&
-                   aligned16(a.k_out) && aligned16(a.k_cache) && aligned16(a.v_cache) &&
-                   aligned16(a.table) && aligned16(a.q_weight) && aligned16(a.k_weight);
-  // group numbers, slots and strides are 32-bit in the vector kernel
-  if (vec && a.tokens * (a.Hq + 2 * a.Hkv) <= 0x7fffffff && a.num_slots <= 0x7fffffff &&
-      (strides * ES) >> 31 == 0)
-    return a.D <= 64 ? launch_vec_heads<DT, 8>(a, num_sms, stream)
-         : a.D <= 128 ? launch_vec_heads<DT, 16>(a, num_sms, stream)
-                      : launch_vec_heads<DT, 32>(a, num_sms, stream);
+  const bool vec = (strides * ES) % 16 == 0 && aligned16(a.q) && aligned16(a.k) && aligned16(a.v) &&
+                   aligned16(a.q_out) && aligned16(a.k_out) && aligned16(a.k_cache) &&
+                   aligned16(a.v_cache) && aligned16(a.table) && aligned16(a.q_weight) &&
+                   aligned16(a.k_weight) &&
+                   // group numbers, slots and strides are 32-bit in the vector kernel
+                   a.tokens * (a.Hq + 2 * a.Hkv) <= 0x7fffffff && a.num_slots <= 0x7fffffff &&
+                   (strides * ES) >> 31 == 0;
+  // whole packs on each side of a rotary pair and past the rotated part
+  auto packs = [&](int n) { return a.rot % (2 * n) == 0 && (a.D - a.rot) % (2 * n) == 0; };
+  if (vec && packs(16 / ES)) return launch_vec<DT, 16>(a, num_sms, stream);
+  if constexpr (DT != DT_F32)
+    if (vec && packs(8 / ES)) return launch_vec<DT, 8>(a, num_sms, stream);
   const int heads = a.Hq + (a.k_cache != nullptr ? 2 : 1) * a.Hkv;
   const int64_t blocks = (a.tokens * heads + 7) / 8;
   if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;

@@ -33,13 +33,13 @@ def _refuse_grad(what: str) -> None:
     raise ValueError(f"{what} has no backward; call it under torch.no_grad()")
 
 
-def _call(fn, on: torch.Tensor, params: bytes) -> None:
-    """One library call on ``on``'s device and its current stream."""
-    if on.get_device() == torch.cuda.current_device():
-        rc = fn(params, _lib.stream_of(on))
+def _call(fn, device: int, params: bytes) -> None:
+    """One library call on ``device`` and its current stream."""
+    if device == torch.cuda.current_device():
+        rc = fn(params, _lib.stream_of_device(device))
     else:
-        with torch.cuda.device(on.device):
-            rc = fn(params, _lib.stream_of(on))
+        with torch.cuda.device(device):
+            rc = fn(params, _lib.stream_of_device(device))
     if rc:
         _lib.check(rc)
 
@@ -118,19 +118,19 @@ def qk_norm_rope(
     span, rotary = table.shape
     if not rotary or rotary % 2 or rotary > dim:
         raise ValueError("rotary_dim must be even and in [2, head_dim]")
-    tensors = [q, k, positions, table]
     weight_code = code
-    if q_weight is not None or k_weight is not None:
-        weights = [w for w in (q_weight, k_weight) if w is not None]
-        for w in weights:
-            if w.shape != (dim,) or w.dtype != weights[0].dtype:
-                raise ValueError("norm weights must share one dtype and have shape [head_dim]")
-        weight_code = _lib.dtype_code(weights[0].dtype)
-        tensors += weights
+    if q_weight is not None:
+        if q_weight.shape != (dim,) or k_weight is not None and q_weight.dtype != k_weight.dtype:
+            raise ValueError("norm weights must share one dtype and have shape [head_dim]")
+        weight_code = _lib.dtype_code(q_weight.dtype)
+    if k_weight is not None:
+        if k_weight.shape != (dim,):
+            raise ValueError("norm weights must share one dtype and have shape [head_dim]")
+        weight_code = _lib.dtype_code(k_weight.dtype)
     paged = k_cache is not None
-    kc = vc = (0, 0, 0)
     if (v is not None) != paged or (v_cache is not None) != paged or (slots is not None) != paged:
         raise ValueError("v, k_cache, v_cache and slots go together")
+    kc = vc = (0, 0, 0)
     if paged:
         if v.shape != kshape or v.dtype != dtype:
             raise ValueError("v must have the shape and dtype of k")
@@ -141,44 +141,62 @@ def qk_norm_rope(
         if v_cache.shape != cshape or not cshape[0] or not cshape[1]:
             raise ValueError("k_cache and v_cache must have identical non-empty shapes")
         kc, vc = k_cache.stride(), v_cache.stride()
-        if dim > 1 and (kc[3] != 1 or vc[3] != 1):
+        if kc[3] != 1 or vc[3] != 1:
             raise ValueError("a cache's head dimension must be contiguous")
         if slots.shape != (tokens,) or slots.dtype != torch.int64:
             raise ValueError("slots must be an int64 tensor [tokens]")
-        tensors += (v, k_cache, v_cache, slots)
-    if torch.is_grad_enabled() and any([t.requires_grad for t in tensors]):
+    if torch.is_grad_enabled() and (
+            q.requires_grad or k.requires_grad or table.requires_grad
+            or q_weight is not None and q_weight.requires_grad
+            or k_weight is not None and k_weight.requires_grad
+            or paged and (v.requires_grad or k_cache.requires_grad or v_cache.requires_grad)):
         _refuse_grad("qk_norm_rope")
     device = q.get_device()
-    if device < 0 or any([t.get_device() != device for t in tensors]):
-        _lib.require_cuda(*tensors)
-    q, k = _rows(q), _rows(k)
+    if device < 0 or k.get_device() != device or positions.get_device() != device or table.get_device() != device \
+            or q_weight is not None and q_weight.get_device() != device \
+            or k_weight is not None and k_weight.get_device() != device \
+            or paged and (v.get_device() != device or k_cache.get_device() != device
+                          or v_cache.get_device() != device or slots.get_device() != device):
+        _lib.require_cuda(q, k, positions, table, q_weight, k_weight, v, k_cache, v_cache, slots)
+    # the head dimension contiguous (a copy only where it is not), the small ones as a whole
+    qs, ks = q.stride(), k.stride()
+    if qs[2] != 1:
+        q = q.contiguous()
+        qs = q.stride()
+    if ks[2] != 1:
+        k = k.contiguous()
+        ks = k.stride()
     positions, table = positions.contiguous(), table.contiguous()
     if q_weight is not None:
         q_weight = q_weight.contiguous()
     if k_weight is not None:
         k_weight = k_weight.contiguous()
-    qs, ks, vs = q.stride(), k.stride(), (0, 0)
-    k_out = None
-    v_ptr = kc_ptr = vc_ptr = slots_ptr = pages = page_size = 0
     if heads_first:
         q_out = q.new_empty((q_heads, tokens, dim))
-        out = (dim, tokens * dim, dim, tokens * dim)
+        qo_t, qo_h, ko_t, ko_h = dim, tokens * dim, dim, tokens * dim
     else:
         q_out = q.new_empty(qshape)
-        out = (q_heads * dim, dim, kv_heads * dim, dim)
+        qo_t, qo_h, ko_t, ko_h = q_heads * dim, dim, kv_heads * dim, dim
     if paged:
-        v, slots = _rows(v), slots.contiguous()
+        k_out, k_out_ptr = None, 0
         vs = v.stride()
+        if vs[2] != 1:
+            v = v.contiguous()
+            vs = v.stride()
+        slots = slots.contiguous()
+        v_ptr, kc_ptr, vc_ptr, slots_ptr = v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr()
         pages, page_size = cshape[0], cshape[1]
-        v_ptr, slots_ptr = v.data_ptr(), slots.data_ptr()
-        kc_ptr, vc_ptr = k_cache.data_ptr(), v_cache.data_ptr()
     else:
         k_out = q.new_empty((kv_heads, tokens, dim) if heads_first else kshape)
-    _call(_lib.lib().fpv2_qk_norm_rope, q, _pack_rope(
+        k_out_ptr = k_out.data_ptr()
+        vs = (0, 0)
+        v_ptr = kc_ptr = vc_ptr = slots_ptr = pages = page_size = 0
+    _call(_lib.lib().fpv2_qk_norm_rope, device, _pack_rope(
         q.data_ptr(), k.data_ptr(), v_ptr, code, tokens, q_heads, kv_heads, dim, qs[0], qs[1], ks[0], ks[1],
         vs[0], vs[1], positions.data_ptr(), wide, table.data_ptr(), span, rotary, bool(interleaved),
-        _address(q_weight), _address(k_weight), weight_code, eps, q_out.data_ptr(), _address(k_out), *out,
-        kc_ptr, vc_ptr, kc[0], kc[1], kc[2], vc[0], vc[1], vc[2], slots_ptr, pages, page_size))
+        0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(),
+        weight_code, eps, q_out.data_ptr(), k_out_ptr, qo_t, qo_h, ko_t, ko_h, kc_ptr, vc_ptr,
+        kc[0], kc[1], kc[2], vc[0], vc[1], vc[2], slots_ptr, pages, page_size))
     return q_out, k_out
 
 
@@ -259,9 +277,11 @@ def decode_attention(
     lse = q.new_empty(shape[:-1], dtype=torch.float32) if return_lse else None
     if batch:
         qs, ks, vs = q.stride(), k_cache.stride(), v_cache.stride()
-        if qs[-1] != 1 or any([x & 1 for x in qs[:-1]]) or q.data_ptr() & 3:
+        token_stride = qs[1] if len(shape) == 4 else 0
+        if qs[-1] != 1 or (qs[0] | token_stride | qs[-2]) & 1 or q.data_ptr() & 3:
             q = q.clone(memory_format=torch.contiguous_format)
             qs = q.stride()
+            token_stride = qs[1] if len(shape) == 4 else 0
         if ks[3] != 1 or vs[3] != 1:
             raise ValueError("a cache's head dimension must be contiguous")
         if block_tables.stride(1) != 1:
@@ -269,8 +289,7 @@ def decode_attention(
         lengths = lengths.contiguous()
         nbytes = _workspace_bytes(new, q_heads, kv_heads, dim)
         workspace = q.new_empty(nbytes, dtype=torch.uint8)
-        token_stride = qs[1] if len(shape) == 4 else 0
-        _call(_lib.lib().fpv2_decode_attention, q, _pack_decode(
+        _call(_lib.lib().fpv2_decode_attention, device, _pack_decode(
             q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _lib.dtype_code(dtype), batch, new, q_heads,
             kv_heads, dim, qs[0], token_stride, qs[-2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
             block_tables.data_ptr(), block_tables.stride(0), width, lengths.data_ptr(), pages, page_size,
@@ -329,12 +348,14 @@ def sample_tokens(
     if logits.requires_grad and torch.is_grad_enabled():
         _refuse_grad("sample_tokens")
     device = logits.get_device()
-    if device < 0 or any([t is not None and t.get_device() != device for t in (noise, heat, k, p, least)]):
+    if device < 0 or noise.get_device() != device or heat is not None and heat.get_device() != device \
+            or k is not None and k.get_device() != device or p is not None and p.get_device() != device \
+            or least is not None and least.get_device() != device:
         _lib.require_cuda(logits, noise, heat, k, p, least)
     logits, noise = _rows(logits), _rows(noise)
     tokens = logits.new_empty(rows, dtype=torch.int64)
     logprobs = logits.new_empty(rows, dtype=torch.float32) if return_logprobs else None
-    _call(_lib.lib().fpv2_sample_tokens, logits, _pack_sample(
+    _call(_lib.lib().fpv2_sample_tokens, device, _pack_sample(
         logits.data_ptr(), code, rows, vocab, logits.stride(0), noise.data_ptr(), noise.stride(0),
         _address(heat), heat_all, _address(k), int(k_all), _address(p), p_all, _address(least), least_all,
         tokens.data_ptr(), _address(logprobs)))
