@@ -57,12 +57,6 @@ __device__ __forceinline__ float unorder(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
 
-__device__ __forceinline__ float lg2(float x) {
-  float y;
-  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // Larger of two packed pairs; of a number and a NaN the number.
 template <int DT> __device__ __forceinline__ uint32_t max_pair(uint32_t a, uint32_t b) {
   uint32_t r;
@@ -347,15 +341,11 @@ __device__ void sort_down(unsigned long long* v, int n, unsigned long long (&x)[
   }
 }
 
-// Once a CTA's candidates are gathered: tells the others their number and waits for
-// the cluster, then sets part_start to where each CTA's start in a list of all of them;
-// returns the number of all, the same in every thread of the cluster.
-__device__ int place_parts(cg::cluster_group& cl, Shared& sh) {
-  const int lane = threadIdx.x & 31, nblocks = (int)cl.num_blocks();
-  __syncthreads();
-  if ((int)threadIdx.x < nblocks) cl.map_shared_rank(&sh, threadIdx.x)->count_of[cl.block_rank()] = sh.count;
-  cl.sync();
-  const int c = lane < nblocks ? (int)sh.count_of[lane] : 0;
+// Sets part_start to where each CTA's candidates start in a list of all of them, from
+// lane r's number of CTA r's; returns the number of all. Every warp calls it; the other
+// warps may use part_start after a barrier.
+__device__ int place_parts(Shared& sh, int c) {
+  const int lane = threadIdx.x & 31;
   int upto = c;
 #pragma unroll
   for (int o = 1; o < kMaxCluster; o <<= 1) {
@@ -367,9 +357,26 @@ __device__ int place_parts(cg::cluster_group& cl, Shared& sh) {
   return __shfl_sync(0xffffffffu, upto, kMaxCluster - 1);
 }
 
+// Once a CTA's candidates are gathered: tells the others their number and waits for the
+// cluster; then as above.
+__device__ int exchange_parts(cg::cluster_group& cl, Shared& sh) {
+  const int lane = threadIdx.x & 31, nblocks = (int)cl.num_blocks();
+  __syncthreads();
+  if ((int)threadIdx.x < nblocks) cl.map_shared_rank(&sh, threadIdx.x)->count_of[cl.block_rank()] = sh.count;
+  cl.sync();
+  return place_parts(sh, lane < nblocks ? (int)sh.count_of[lane] : 0);
+}
+
+// The largest number of candidates a CTA has.
+__device__ __forceinline__ int largest_part(Shared& sh, int nblocks) {
+  int most = 0;
+  for (int q = 0; q < nblocks; ++q) most = max(most, (int)sh.count_of[q]);
+  return most;
+}
+
 // Sorts the cluster's candidates: afterwards every CTA has all of them, each CTA's part
 // (from part_start) sorted (descending, ties by index ascending) with the running weight
-// of the part before each. All CTAs call it, after place_parts().
+// of the part before each. All CTAs call it, after part_start was set.
 __device__ void merge_lists(cg::cluster_group& cl, Shared& sh, const RowState& row, unsigned long long* list,
                             float* ahead) {
   const int tid = threadIdx.x, me = (int)cl.block_rank(), nblocks = (int)cl.num_blocks();
@@ -456,11 +463,6 @@ __device__ __forceinline__ void for_places(Shared& sh, const unsigned long long*
 __device__ __forceinline__ void gather(Shared& sh, unsigned long long* list, float x, int64_t at) {
   const unsigned i = atomicAdd(&sh.count, 1u);
   if (i < kList) list[i] = pack(order(x), at);
-}
-
-// Starts bringing `bytes` from p (both multiples of 16) into L2.
-__device__ __forceinline__ void prefetch_l2_bulk(const void* p, unsigned bytes) {
-  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
 }
 
 __device__ __forceinline__ void prefetch_l2(const void* p) {
@@ -707,11 +709,16 @@ __device__ float min_p_logit(const RowState& row) {
 // Top-p over the whole row: cut after the shortest prefix with p of the weight.
 // Returns false (everywhere) when the crossing bin does not fit the list.
 template <int DT>
-__device__ bool nucleus(cg::cluster_group& cl, Shared& sh, const Slice<DT>& sl, const RowState& row,
+__device__ bool nucleus(cg::cluster_group& cl, Shared& sh, const Slice<DT>& sl, RowState row,
                         unsigned long long* list, float* ahead, double& whole, Cut& cut) {
   constexpr int VE = Slice<DT>::VE;
   const int tid = threadIdx.x;
+  // Tokens with less than (1 - p) / vocab of the largest one's weight do not reach 1 - p of
+  // all weight together, so the prefix ends above them: the bins span the rest.
+  const float span = fminf(kSpan, logf((float)sl.vocab) - logf(fmaxf(1.f - row.top_p, 1e-9f)) + 0.1f);
+  row.scale *= kSpan / span;
   float s[1] = {0.f};
+#pragma unroll 2
   for (int j = tid; j < sl.chunks; j += kThreads) {
     float x[VE];
     sl.get(j, x);
@@ -719,7 +726,6 @@ __device__ bool nucleus(cg::cluster_group& cl, Shared& sh, const Slice<DT>& sl, 
     for (int i = 0; i < VE; ++i) {
       s[0] += row.weight(x[i]);
       const int b = __float_as_int(row.place(x[i])) & (kBins - 1);
-      // past the last bin there is no weight to speak of
       if (b < kBins - 1) atomicAdd(&sh.hist[b], 1u);
     }
   }
@@ -734,23 +740,36 @@ __device__ bool nucleus(cg::cluster_group& cl, Shared& sh, const Slice<DT>& sl, 
       c1 += u.y;
     }
   whole = all_sums(cl, sh, 0);
-  if (tid == 0) sh.found_bin = kBins - 2;
-  // a bin weighs about its count times its middle's weight
+  if (tid == 0) sh.found_bin = kBins - 3;
+  // A bin weighs about its count times its middle's weight. The crossing is looked for in
+  // two bins, the one where the estimates cross and the neighbour on the nearer side: the
+  // largest tokens are few, and where they lie in their bins is not averaged out.
   const float per_bin = row.to_log2 / row.scale;
   const double m0 = (double)c0 * ex2(-(tid == 0 ? 0.25f : 2.f * tid) * per_bin);
   const double m1 = (double)c1 * ex2(-(2.f * tid + 1.f) * per_bin);
   const double start = block_before(sh, m0 + m1);
   const double target = (double)row.top_p * whole;
-  if (start + m0 >= target)
-    atomicMin(&sh.found_bin, min(2u * tid, (unsigned)kBins - 2u));
-  else if (start + m0 + m1 >= target)
-    atomicMin(&sh.found_bin, min(2u * tid + 1u, (unsigned)kBins - 2u));
+  if (start + m0 + m1 >= target) {
+    const bool second = start + m0 < target;
+    const bool low_half = target - start - (second ? m0 : 0.0) < 0.5 * (second ? m1 : m0);
+    const int lower = 2 * tid + (second ? 1 : 0) - (low_half ? 1 : 0);
+    atomicMin(&sh.found_bin, (unsigned)min(max(lower, 0), kBins - 3));
+  }
   __syncthreads();
-  int bin = (int)sh.found_bin, moved = 0;
+  int bin = (int)sh.found_bin, moved = 0;   // the lower one of the two
   for (int tries = 0; tries < 16; ++tries) {
-    // the weight above the bin, and the bin's logits
+    // how many of the bins' logits each CTA has
+    int mine = 0;
+    if ((tid & 31) < (int)cl.num_blocks()) {
+      const unsigned* hist = cl.map_shared_rank(&sh, tid & 31)->hist;
+      mine = (int)(hist[bin] + hist[bin + 1]);
+    }
+    const int n = place_parts(sh, mine);
+    if (n > kList) return false;
+    // the weight above the bins, and the bins' logits
     const float at_bin = 8388608.f + (float)bin;
     float a[1] = {0.f};
+#pragma unroll 2
     for (int j = tid; j < sl.chunks; j += kThreads) {
       float x[VE];
       sl.get(j, x);
@@ -758,15 +777,13 @@ __device__ bool nucleus(cg::cluster_group& cl, Shared& sh, const Slice<DT>& sl, 
       for (int i = 0; i < VE; ++i) {
         const float p = row.place(x[i]);
         if (p < at_bin) a[0] += row.weight(x[i]);
-        if (p == at_bin) gather(sh, list, x[i], sl.index(j) + i);
+        if (p == at_bin || p == at_bin + 1.f) gather(sh, list, x[i], sl.index(j) + i);
       }
     }
     const int slot = 1 + (tries & 1);   // the other one may still be read
     block_sum(sh, a, slot);
-    const int n = place_parts(cl, sh);
-    if (n > kList) return false;
-    const double above = all_sums(cl, sh, slot);
     merge_lists(cl, sh, row, list, ahead);
+    const double above = all_sums(cl, sh, slot);
     // the last one that the prefix has to take: the smallest with less than the target before it
     unsigned long long least = 0;   // inverted, so that the smallest is the best
     for_places(sh, list, ahead, (int)cl.block_rank(), (int)cl.num_blocks(), [&](int, unsigned long long v, int, float before) {
@@ -780,12 +797,13 @@ __device__ bool nucleus(cg::cluster_group& cl, Shared& sh, const Slice<DT>& sl, 
     least = warp_best((tid & 31) < (int)cl.num_blocks() ? sh.least_of[tid & 31] : 0ull);
     if (tid == 0) sh.count = 0;
     __syncthreads();
-    // The estimate of the bin is off by a rounding at most, so a step that would turn back
-    // has met the crossing.
+    // a step that would turn back has met the crossing
     if (above >= target && bin > 0 && moved <= 0) {
-      bin += moved = -1;
-    } else if (total < target && bin < kBins - 2 && moved >= 0) {
-      bin += moved = 1;
+      moved = -1;
+      bin = max(bin - 2, 0);
+    } else if (total < target && bin < kBins - 3 && moved >= 0) {
+      moved = 1;
+      bin = min(bin + 2, kBins - 3);
     } else {
       if (least == 0) {   // nothing of the bin is needed
         cut.x = row.top - ((float)bin - 0.5f) / row.scale;
@@ -804,38 +822,46 @@ __device__ bool nucleus(cg::cluster_group& cl, Shared& sh, const Slice<DT>& sl, 
 // pack(order(score), index), thread by thread. With sum_here the weights of all tokens
 // are added to `sum`.
 //
-// A thread's noise is loaded 16 values ahead of their use. Scores are first taken to
-// about 1e-4, in powers of two, and a thread keeps its best chunk of them; then only
-// the chunks within a margin of the CTA's best are scored exactly.
+// A thread's noise is loaded 16 values ahead of their use. Scores are first taken
+// roughly, in powers of two: for e = 2^k (1 + m) the exponent and mantissa bits read as one
+// number are k + m = log2 e - [0, 0.0861], three integer and float operations in place of
+// the special-function unit's, which the weights' exponentials keep busy. A thread keeps
+// its best chunk of them; then only the chunks within reach of the CTA's best are scored
+// exactly.
 template <int DT, bool ALL>
 __device__ __forceinline__ unsigned long long race(Shared& sh, const Slice<DT>& sl, const RowState& row,
                                                    const Cut cut, const float* noise, bool sum_here, float& sum) {
   constexpr int VE = Slice<DT>::VE, DEPTH = 16 / VE;
+  constexpr float kReach = 0.0861f + 1e-3f;   // the log's error, and the rounding of scores to about 500
   const int tid = threadIdx.x;
+  // chunks whose noise is whole 16-byte words: all but a row's first and last, or none
   const bool aligned = reinterpret_cast<uintptr_t>(noise + sl.first) % 16 == 0;
-  float e[DEPTH][VE];
-  auto fetch = [&](int j, float (&to)[VE]) {
+  const int whole0 = sl.chunks > 0 && !sl.inside(0) ? 1 : 0;
+  const int whole1 = !aligned ? 0 : sl.chunks > 0 && !sl.inside(sl.chunks - 1) ? sl.chunks - 1 : sl.chunks;
+  const int4* words = reinterpret_cast<const int4*>(noise + sl.first);
+  int e[DEPTH][VE];   // bit patterns
+  auto fetch = [&](int j, int (&to)[VE]) {
 #pragma unroll
-    for (int i = 0; i < VE; ++i) to[i] = INFINITY;
+    for (int i = 0; i < VE; ++i) to[i] = 0x7F800000;
     if (j >= sl.chunks || (!ALL && !(sl.highest(j) >= cut.x))) return;
-    const int64_t at = sl.index(j);
-    if (aligned && sl.inside(j)) {
+    if (j >= whole0 && j < whole1) {
 #pragma unroll
       for (int i = 0; i < VE; i += 4) {
-        const float4 f = __ldcs(reinterpret_cast<const float4*>(noise + at + i));
+        const int4 f = __ldcs(words + j * (VE / 4) + i / 4);
         to[i] = f.x, to[i + 1] = f.y, to[i + 2] = f.z, to[i + 3] = f.w;
       }
     } else {
+      const int64_t at = sl.index(j);
 #pragma unroll
       for (int i = 0; i < VE; ++i)
-        if (at + i >= 0 && at + i < sl.vocab) to[i] = noise[at + i];
+        if (at + i >= 0 && at + i < sl.vocab) to[i] = __float_as_int(noise[at + i]);
     }
   };
 #pragma unroll
   for (int u = 0; u < DEPTH; ++u) fetch(tid + u * kThreads, e[u]);
   float best = -INFINITY, second = -INFINITY;   // of the thread's chunks
-  int best_j = 0;
-  bool any = false, odd = false;
+  int best_j = 0, least = 0x7F800000;
+  bool any = false;
   for (int jw = tid; jw < sl.chunks; jw += DEPTH * kThreads) {
 #pragma unroll
     for (int u = 0; u < DEPTH; ++u) {
@@ -843,12 +869,15 @@ __device__ __forceinline__ unsigned long long race(Shared& sh, const Slice<DT>& 
       if (j < sl.chunks) {
         float x[VE], near = -INFINITY;
         sl.get(j, x);
-        const int at = (int)sl.index(j);
+        const int at = (int)sl.first + j * VE;
 #pragma unroll
         for (int i = 0; i < VE; ++i) {
           const float t = (x[i] - row.top) * row.to_log2;
           if (sum_here) sum += ex2(t);
-          const float score = t - lg2(e[u][i]);
+          least = min(least, e[u][i]);
+          // 2^23 + bits / 2^8, exactly: 2^15 (k + m) and a constant
+          const float bits = __int_as_float(0x4B000000 | e[u][i] >> 8);
+          const float score = fmaf(bits, -0x1p-15f, t);
           if (ALL) {
             near = fmaxf(near, score);
           } else if (cut.keeps(x[i], at + i)) {
@@ -856,8 +885,6 @@ __device__ __forceinline__ unsigned long long race(Shared& sh, const Slice<DT>& 
             any = true;
           }
         }
-        // (a noise of 0 or below the normal range: an infinite score, which says nothing)
-        odd |= near == INFINITY;
         if (near > best) {
           second = best;
           best = near;
@@ -869,32 +896,39 @@ __device__ __forceinline__ unsigned long long race(Shared& sh, const Slice<DT>& 
       }
     }
   }
-  const unsigned high = __reduce_max_sync(0xffffffffu, order(best));
   any |= ALL && sl.chunks > 0;
+  const unsigned high = __reduce_max_sync(0xffffffffu, order(best));
   __syncthreads();
   if ((tid & 31) == 0) sh.warp_best[tid >> 5] = high;
-  odd = __syncthreads_or(odd);
+  // noise that is no positive normal number has no such logarithm: all is scored exactly
+  bool odd = __syncthreads_or(least < 0x00800000);
   any = __syncthreads_or(any);
   const unsigned cta =
       __reduce_max_sync(0xffffffffu, (unsigned)sh.warp_best[tid & (kWarps - 1)]);
-  const float bar = unorder(cta) - 3e-3f;
-  // nothing within reach of a number: noise out of contract, all of it is scored
+  const float bar = unorder(cta) - kReach;
   odd |= any && !(bar > -INFINITY);
   unsigned long long best_key = 0;
   if (odd || best >= bar) {
     const bool every = odd || second >= bar;
     for (int j = every ? tid : best_j; j < sl.chunks; j += every ? kThreads : 0x40000000) {
-      float x[VE];
+      float x[VE], n[VE];
       sl.get(j, x);
+      const int at = (int)sl.first + j * VE;
+#pragma unroll
+      for (int i = 0; i < VE; ++i) n[i] = at + i >= 0 && at + i < sl.vocab ? noise[at + i] : INFINITY;
 #pragma unroll 1
       for (int i = 0; i < VE; ++i) {
-        float mine = x[0];
+        float mine = x[0], its = n[0];
 #pragma unroll
-        for (int q = 1; q < VE; ++q) mine = i == q ? x[q] : mine;
-        const int64_t at = sl.index(j) + i;
-        if (!cut.keeps(mine, (int)at)) continue;
+        for (int q = 1; q < VE; ++q) {
+          mine = i == q ? x[q] : mine;
+          its = i == q ? n[q] : its;
+        }
+        const float bits = __int_as_float(0x4B000000 | __float_as_int(its) >> 8);
+        if (!cut.keeps(mine, at + i) || (!odd && fmaf(bits, -0x1p-15f, (mine - row.top) * row.to_log2) < bar))
+          continue;
         const float z = row.z(mine);
-        if (z > -INFINITY) best_key = max(best_key, pack(order(race_score(z, noise[at])), at));
+        if (z > -INFINITY) best_key = max(best_key, pack(order(race_score(z, its)), at + i));
       }
     }
   }
@@ -971,14 +1005,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a,
   const int need = (k_set + nblocks - 1) / nblocks;
   const bool use_list = !single && use_k && need <= kThreads;
   const float* noise = a.noise + r * a.noise_stride;
-  if (!single && !use_k) {
-    // much or all of the noise is going to be read, after the logits were looked at
-    const int64_t n0 = max((int64_t)0, sl.first), n1 = min((int64_t)a.vocab, sl.index(sl.chunks));
-    const uintptr_t p0 = (reinterpret_cast<uintptr_t>(noise + n0) + 15) / 16 * 16;
-    const uintptr_t p1 = reinterpret_cast<uintptr_t>(noise + n1) / 16 * 16;
-    const uintptr_t p = p0 + (uintptr_t)tid * 2048;
-    if (p < p1) prefetch_l2_bulk(reinterpret_cast<const void*>(p), (unsigned)min((uintptr_t)2048, p1 - p));
-  }
   sh.hist[tid] = sh.hist[tid + kThreads] = 0;
   if (tid == 0) sh.count = 0;
   // A thread reads back its own chunks only, here and below, but for tie_index().
@@ -1082,7 +1108,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a,
     }
     if (want_sum) block_sum(sh, s);
     part = sh.row_sums[0];
-    const int n = place_parts(cl, sh);
+    const int n = exchange_parts(cl, sh);
     if (n <= kFew) {
       // CTA 0 alone: it gets the candidates and counts for each the larger ones and their
       // weight, two threads a candidate. Weights are whole numbers here, as the
@@ -1128,34 +1154,35 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a,
       best = block_best(sh, kept && z > -INFINITY ? (unsigned long long)order(race_score(z, e)) << 32 | (uint32_t)v
                                                   : 0ull);
       if (tid == 0) sh.best_of[0] = best;
-    } else if (n <= kList) {
+    } else if (n <= kList && largest_part(sh, nblocks) <= kBins) {
       done = true;
       merge_lists(cl, sh, row, list, ahead);
+      // the weight before each of this CTA's candidates, -1 past the k-th, and the weight of
+      // the first k: what is before the last of them, and its own
+      float* weight_before = reinterpret_cast<float*>(sh.hist);
+      const int last = min(n, k_set) - 1;
+      for_places(sh, list, ahead, rank, nblocks, [&](int i, unsigned long long v, int place, float before) {
+        weight_before[i] = place < k_set ? before : -1.f;
+        if (place != last || !use_p) return;
+        const double share = (double)before + (double)row.weight(unorder((uint32_t)(v >> 32)));
+        for (int q = 0; q < nblocks; ++q) cl.map_shared_rank(&sh, q)->share = share;
+      });
       float target = INFINITY;
       if (use_p) {
-        // the weight of the first k: what is before the last of them, and its own
-        const int last = min(n, k_set) - 1;
-        for_places(sh, list, ahead, rank, nblocks, [&](int, unsigned long long v, int place, float before) {
-          if (place != last) return;
-          const double share = (double)before + (double)row.weight(unorder((uint32_t)(v >> 32)));
-          for (int q = 0; q < nblocks; ++q) cl.map_shared_rank(&sh, q)->share = share;
-        });
         cl.sync();
         target = (float)((double)row.top_p * sh.share);
+      } else {
+        __syncthreads();
       }
-      // which are kept, then their race with all noise loads in flight at once
-      unsigned char* kept = reinterpret_cast<unsigned char*>(sh.hist);
-      for_places(sh, list, ahead, rank, nblocks, [&](int i, unsigned long long v, int place, float before) {
-        const float z = row.z(unorder((uint32_t)(v >> 32)));
-        kept[i] = place < k_set && z > -INFINITY && (place == 0 || (before < target && expf(z) >= row.min_p));
-      });
-      __syncthreads();
       const int start = sh.part_start[rank], own = sh.part_start[rank + 1] - start;
       for (int i = tid; i < own; i += kThreads) {
-        if (!kept[i]) continue;
+        const float before = weight_before[i];
+        if (!(before >= 0.f)) continue;
         const unsigned long long v = list[start + i];
-        const float score = race_score(row.z(unorder((uint32_t)(v >> 32))), noise[(int)~(uint32_t)v]);
-        best = max(best, (unsigned long long)order(score) << 32 | (uint32_t)v);
+        const float e = noise[(int)~(uint32_t)v], z = row.z(unorder((uint32_t)(v >> 32)));
+        // nothing is before the first one alone
+        if (before == 0.f || (z > -INFINITY && before < target && expf(z) >= row.min_p))
+          best = max(best, (unsigned long long)order(race_score(z, e)) << 32 | (uint32_t)v);
       }
       best = block_best(sh, best);
       cl.sync();   // the lists and part weights were read
@@ -1247,7 +1274,7 @@ template <int DT> cudaError_t launch_dt(const SampleArgs& a, int num_sms, cudaSt
   // by one CTA an SM, or read again each time.
   int n = 1;
   while (n < kMaxCluster && (chunks + n - 1) / n * 16 > kSliceTwo) n *= 2;
-  while (n < kMaxCluster && (int64_t)a.rows * n * 2 <= num_sms) n *= 2;
+  while (n < kMaxCluster && (int64_t)a.rows * n * 2 <= 2 * num_sms) n *= 2;
   const int64_t per = (chunks + n - 1) / n;
   const bool held = per * 16 <= kSliceOne;
   const int smem = kListBytes + (held ? (int)per * 16 : 0);
