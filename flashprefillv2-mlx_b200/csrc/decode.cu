@@ -216,6 +216,8 @@ __global__ void __launch_bounds__(Shape<D>::NW * 32, 1) decode_kernel(const Deco
   constexpr float kSlack = 8.f;
   using T = typename Elem<DT>::T;
   extern __shared__ __align__(16) unsigned char smem[];
+  // launched while the kernel before it in the stream still runs: wait for its results
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;   // mma fragments: rows g and g + 8, column pair c
@@ -570,18 +572,20 @@ __global__ void __launch_bounds__(Shape<D>::NW * 32, 1) decode_kernel(const Deco
 
 // Joins the pieces of the sequences that were cut:
 //   m = max m_i,  o = sum 2^(m_i - m) o_i / sum 2^(m_i - m) l_i,
-// and fills the rows of empty sequences. A warp takes a row (ROW_CTA: a CTA, for few rows
-// of many pieces each).
+// and fills the rows of empty sequences. A warp takes a row, or, for few rows of many
+// pieces each (ROW_CTA), a CTA takes 32 dimensions of a row, a warp an eighth of the
+// pieces.
 // It fits beside the first kernel's CTAs, so it is launched and has its part boundaries
 // when that one ends.
 
 template <int DT, int D, bool ROW_CTA>
 __global__ void __launch_bounds__(256, 4) decode_join_kernel(const DecodeArgs a, int parts) {
-  constexpr int TK = Shape<D>::TK, NV = D / 32, WARPS = 8, WPR = ROW_CTA ? WARPS : 1;
-  __shared__ float red[WPR][D + 1];
+  constexpr int TK = Shape<D>::TK, NV = ROW_CTA ? 1 : D / 32, WARPS = 8, WPR = ROW_CTA ? WARPS : 1;
+  __shared__ float red[WPR][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % WPR;
   const int R = a.G * a.T, per = 8 * blocks_of(R, D), groups = row_groups(R, D), cols = a.Hkv * groups;
-  const unsigned id = ROW_CTA ? blockIdx.x : blockIdx.x * WARPS + warp;   // (b * Hkv + h) * R + r
+  const unsigned id = ROW_CTA ? blockIdx.x / (D / 32) : blockIdx.x * WARPS + warp;   // (b * Hkv + h) * R + r
+  const int d0 = lane + (ROW_CTA ? (int)(blockIdx.x % (D / 32)) * 32 : 0);   // the lane's first dimension
   const unsigned head = id / (unsigned)R;
   const int r = (int)(id - head * R), b = (int)(head / (unsigned)a.Hkv), h = (int)(head - (unsigned)b * a.Hkv);
   if (b >= a.B) return;
@@ -593,6 +597,7 @@ __global__ void __launch_bounds__(256, 4) decode_join_kernel(const DecodeArgs a,
   const int p1 = n > 0 ? (int)quotient(before + kSeqCost + n - 1, chunk) : p0;
   const bool late = before >= (int64_t)p0 * chunk;   // the sequence starts in its first part
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (n > 0 && p0 == p1) return;   // finished by its warp
   const float2* ml = reinterpret_cast<const float2*>(a.workspace);
   const float* po = reinterpret_cast<const float*>(ml + (int64_t)parts * 2 * cols * per);
@@ -606,7 +611,7 @@ __global__ void __launch_bounds__(256, 4) decode_join_kernel(const DecodeArgs a,
   float acc[NV], l = 0.f, base = 0.f;
 #pragma unroll
   for (int j = 0; j < NV; ++j) acc[j] = 0.f;
-  constexpr int U = NV <= 2 ? 8 : NV <= 4 ? 4 : 2;   // pieces in flight a warp
+  constexpr int U = NV == 1 ? 10 : NV == 2 ? 8 : NV <= 4 ? 4 : 2;   // pieces in flight a warp
   for (int i0 = sub; i0 < count; i0 += U * WPR) {
     float2 x[U];
     float v[U][NV];
@@ -620,7 +625,7 @@ __global__ void __launch_bounds__(256, 4) decode_join_kernel(const DecodeArgs a,
         const int64_t at = slot_row(i);
         x[u] = ml[at];
 #pragma unroll
-        for (int j = 0; j < NV; ++j) v[u][j] = po[at * D + lane + 32 * j];
+        for (int j = 0; j < NV; ++j) v[u][j] = po[at * D + d0 + 32 * j];
       }
     }
     if (i0 == sub) {   // the maximum, while the first outputs are on their way
@@ -638,16 +643,14 @@ __global__ void __launch_bounds__(256, 4) decode_join_kernel(const DecodeArgs a,
   }
   if constexpr (ROW_CTA) {
     // (a warp without pieces did not reduce its maximum: the first has one and writes)
-#pragma unroll
-    for (int j = 0; j < NV; ++j) red[sub][lane + 32 * j] = acc[j];
-    if (lane == 0) red[sub][D] = l;
+    red[sub][lane] = acc[0];
+    if (lane == 0) red[sub][32] = l;
     __syncthreads();
     if (sub != 0) return;
 #pragma unroll
     for (int w = 1; w < WPR; ++w) {
-#pragma unroll
-      for (int j = 0; j < NV; ++j) acc[j] += red[w][lane + 32 * j];
-      l += red[w][D];
+      acc[0] += red[w][lane];
+      l += red[w][32];
     }
   }
   const bool any = l > 0.f || l != l;
@@ -657,8 +660,8 @@ __global__ void __launch_bounds__(256, 4) decode_join_kernel(const DecodeArgs a,
   using E = Elem<DT>;
   typename E::T* dst = reinterpret_cast<typename E::T*>(a.out) + row * D;
 #pragma unroll
-  for (int j = 0; j < NV; ++j) dst[lane + 32 * j] = E::from_f(acc[j] * inv);
-  if (a.lse != nullptr && lane == 0) a.lse[row] = any ? m * kLn2 + logf(l) : -INFINITY;
+  for (int j = 0; j < NV; ++j) dst[d0 + 32 * j] = E::from_f(acc[j] * inv);
+  if (a.lse != nullptr && d0 == 0) a.lse[row] = any ? m * kLn2 + logf(l) : -INFINITY;
 }
 
 // Parts of the tile stream: with `cols` warps for each part, one wave of warps.
@@ -673,20 +676,22 @@ template <int D> size_t workspace_for(int rows, int Hkv) {
 }
 
 
-template <int DT, int D, bool ROW_CTA>
-cudaError_t launch_join(const DecodeArgs& a, int parts, cudaStream_t stream) {
-  const int64_t rows = (int64_t)a.B * a.Hq * a.T, blocks = ROW_CTA ? rows : (rows + 7) / 8;
-  if (rows > 0x7fffffff) return cudaErrorInvalidConfiguration;
+// A launch whose CTAs may come up while the kernel before it in the stream still runs;
+// both kernels here wait for that one's end before they touch memory it may write.
+template <typename... P>
+cudaError_t launch_early(void (*kernel)(P...), int64_t blocks, int threads, int smem, cudaStream_t stream, P... p) {
+  if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)blocks);
-  cfg.blockDim = dim3(256);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, decode_join_kernel<DT, D, ROW_CTA>, a, parts);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p...);
   if (e == cudaSuccess) count_launch();
   return e;
 }
@@ -697,15 +702,12 @@ template <int DT, int D, int NB> cudaError_t launch_blocks(const DecodeArgs& a, 
   static std::atomic<uint64_t> allowed{0};
   cudaError_t e = allow_shared(reinterpret_cast<const void*>(decode_kernel<DT, D, NB>), SMEM, allowed);
   if (e != cudaSuccess) return e;
-  const int64_t blocks = ((int64_t)parts * cols + NW - 1) / NW;
-  if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  decode_kernel<DT, D, NB><<<(unsigned)blocks, NW * 32, SMEM, stream>>>(a, parts);
-  e = cudaGetLastError();
+  e = launch_early(decode_kernel<DT, D, NB>, ((int64_t)parts * cols + NW - 1) / NW, NW * 32, SMEM, stream, a, parts);
   if (e != cudaSuccess) return e;
-  count_launch();
-  // few rows with many pieces each: a CTA a row; else a warp a row
-  return parts / a.B >= 16 ? launch_join<DT, D, true>(a, parts, stream)
-                           : launch_join<DT, D, false>(a, parts, stream);
+  const int64_t rows = (int64_t)a.B * a.Hq * a.T;
+  // few rows with many pieces each: a CTA 32 dimensions of a row; else a warp a row
+  return parts / a.B >= 16 ? launch_early(decode_join_kernel<DT, D, true>, rows * (D / 32), 256, 0, stream, a, parts)
+                           : launch_early(decode_join_kernel<DT, D, false>, (rows + 7) / 8, 256, 0, stream, a, parts);
 }
 
 template <int DT, int D> cudaError_t launch_dim(const DecodeArgs& a, cudaStream_t stream) {
