@@ -70,14 +70,15 @@ template <int DT> constexpr uint32_t kMinusInfPair = DT == DT_BF16 ? 0xFF80FF80u
 
 // One row's slice in a CTA: chunks of 16 bytes, aligned in memory, so the first and
 // the last chunk of a row may be partly outside it (filled with -inf).
-template <int DT> struct Slice {
+template <int DT, bool HELD> struct Slice {
   static constexpr int VE = DT == DT_F32 ? 4 : 8;
   using T = typename Elem<DT>::T;
   const T* row;
-  const uint4* held;   // shared memory, null when the slice is read from global each time
+  uint4* held;         // shared memory (HELD), else the slice is read from global each time
   int64_t first;       // index of the first element of chunk 0 (may be negative)
   int chunks, vocab;
   bool infinite;       // the row's maximum is +inf: such logits count as 0, others as -inf
+                       // (and are held so)
 
   __device__ __forceinline__ int64_t index(int j) const { return first + (int64_t)j * VE; }
   __device__ __forceinline__ bool inside(int j) const {
@@ -93,9 +94,13 @@ template <int DT> struct Slice {
       e[i] = at + i >= 0 && at + i < vocab ? row[at + i] : Elem<DT>::from_f(-INFINITY);
     return u;
   }
+  __device__ __forceinline__ uint4 at(int j) const {
+    if constexpr (HELD) return held[j];
+    return load(j);
+  }
   // the chunk as floats, NaN as -inf
   __device__ __forceinline__ void get(int j, float (&x)[VE]) const {
-    const uint4 u = held != nullptr ? held[j] : load(j);
+    const uint4 u = at(j);
     const uint32_t r[4] = {u.x, u.y, u.z, u.w};
     if constexpr (DT == DT_F32) {
 #pragma unroll
@@ -108,14 +113,35 @@ template <int DT> struct Slice {
         x[2 * i + 1] = f.y;
       }
     }
-    if (infinite) {
+    if constexpr (!HELD)
+      if (infinite) {
 #pragma unroll
-      for (int i = 0; i < VE; ++i) x[i] = x[i] == INFINITY ? 0.f : -INFINITY;
-    }
+        for (int i = 0; i < VE; ++i) x[i] = x[i] == INFINITY ? 0.f : -INFINITY;
+      }
+  }
+  // rewrites this thread's chunks for a row whose maximum is +inf
+  __device__ __forceinline__ void to_infinite() {
+    infinite = true;
+    if constexpr (HELD)
+      for (int j = threadIdx.x; j < chunks; j += kThreads) {
+        float x[VE];
+        get(j, x);
+        uint32_t u[4];
+#pragma unroll
+        for (int i = 0; i < VE; ++i) x[i] = x[i] == INFINITY ? 0.f : -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (DT == DT_F32)
+            u[i] = __float_as_uint(x[i]);
+          else
+            u[i] = pack2<DT>(x[2 * i], x[2 * i + 1]);
+        }
+        held[j] = make_uint4(u[0], u[1], u[2], u[3]);
+      }
   }
   // the largest logit of a chunk (NaN and a row with infinities aside: it may be too large)
   __device__ __forceinline__ float highest(int j) const {
-    const uint4 u = held != nullptr ? held[j] : load(j);
+    const uint4 u = at(j);
     if constexpr (DT == DT_F32) {
       return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)),
                    fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
@@ -136,7 +162,7 @@ template <int DT> struct Slice {
     } else {
       uint32_t best = kMinusInfPair<DT>;
       for (int j = threadIdx.x; j < chunks; j += kThreads) {
-        const uint4 u = held != nullptr ? held[j] : load(j);
+        const uint4 u = at(j);
         best = max_pair<DT>(max_pair<DT>(max_pair<DT>(u.x, u.y), max_pair<DT>(u.z, u.w)), best);
       }
       const float2 f = unpack2<DT>(best);
@@ -492,10 +518,10 @@ struct Found {
   bool single;
 };
 
-template <int DT, bool WEIGHT>
-__device__ Found search(cg::cluster_group& cl, Shared& sh, const Slice<DT>& sl, const RowState& row,
+template <int DT, bool HELD, bool WEIGHT>
+__device__ Found search(cg::cluster_group& cl, Shared& sh, const Slice<DT, HELD>& sl, const RowState& row,
                         double target, const Cut& within) {
-  constexpr int VE = Slice<DT>::VE;
+  constexpr int VE = Slice<DT, HELD>::VE;
   const int tid = threadIdx.x;
   // linear bins
   for (int j = tid; j < sl.chunks; j += kThreads) {
@@ -649,9 +675,9 @@ __device__ Found search(cg::cluster_group& cl, Shared& sh, const Slice<DT>& sl, 
 }
 
 // Index of the `need`-th logit (from 1) equal to `value`, in index order.
-template <int DT>
-__device__ int tie_index(cg::cluster_group& cl, Shared& sh, const Slice<DT>& sl, float value, unsigned need) {
-  constexpr int VE = Slice<DT>::VE;
+template <int DT, bool HELD>
+__device__ int tie_index(cg::cluster_group& cl, Shared& sh, const Slice<DT, HELD>& sl, float value, unsigned need) {
+  constexpr int VE = Slice<DT, HELD>::VE;
   const int share = (sl.chunks + kThreads - 1) / kThreads;   // chunks a thread, consecutive
   const int j0 = min(sl.chunks, (int)threadIdx.x * share), j1 = min(sl.chunks, j0 + share);
   unsigned mine = 0;
@@ -708,10 +734,10 @@ __device__ float min_p_logit(const RowState& row) {
 
 // Top-p over the whole row: cut after the shortest prefix with p of the weight.
 // Returns false (everywhere) when the crossing bin does not fit the list.
-template <int DT>
-__device__ bool nucleus(cg::cluster_group& cl, Shared& sh, const Slice<DT>& sl, RowState row,
+template <int DT, bool HELD>
+__device__ bool nucleus(cg::cluster_group& cl, Shared& sh, const Slice<DT, HELD>& sl, RowState row,
                         unsigned long long* list, float* ahead, double& whole, Cut& cut) {
-  constexpr int VE = Slice<DT>::VE;
+  constexpr int VE = Slice<DT, HELD>::VE;
   const int tid = threadIdx.x;
   // Tokens with less than (1 - p) / vocab of the largest one's weight do not reach 1 - p of
   // all weight together, so the prefix ends above them: the bins span the rest.
@@ -828,10 +854,10 @@ __device__ bool nucleus(cg::cluster_group& cl, Shared& sh, const Slice<DT>& sl, 
 // the special-function unit's, which the weights' exponentials keep busy. A thread keeps
 // its best chunk of them; then only the chunks within reach of the CTA's best are scored
 // exactly.
-template <int DT, bool ALL>
-__device__ __forceinline__ unsigned long long race(Shared& sh, const Slice<DT>& sl, const RowState& row,
+template <int DT, bool HELD, bool ALL>
+__device__ __forceinline__ unsigned long long race(Shared& sh, const Slice<DT, HELD>& sl, const RowState& row,
                                                    const Cut cut, const float* noise, bool sum_here, float& sum) {
-  constexpr int VE = Slice<DT>::VE, DEPTH = 16 / VE;
+  constexpr int VE = Slice<DT, HELD>::VE, DEPTH = 16 / VE;
   constexpr float kReach = 0.0861f + 1e-3f;   // the log's error, and the rounding of scores to about 500
   const int tid = threadIdx.x;
   // chunks whose noise is whole 16-byte words: all but a row's first and last, or none
@@ -949,10 +975,10 @@ __device__ __forceinline__ bool leave(cg::cluster_group& cl, Shared& sh, unsigne
   return false;
 }
 
-template <int DT>
-__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a, int per) {
+template <int DT, bool HELD>
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a) {
   using T = typename Elem<DT>::T;
-  constexpr int VE = Slice<DT>::VE;
+  constexpr int VE = Slice<DT, HELD>::VE;
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ Shared sh;
   cg::cluster_group cl = cg::this_cluster();
@@ -965,18 +991,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a,
   // (with the wait below: every CTA of the cluster runs before its shared memory is written)
   asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
 
-  Slice<DT> sl;
+  Slice<DT, HELD> sl;
   sl.row = reinterpret_cast<const T*>(a.logits) + r * a.logits_stride;
   sl.vocab = a.vocab;
   sl.infinite = false;
   const int mis = (int)(reinterpret_cast<uintptr_t>(sl.row) % 16 / sizeof(T));
   const int all = (int)(((int64_t)mis + a.vocab + VE - 1) / VE);
-  const int share = (all + nblocks - 1) / nblocks;   // <= per when slices are held
+  const int share = (all + nblocks - 1) / nblocks;
   const int c0 = min(all, rank * share);
   sl.chunks = min(share, all - c0);
   sl.first = (int64_t)c0 * VE - mis;
-  sl.held = nullptr;
-  if (per > 0) {
+  sl.held = held;
+  if constexpr (HELD) {
     for (int j = tid; j < sl.chunks; j += kThreads) {
       if (sl.inside(j))
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(held + j)),
@@ -986,7 +1012,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a,
         held[j] = sl.load(j);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
-    sl.held = held;
   }
   // settings
   RowState row;
@@ -1065,7 +1090,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a,
     return;
   }
   if (row.top == INFINITY) {
-    sl.infinite = true;
+    sl.to_infinite();
     row.top = bound = 0.f;
   }
 
@@ -1198,7 +1223,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a,
     bool have_sum = false;
     double whole = 0;
     if (use_k) {
-      const Found f = search<DT, false>(cl, sh, sl, row, (double)k_set, cut);
+      const Found f = search<DT, HELD, false>(cl, sh, sl, row, (double)k_set, cut);
       cut.x = unorder(f.key);
       if (f.single && f.above + (double)f.count > (double)k_set)
         cut.last = tie_index(cl, sh, sl, cut.x, (unsigned)((double)k_set - f.above));
@@ -1220,7 +1245,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a,
         double left[1];
         cluster_sum(cl, sh, s, left);
         const double target = (double)row.top_p * left[0];
-        const Found f = search<DT, true>(cl, sh, sl, row, target, cut);
+        const Found f = search<DT, HELD, true>(cl, sh, sl, row, target, cut);
         const float x = fmaxf(unorder(f.key), cut.x);
         int last = x > cut.x ? kAnyIndex : cut.last;
         if (f.single && f.count > 0) {
@@ -1241,8 +1266,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a,
     const bool sum_here = want_sum && !have_sum;
     float s[1] = {0.f};
     best = block_best(sh, cut.x == -kFloatMax && cut.last == kAnyIndex
-                              ? race<DT, true>(sh, sl, row, cut, noise, sum_here, s[0])
-                              : race<DT, false>(sh, sl, row, cut, noise, sum_here, s[0]));
+                              ? race<DT, HELD, true>(sh, sl, row, cut, noise, sum_here, s[0])
+                              : race<DT, HELD, false>(sh, sl, row, cut, noise, sum_here, s[0]));
     if (sum_here) block_sum(sh, s, 3);
     part = sum_here ? sh.row_sums[3] : rank == 0 ? whole : 0.0;
     if (leave(cl, sh, best, part)) return;
@@ -1267,7 +1292,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a,
 }
 
 template <int DT> cudaError_t launch_dt(const SampleArgs& a, int num_sms, cudaStream_t stream) {
-  constexpr int VE = Slice<DT>::VE;
+  constexpr int VE = Slice<DT, true>::VE;
   const int64_t chunks = ((int64_t)a.vocab + 2 * VE - 2) / VE;   // of a row at any alignment
   // The smallest cluster that holds a row with two CTAs an SM (one computes while the
   // other loads), larger while the GPU has room for more CTAs; a row past that is held
@@ -1278,8 +1303,10 @@ template <int DT> cudaError_t launch_dt(const SampleArgs& a, int num_sms, cudaSt
   const int64_t per = (chunks + n - 1) / n;
   const bool held = per * 16 <= kSliceOne;
   const int smem = kListBytes + (held ? (int)per * 16 : 0);
-  static std::atomic<uint64_t> allowed{0};
-  cudaError_t e = allow_shared(reinterpret_cast<const void*>(sample_kernel<DT>), kListBytes + kSliceOne, allowed);
+  auto kernel = held ? sample_kernel<DT, true> : sample_kernel<DT, false>;
+  static std::atomic<uint64_t> allowed[2];
+  cudaError_t e = allow_shared(reinterpret_cast<const void*>(kernel), kListBytes + (held ? kSliceOne : 0),
+                               allowed[held]);
   if (e != cudaSuccess) return e;
   if ((int64_t)a.rows * n > 0x7fffffff) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg = {};
@@ -1293,7 +1320,7 @@ template <int DT> cudaError_t launch_dt(const SampleArgs& a, int num_sms, cudaSt
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, sample_kernel<DT>, a, held ? (int)per : 0);
+  e = cudaLaunchKernelEx(&cfg, kernel, a);
   if (e == cudaSuccess) count_launch();
   return e;
 }
