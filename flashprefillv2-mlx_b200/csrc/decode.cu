@@ -82,7 +82,7 @@ template <int TK> __device__ __forceinline__ Seq seq_of(const DecodeArgs& a, int
   return s;
 }
 
-__device__ __forceinline__ int warp_sum(int v) {
+__device__ __forceinline__ int64_t warp_sum(int64_t v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
@@ -90,8 +90,8 @@ __device__ __forceinline__ int warp_sum(int v) {
 
 // A sequence costs its tiles and about two more, for its queries' way in and its
 // results' way out; the stream that is cut into parts counts those first, ahead of the
-// tiles. (Without them a part of many short sequences took three times the average part's
-// time: 24 sequences of 3 to 20011 keys, 55 us against @@ us.)
+// tiles. (Without them a part of many short sequences takes three times the average part's
+// time: for 24 sequences of 3 to 20011 keys the slowest warp 83k cycles instead of 44k.)
 constexpr int kSeqCost = 2;
 __device__ __forceinline__ int cost_of(const Seq& s) { return s.tiles > 0 ? s.tiles + kSeqCost : 0; }
 
@@ -112,8 +112,13 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
   return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
 }
 
+// Stream units a part. Not fewer than balances what a tile adds to the first kernel (about
+// 1000 cycles) with what a piece adds to the second (about 11: eight warps, ten in flight
+// each): the square root of total / 90. It matters with few KV heads, where one wave of
+// warps is many parts (1 x 20000 keys of one KV head of 64: 17.9 us in 1184 parts, 14.1 us in
+// 209).
 __device__ __forceinline__ int64_t part_tiles(int64_t total, int parts) {
-  return quotient(total + parts - 1, parts);
+  return max(quotient(total + parts - 1, parts), (int64_t)sqrtf((float)total * (1.f / 90.f)));
 }
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
@@ -241,11 +246,11 @@ __global__ void __launch_bounds__(Shape<D>::NW * 32, 1) decode_kernel(const Deco
     int64_t run = 0;
     int b0 = 0;
     while (true) {
-      const int n = cost_of(seq_of<TK>(a, b0 + lane));
-      int incl = n;
+      const int64_t n = cost_of(seq_of<TK>(a, b0 + lane));
+      int64_t incl = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, incl, o);
+        const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += v;
       }
       const unsigned past = __ballot_sync(0xffffffffu, run + incl > begin);

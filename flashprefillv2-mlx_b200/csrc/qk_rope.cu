@@ -11,6 +11,7 @@
 // Every element is read once and written once with a handful of operations, so
 // DRAM bandwidth bounds the long calls and launch latency the short ones.
 #include <algorithm>
+#include <cstdint>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -68,7 +69,6 @@ __device__ __forceinline__ float2 mul_f32x2(float2 a, float2 b) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
-__device__ __forceinline__ float2 neg(float2 a) { return make_float2(-a.x, -a.y); }
 
 // BYTES (8 or 16) of values as they are in memory, and as pairs of floats.
 template <int DT, int BYTES> struct Pack {
@@ -143,18 +143,18 @@ template <int N> __device__ __forceinline__ void load_weights(const void* w, int
 // token, `apart` heads from one to the next, so neighbouring groups read neighbouring
 // heads, the token's table row and cache slot are looked up once and the norm weights
 // stay in registers from head to head; the next AHEAD heads are being loaded meanwhile.
+// With AHEAD 0 a group takes one head (few tokens), in fewer registers.
 //
-// Bytes in flight against registers: a 16-bit type has 16 values of 8 bytes each in the
-// works a lane, and does best with two heads ahead and two CTAs an SM (2048 tokens of
-// 32 + 8 + 8 heads of 128: 16.7 us; one ahead and four CTAs 24.7 us, with spills), float32
-// has half the values and wants the CTAs (16384 tokens: 121 us; two ahead and two 151 us).
-template <int DT> constexpr int kAhead = DT == DT_F32 ? 1 : 2;
-template <int DT> constexpr int kCtas = DT == DT_F32 ? 4 : 2;
+// A step is about 200 instructions a warp, mostly on latencies: a 16-bit type does best
+// with two heads ahead and two CTAs an SM, float32, whose lanes hold half the values, with
+// one ahead and four (12000 tokens of 32 + 8 heads of 128, float32: 91 us, 5.5 TB/s; two
+// ahead and three CTAs 94 us).
+template <int DT, int AHEAD> constexpr int kCtas = AHEAD == 0 ? 3 : DT == DT_F32 ? 4 : 2;
 
-template <int DT, int BYTES, int LANES, bool INTER>
-__global__ void __launch_bounds__(256, kCtas<DT>) qk_rope_vec_kernel(const RopeArgs a, int apart) {
+template <int DT, int BYTES, int LANES, bool INTER, int AHEAD>
+__global__ void __launch_bounds__(256, (kCtas<DT, AHEAD>)) qk_rope_vec_kernel(const RopeArgs a, int apart) {
   using P = Pack<DT, BYTES>;
-  constexpr int ES = DT == DT_F32 ? 4 : 2, N = P::N, H = N / 2, AHEAD = kAhead<DT>;
+  constexpr int ES = DT == DT_F32 ? 4 : 2, N = P::N, H = N / 2;
   const int heads = a.Hq + (a.k_cache != nullptr ? 2 : 1) * a.Hkv;
   const int c = threadIdx.x % LANES;
   const unsigned group = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(256, kCtas<DT>) qk_rope_vec_kernel(const RopeA
   };
   P x[AHEAD + 1][2] = {};
 #pragma unroll
-  for (int i = 0; i < AHEAD; ++i) load(h0 + i * apart, x[i]);
+  for (int i = 0; i < (AHEAD > 0 ? AHEAD : 1); ++i) load(h0 + i * apart, x[i]);
   float2 co[H], si[H];   // interleaved: of the first pack's pairs, then of the second's
 #pragma unroll
   for (int j = 0; j < H; ++j) {   // no rotation: by nothing
@@ -235,22 +235,29 @@ __global__ void __launch_bounds__(256, kCtas<DT>) qk_rope_vec_kernel(const RopeA
   float2 w[2 * H];
 #pragma unroll
   for (int j = 0; j < 2 * H; ++j) w[j] = make_float2(1.f, 1.f);
+  float2 ns[H];   // the sines, negated
+#pragma unroll
+  for (int j = 0; j < H; ++j) ns[j] = make_float2(-si[j].x, -si[j].y);
   // every lane of a warp takes the same number of steps
   const int steps = (heads + apart - 1) / apart;
-  for (int step = 0; step < steps; ++step) {
-    const int h = h0 + step * apart;
-    load(h + AHEAD * apart, x[AHEAD]);
-    float2 y[2 * H];
-    x[0][0].to(y);
-    x[0][1].to(y + H);
-    float2 s2 = mul_f32x2(y[0], y[0]);
+  for (int step0 = 0; step0 < steps; step0 += AHEAD + 1) {
 #pragma unroll
-    for (int j = 1; j < 2 * H; ++j) s2 = fma_f32x2(y[j], y[j], s2);
-    float ss = s2.x + s2.y;
+    for (int u = 0; u <= AHEAD; ++u) {
+      if (step0 + u >= steps) break;
+      const int h = h0 + (step0 + u) * apart;
+      if constexpr (AHEAD > 0) load(h + AHEAD * apart, x[(u + AHEAD) % (AHEAD + 1)]);
+      P (&mine)[2] = x[u];
+      float2 y[2 * H];
+      mine[0].to(y);
+      mine[1].to(y + H);
+      float2 s2 = mul_f32x2(y[0], y[0]);
 #pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    char* const to = h < kv0 ? qd : h < v0 ? kd : vd;
-    if (live && h < heads && to != nullptr) {
+      for (int j = 1; j < 2 * H; ++j) s2 = fma_f32x2(y[j], y[j], s2);
+      float ss = s2.x + s2.y;
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      char* const to = h < kv0 ? qd : h < v0 ? kd : vd;
+      if (!live || h >= heads || to == nullptr) continue;
       char* const dst = to + (h < kv0 ? (int64_t)h * qsd
                               : h < v0 ? (int64_t)(h - kv0) * ksd : (int64_t)(h - v0) * vsd);
       if (h < v0) {
@@ -271,27 +278,23 @@ __global__ void __launch_bounds__(256, kCtas<DT>) qk_rope_vec_kernel(const RopeA
         if constexpr (INTER) {
 #pragma unroll
           for (int j = 0; j < 2 * H; ++j) {
-            const float cj = j & 1 ? co[j / 2].y : co[j / 2].x, sj = j & 1 ? si[j / 2].y : si[j / 2].x;
-            y[j] = fma_f32x2(y[j], make_float2(cj, cj), mul_f32x2(make_float2(-y[j].y, y[j].x), make_float2(sj, sj)));
+            const float cj = j & 1 ? co[j / 2].y : co[j / 2].x;
+            const float sj = j & 1 ? si[j / 2].y : si[j / 2].x, nj = j & 1 ? ns[j / 2].y : ns[j / 2].x;
+            y[j] = fma_f32x2(y[j], make_float2(cj, cj), mul_f32x2(make_float2(y[j].y, y[j].x), make_float2(nj, sj)));
           }
         } else {
 #pragma unroll
           for (int j = 0; j < H; ++j) {
-            const float2 u = y[j], v = y[j + H];
-            y[j] = fma_f32x2(u, co[j], neg(mul_f32x2(v, si[j])));
-            y[j + H] = fma_f32x2(v, co[j], mul_f32x2(u, si[j]));
+            const float2 p = y[j], v = y[j + H];
+            y[j] = fma_f32x2(p, co[j], mul_f32x2(v, ns[j]));
+            y[j + H] = fma_f32x2(v, co[j], mul_f32x2(p, si[j]));
           }
         }
-        x[0][0].from(y);
-        x[0][1].from(y + H);
+        mine[0].from(y);
+        mine[1].from(y + H);
       }
-      x[0][0].store(dst + d0 * ES);
-      x[0][1].store(dst + d1 * ES);
-    }
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {
-      x[i][0] = x[i + 1][0];
-      x[i][1] = x[i + 1][1];
+      mine[0].store(dst + d0 * ES);
+      mine[1].store(dst + d1 * ES);
     }
   }
 }
@@ -344,21 +347,40 @@ __global__ void __launch_bounds__(256) qk_rope_any_kernel(const RopeArgs a) {
   }
 }
 
-template <int DT, int BYTES, int LANES>
-cudaError_t launch_lanes(const RopeArgs& a, int num_sms, cudaStream_t stream) {
-  const int heads = a.Hq + (a.k_cache != nullptr ? 2 : 1) * a.Hkv;
-  // as many heads a lane group, up to eight, as leave every SM its CTAs
-  const int64_t groups = (int64_t)kCtas<DT> * num_sms * (256 / LANES);
-  const int64_t most = std::min<int64_t>(8, std::max<int64_t>(1, a.tokens * heads / groups));
-  const int apart = (heads + (int)most - 1) / (int)most;
+template <int DT, int BYTES, int LANES, int AHEAD>
+cudaError_t launch_apart(const RopeArgs& a, int apart, cudaStream_t stream) {
   const int64_t blocks = (a.tokens * apart * LANES + 255) / 256;
   if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
   if (a.interleaved)
-    qk_rope_vec_kernel<DT, BYTES, LANES, true><<<(unsigned)blocks, 256, 0, stream>>>(a, apart);
+    qk_rope_vec_kernel<DT, BYTES, LANES, true, AHEAD><<<(unsigned)blocks, 256, 0, stream>>>(a, apart);
   else
-    qk_rope_vec_kernel<DT, BYTES, LANES, false><<<(unsigned)blocks, 256, 0, stream>>>(a, apart);
+    qk_rope_vec_kernel<DT, BYTES, LANES, false, AHEAD><<<(unsigned)blocks, 256, 0, stream>>>(a, apart);
   count_launch();
   return cudaGetLastError();
+}
+
+template <int DT, int BYTES, int LANES>
+cudaError_t launch_lanes(const RopeArgs& a, int num_sms, cudaStream_t stream) {
+  constexpr int AHEAD = DT == DT_F32 ? 1 : 2;
+  const int heads = a.Hq + (a.k_cache != nullptr ? 2 : 1) * a.Hkv;
+  constexpr int GROUPS = 256 / LANES;   // of a CTA
+  // one head a lane group while the CTAs about fit on the GPU at once
+  if (a.tokens * heads <= 4ll * num_sms * GROUPS)
+    return launch_apart<DT, BYTES, LANES, 0>(a, heads, stream);
+  // else as many as make the shortest sum of waves of CTAs, a group's start (its token's
+  // table row, the weights) counting as three heads
+  const int64_t slots = (int64_t)kCtas<DT, AHEAD> * num_sms * GROUPS;
+  int best = heads;
+  int64_t least = INT64_MAX;
+  for (int steps = 1; steps <= std::min(heads, 24); ++steps) {
+    const int apart = (heads + steps - 1) / steps;
+    const int64_t cost = (a.tokens * apart + slots - 1) / slots * (steps + 3);
+    if (cost < least) {
+      least = cost;
+      best = apart;
+    }
+  }
+  return launch_apart<DT, BYTES, LANES, AHEAD>(a, best, stream);
 }
 
 template <int DT, int BYTES> cudaError_t launch_vec(const RopeArgs& a, int num_sms, cudaStream_t stream) {
