@@ -82,17 +82,17 @@ template <int TK> __device__ __forceinline__ Seq seq_of(const DecodeArgs& a, int
   return s;
 }
 
-__device__ __forceinline__ int64_t warp_sum(int64_t v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+__device__ __forceinline__ int64_t warp_sum(uint32_t v) {
+  const uint32_t low = __reduce_add_sync(0xffffffffu, v & 0xffffu), high = __reduce_add_sync(0xffffffffu, v >> 16);
+  return ((int64_t)high << 16) + low;
 }
 
-// A sequence costs its tiles and about two more, for its queries' way in and its
-// results' way out; the stream that is cut into parts counts those first, ahead of the
-// tiles. (Without them a part of many short sequences takes three times the average part's
-// time: for 24 sequences of 3 to 20011 keys the slowest warp 83k cycles instead of 44k.)
-constexpr int kSeqCost = 2;
+// A sequence costs its tiles and some more, for its queries' way in and its results' way
+// out; the stream that is cut into parts counts that first, ahead of the tiles. (24
+// sequences of 3 to 20011 keys, 32 rows a head: the slowest warp takes 83k cycles without it,
+// 44k with two tiles' worth; in all 38.0 us with two, 34.6 with four, 33.6 with six. 40
+// sequences of 9 to 900 keys, 4 rows: 17.0, 17.1 and 17.6 us.)
+constexpr int kSeqCost = 4;
 __device__ __forceinline__ int cost_of(const Seq& s) { return s.tiles > 0 ? s.tiles + kSeqCost : 0; }
 
 // Stream units before sequence `want` and in total (warp-wide).
@@ -101,8 +101,8 @@ __device__ __forceinline__ void scan_to(const DecodeArgs& a, int lane, int want,
                                         int64_t& total) {
   before = total = 0;
   for (int b0 = 0; b0 < a.B; b0 += 32) {
-    const int n = cost_of(seq_of<TK>(a, b0 + lane));
-    before += warp_sum(b0 + lane < want ? n : 0);
+    const uint32_t n = cost_of(seq_of<TK>(a, b0 + lane));
+    if (want > b0) before += warp_sum(b0 + lane < want ? n : 0u);
     total += warp_sum(n);
   }
 }
@@ -246,25 +246,29 @@ __global__ void __launch_bounds__(Shape<D>::NW * 32, 1) decode_kernel(const Deco
     int64_t run = 0;
     int b0 = 0;
     while (true) {
-      const int64_t n = cost_of(seq_of<TK>(a, b0 + lane));
-      int64_t incl = n;
+      const uint32_t n = cost_of(seq_of<TK>(a, b0 + lane));
+      if (b0 + 32 < a.B) {   // (the last 32 hold it if those before do not)
+        const int64_t sum = warp_sum(n);
+        if (run + sum <= begin) {
+          run += sum;
+          b0 += 32;
+          continue;
+        }
+      }
+      uint32_t ahead = n;   // units of the lanes before this one; less than 32 (2^27 + 2)
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += v;
+        const uint32_t v = __shfl_up_sync(0xffffffffu, ahead, o);
+        if (lane >= o) ahead += v;
       }
-      const unsigned past = __ballot_sync(0xffffffffu, run + incl > begin);
-      if (past) {
-        const int at = __ffs(past) - 1;
-        f.b = b0 + at;
-        run += __shfl_sync(0xffffffffu, incl - n, at);   // where the sequence starts
-        f.t = max((int)(begin - run) - kSeqCost, 0);
-        f.at = run + kSeqCost + f.t;
-        started = run < begin;
-        break;
-      }
-      run += __shfl_sync(0xffffffffu, incl, 31);
-      b0 += 32;
+      ahead -= n;
+      const int at = 31 - __clz(__ballot_sync(0xffffffffu, n > 0 && (int64_t)ahead <= begin - run));
+      f.b = b0 + at;
+      run += __shfl_sync(0xffffffffu, ahead, at);   // where the sequence starts
+      f.t = max((int)(begin - run) - kSeqCost, 0);
+      f.at = run + kSeqCost + f.t;
+      started = run < begin;
+      break;
     }
     f.s = seq_of<TK>(a, f.b);
   }
