@@ -110,6 +110,13 @@ template <int DT, int BYTES> struct Pack {
     }
   }
 };
+template <int BYTES> __device__ __forceinline__ void cp_async(uint32_t dst, const void* src) {
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+
 // N floats as pairs
 template <int N> __device__ __forceinline__ void load_floats(const float* p, float2* x) {
   if constexpr (N == 2) {
@@ -142,13 +149,16 @@ template <int N> __device__ __forceinline__ void load_weights(const void* w, int
 // pairs), so the rotation needs no other lane. A group of LANES lanes takes heads of one
 // token, `apart` heads from one to the next, so neighbouring groups read neighbouring
 // heads, the token's table row and cache slot are looked up once and the norm weights
-// stay in registers from head to head; the next AHEAD heads are being loaded meanwhile.
-// With AHEAD 0 a group takes one head (few tokens), in fewer registers.
+// stay in registers from head to head.
 //
-// A step is about 200 instructions a warp, mostly on latencies: a 16-bit type does best
-// with two heads ahead and two CTAs an SM, float32, whose lanes hold half the values, with
-// one ahead and four (12000 tokens of 32 + 8 heads of 128, float32: 91 us, 5.5 TB/s; two
-// ahead and three CTAs 94 us).
+// DRAM bounds it once enough is on its way: the next AHEAD heads are copied to shared
+// memory meanwhile, where they cost no registers (held in registers, two ahead, 16384
+// bf16 tokens of 32 + 8 + 8 heads of 128 took 97 us, half of a warp's time waiting for
+// loads; so 72 us, 5.7 TB/s; float32, 32 + 8 heads: 115 and 105 us, 6.5 TB/s, a copy's
+// rate). 5 ahead measure the same as 3. Two CTAs of 256 threads an SM hold a 16-bit type's
+// values without spills (4096 tokens 19.6 us; three CTAs 23.5 us), four a float32 type's,
+// which are half as many a lane. With AHEAD 0 a group takes one head (few tokens),
+// loaded to registers.
 template <int DT, int AHEAD> constexpr int kCtas = AHEAD == 0 ? 3 : DT == DT_F32 ? 4 : 2;
 
 template <int DT, int BYTES, int LANES, bool INTER, int AHEAD>
@@ -184,16 +194,31 @@ __global__ void __launch_bounds__(256, (kCtas<DT, AHEAD>)) qk_rope_vec_kernel(co
   const char* ks = reinterpret_cast<const char*>(a.k) + t * (int)a.k_st * ES;
   const char* vs = reinterpret_cast<const char*>(a.v) + t * (int)a.v_st * ES;
   const int qsh = (int)a.q_sh * ES, ksh = (int)a.k_sh * ES, vsh = (int)a.v_sh * ES;
-  auto load = [&](int h, P (&x)[2]) {
-    if (!live || h >= heads) return;
-    const char* src = h < kv0 ? qs + (int64_t)h * qsh
-                    : h < v0 ? ks + (int64_t)(h - kv0) * ksh : vs + (int64_t)(h - v0) * vsh;
-    x[0].load(src + d0 * ES);
-    x[1].load(src + d1 * ES);
+  auto source = [&](int h) {
+    return h < kv0 ? qs + (int64_t)h * qsh
+         : h < v0 ? ks + (int64_t)(h - kv0) * ksh : vs + (int64_t)(h - v0) * vsh;
   };
-  P x[AHEAD + 1][2] = {};
+  // the heads on their way, each lane's own two packs: no lane reads another's, so a wait
+  // for the lane's copies is all the order they need
+  __shared__ __align__(16) unsigned char ring[AHEAD > 0 ? (AHEAD + 1) * 2 * 256 * BYTES : 16];
+  const uint32_t mine_at = smem_u32(ring) + threadIdx.x * BYTES;
+  P mine[2] = {};
+  auto issue = [&](int h, int slot) {
+    if (live && h < heads) {
+      const char* src = source(h);
+      cp_async<BYTES>(mine_at + slot * 2 * 256 * BYTES, src + d0 * ES);
+      cp_async<BYTES>(mine_at + (slot * 2 + 1) * 256 * BYTES, src + d1 * ES);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if constexpr (AHEAD > 0) {
 #pragma unroll
-  for (int i = 0; i < (AHEAD > 0 ? AHEAD : 1); ++i) load(h0 + i * apart, x[i]);
+    for (int i = 0; i < AHEAD; ++i) issue(h0 + i * apart, i);
+  } else if (live && h0 < heads) {
+    const char* src = source(h0);
+    mine[0].load(src + d0 * ES);
+    mine[1].load(src + d1 * ES);
+  }
   float2 co[H], si[H];   // interleaved: of the first pack's pairs, then of the second's
 #pragma unroll
   for (int j = 0; j < H; ++j) {   // no rotation: by nothing
@@ -240,62 +265,64 @@ __global__ void __launch_bounds__(256, (kCtas<DT, AHEAD>)) qk_rope_vec_kernel(co
   for (int j = 0; j < H; ++j) ns[j] = make_float2(-si[j].x, -si[j].y);
   // every lane of a warp takes the same number of steps
   const int steps = (heads + apart - 1) / apart;
-  for (int step0 = 0; step0 < steps; step0 += AHEAD + 1) {
+  int slot = 0, fill = AHEAD;
+  for (int step = 0, h = h0; step < steps; ++step, h += apart) {
+    if constexpr (AHEAD > 0) {
+      issue(h + AHEAD * apart, fill);
+      fill = slot;
+      asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD) : "memory");
+      mine[0].load(ring + slot * 2 * 256 * BYTES + threadIdx.x * BYTES);
+      mine[1].load(ring + (slot * 2 + 1) * 256 * BYTES + threadIdx.x * BYTES);
+      slot = slot == AHEAD ? 0 : slot + 1;
+    }
+    float2 y[2 * H];
+    mine[0].to(y);
+    mine[1].to(y + H);
+    float2 s2 = mul_f32x2(y[0], y[0]);
 #pragma unroll
-    for (int u = 0; u <= AHEAD; ++u) {
-      if (step0 + u >= steps) break;
-      const int h = h0 + (step0 + u) * apart;
-      if constexpr (AHEAD > 0) load(h + AHEAD * apart, x[(u + AHEAD) % (AHEAD + 1)]);
-      P (&mine)[2] = x[u];
-      float2 y[2 * H];
-      mine[0].to(y);
-      mine[1].to(y + H);
-      float2 s2 = mul_f32x2(y[0], y[0]);
+    for (int j = 1; j < 2 * H; ++j) s2 = fma_f32x2(y[j], y[j], s2);
+    float ss = s2.x + s2.y;
 #pragma unroll
-      for (int j = 1; j < 2 * H; ++j) s2 = fma_f32x2(y[j], y[j], s2);
-      float ss = s2.x + s2.y;
-#pragma unroll
-      for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      char* const to = h < kv0 ? qd : h < v0 ? kd : vd;
-      if (!live || h >= heads || to == nullptr) continue;
-      char* const dst = to + (h < kv0 ? (int64_t)h * qsd
-                              : h < v0 ? (int64_t)(h - kv0) * ksd : (int64_t)(h - v0) * vsd);
-      if (h < v0) {
-        const float r = rsqrtf(fmaf(ss, inv_d, a.eps));
-        const void* weight = h < kv0 ? a.q_weight : a.k_weight;
-        if (weight != have) {
-          have = weight;
-          if (weight != nullptr) {
-            load_weights<N>(weight, a.weight_dt, d0, w);
-            load_weights<N>(weight, a.weight_dt, d1, w + H);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 2 * H; ++j) w[j] = make_float2(1.f, 1.f);
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < 2 * H; ++j) y[j] = mul_f32x2(mul_f32x2(y[j], make_float2(r, r)), w[j]);
-        if constexpr (INTER) {
-#pragma unroll
-          for (int j = 0; j < 2 * H; ++j) {
-            const float cj = j & 1 ? co[j / 2].y : co[j / 2].x;
-            const float sj = j & 1 ? si[j / 2].y : si[j / 2].x, nj = j & 1 ? ns[j / 2].y : ns[j / 2].x;
-            y[j] = fma_f32x2(y[j], make_float2(cj, cj), mul_f32x2(make_float2(y[j].y, y[j].x), make_float2(nj, sj)));
-          }
+    for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    char* const to = h < kv0 ? qd : h < v0 ? kd : vd;
+    if (!live || h >= heads || to == nullptr) continue;
+    char* const dst = to + (h < kv0 ? (int64_t)h * qsd
+                            : h < v0 ? (int64_t)(h - kv0) * ksd : (int64_t)(h - v0) * vsd);
+    if (h < v0) {
+      const float r = rsqrtf(fmaf(ss, inv_d, a.eps));
+      const void* weight = h < kv0 ? a.q_weight : a.k_weight;
+      if (weight != have) {
+        have = weight;
+        if (weight != nullptr) {
+          load_weights<N>(weight, a.weight_dt, d0, w);
+          load_weights<N>(weight, a.weight_dt, d1, w + H);
         } else {
 #pragma unroll
-          for (int j = 0; j < H; ++j) {
-            const float2 p = y[j], v = y[j + H];
-            y[j] = fma_f32x2(p, co[j], mul_f32x2(v, ns[j]));
-            y[j + H] = fma_f32x2(v, co[j], mul_f32x2(p, si[j]));
-          }
+          for (int j = 0; j < 2 * H; ++j) w[j] = make_float2(1.f, 1.f);
         }
-        mine[0].from(y);
-        mine[1].from(y + H);
       }
-      mine[0].store(dst + d0 * ES);
-      mine[1].store(dst + d1 * ES);
+#pragma unroll
+      for (int j = 0; j < 2 * H; ++j) y[j] = mul_f32x2(mul_f32x2(y[j], make_float2(r, r)), w[j]);
+      if constexpr (INTER) {
+#pragma unroll
+        for (int j = 0; j < 2 * H; ++j) {
+          const float cj = j & 1 ? co[j / 2].y : co[j / 2].x;
+          const float sj = j & 1 ? si[j / 2].y : si[j / 2].x, nj = j & 1 ? ns[j / 2].y : ns[j / 2].x;
+          y[j] = fma_f32x2(y[j], make_float2(cj, cj), mul_f32x2(make_float2(y[j].y, y[j].x), make_float2(nj, sj)));
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < H; ++j) {
+          const float2 p = y[j], v = y[j + H];
+          y[j] = fma_f32x2(p, co[j], mul_f32x2(v, ns[j]));
+          y[j + H] = fma_f32x2(v, co[j], mul_f32x2(p, si[j]));
+        }
+      }
+      mine[0].from(y);
+      mine[1].from(y + H);
     }
+    mine[0].store(dst + d0 * ES);
+    mine[1].store(dst + d1 * ES);
   }
 }
 
@@ -361,14 +388,15 @@ cudaError_t launch_apart(const RopeArgs& a, int apart, cudaStream_t stream) {
 
 template <int DT, int BYTES, int LANES>
 cudaError_t launch_lanes(const RopeArgs& a, int num_sms, cudaStream_t stream) {
-  constexpr int AHEAD = DT == DT_F32 ? 1 : 2;
+  constexpr int AHEAD = 3;
   const int heads = a.Hq + (a.k_cache != nullptr ? 2 : 1) * a.Hkv;
   constexpr int GROUPS = 256 / LANES;   // of a CTA
   // one head a lane group while the CTAs about fit on the GPU at once
   if (a.tokens * heads <= 4ll * num_sms * GROUPS)
     return launch_apart<DT, BYTES, LANES, 0>(a, heads, stream);
   // else as many as make the shortest sum of waves of CTAs, a group's start (its token's
-  // table row, the weights) counting as three heads
+  // table row, the weights) counting as three heads (31007 tokens of 16 + 4
+  // float32 heads of 96: 76 us; by the CTAs an SM gets, which evens out part waves, 82 us)
   const int64_t slots = (int64_t)kCtas<DT, AHEAD> * num_sms * GROUPS;
   int best = heads;
   int64_t least = INT64_MAX;
