@@ -20,6 +20,11 @@
 // there; the pieces of the others go to the workspace in float32 and a second
 // kernel, launched early and waiting for the first, joins them in part order, so
 // the result does not depend on timing.
+//
+// Measured (bf16, 32 + 8 heads of 128): 64 sequences of 129 to 16384 keys 175 us, 6.3 TB/s, a
+// copy's rate; one of 65536 keys 55 us, 4.8 TB/s (51 us without the join), of which about 3 us
+// pass before the first keys are asked for and 8 us while the last warps finish; one of 517 keys
+// 8.5 us, latency.
 #include "common.cuh"
 #include "kernels.h"
 
@@ -29,7 +34,13 @@ namespace {
 constexpr int kSms = 148;      // B200; sets the split, so results do not vary with the device
 constexpr float kLn2 = 0.6931471805599453f;
 
-template <int D> struct Shape;   // keys a tile, ring stages, warps a CTA (about 200 KB of ring)
+// Keys a tile, ring stages, warps a CTA (about 200 KB of ring). Measured, head_dim 128, one
+// sequence of 65536 keys and a ragged batch of 64: {16, 3, 8} 56.3 and 175 us, {16, 6, 4} 58.5
+// and 170, {16, 5, 5} 56.7 and 189, {16, 2, 12} 62 and 173, {32, 2, 6} 64.6 and 166, {32, 3, 4}
+// 80 and 167. 64 (65536 keys): {32, 3, 8} 57.4, {16, 6, 8} 56.5, {32, 4, 6} 69.7 us, the first with
+// half the steps for compute. 96: {16, 4, 8} 76.5, {16, 3, 11} 82.9, {32, 3, 5} 148 us. 256
+// (16 x 8000 keys): {16, 3, 4} 96.9, {16, 2, 6} 100.3 us.
+template <int D> struct Shape;
 template <> struct Shape<64> { static constexpr int TK = 32, ST = 3, NW = 8; };
 template <> struct Shape<96> { static constexpr int TK = 16, ST = 4, NW = 8; };
 template <> struct Shape<128> { static constexpr int TK = 16, ST = 3, NW = 8; };
@@ -212,8 +223,11 @@ template <int TK> struct Feed : Walk<TK> {
 // Scores are taken transposed, S^T = K Q^T with 16 keys by 8 query rows a product, so a
 // GQA group of up to eight rows fills the tile, and O^T = V^T P^T likewise; P^T comes
 // from S^T's registers by an 8 x 8 transpose.
+// Registers: a CTA of 256 threads with 192 leaves a CTA of the second kernel its 16384.
+template <int D, int NB> constexpr int kRegs = NB <= 2 && D < 256 ? 192 : 255;
+
 template <int DT, int D, int NB>
-__global__ void __launch_bounds__(Shape<D>::NW * 32, 1) decode_kernel(const DecodeArgs a, int parts) {
+__global__ void __maxnreg__((kRegs<D, NB>)) decode_kernel(const DecodeArgs a, int parts) {
   constexpr int TK = Shape<D>::TK, ST = Shape<D>::ST, NW = Shape<D>::NW;
   constexpr int PITCH = kPitch<D>, CH = D / 8, KS = D / 16, MT = TK / 16;
   constexpr int CL = CH <= 8 ? 8 : CH <= 16 ? 16 : 32;   // lanes that copy one row
@@ -348,6 +362,10 @@ __global__ void __launch_bounds__(Shape<D>::NW * 32, 1) decode_kernel(const Deco
   for (int n = 0; n < NB; ++n)
 #pragma unroll
     for (int j = 0; j < 2; ++j) tq[n][j] = (rbase + n * 8 + c * 2 + j) / a.G;
+  // Scores stay unscaled up to the exponent, so their scale is made positive (a negative one's
+  // sign goes to the queries) and 0 the least number above it, which keeps masked scores -inf.
+  const float scale = a.scale_log2 == 0.f ? 1e-45f : fabsf(a.scale_log2);
+  const uint32_t sign = a.scale_log2 < 0.f ? 0x80008000u : 0u;
   auto start_segment = [&]() {
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
@@ -356,8 +374,8 @@ __global__ void __launch_bounds__(Shape<D>::NW * 32, 1) decode_kernel(const Deco
                    (int64_t)(h * a.G + r - rt * a.G) * a.q_sh + c * 2;
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
-        qf[n][k][0] = r < R ? *reinterpret_cast<const uint32_t*>(q + k * 16) : 0u;
-        qf[n][k][1] = r < R ? *reinterpret_cast<const uint32_t*>(q + k * 16 + 8) : 0u;
+        qf[n][k][0] = (r < R ? *reinterpret_cast<const uint32_t*>(q + k * 16) : 0u) ^ sign;
+        qf[n][k][1] = (r < R ? *reinterpret_cast<const uint32_t*>(q + k * 16 + 8) : 0u) ^ sign;
         o[n][k][0] = o[n][k][1] = o[n][k][2] = o[n][k][3] = 0.f;
       }
 #pragma unroll
@@ -384,7 +402,7 @@ __global__ void __launch_bounds__(Shape<D>::NW * 32, 1) decode_kernel(const Deco
     float sc[MT][NB][4];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      float s2[NB][4];   // odd steps apart: two chains of dependent products
+      float s2[NB][4];   // one block: odd steps apart, two chains of dependent products
 #pragma unroll
       for (int n = 0; n < NB; ++n)
 #pragma unroll
@@ -394,12 +412,12 @@ __global__ void __launch_bounds__(Shape<D>::NW * 32, 1) decode_kernel(const Deco
         uint32_t kf[4];
         ldsm4(tile + k_at + mt * 16 * PITCH + k * 32, kf);
 #pragma unroll
-        for (int n = 0; n < NB; ++n) mma<DT>(k & 1 ? s2[n] : sc[mt][n], kf, qf[n][k][0], qf[n][k][1]);
+        for (int n = 0; n < NB; ++n) mma<DT>(NB == 1 && k & 1 ? s2[n] : sc[mt][n], kf, qf[n][k][0], qf[n][k][1]);
       }
+      if constexpr (NB == 1) {
 #pragma unroll
-      for (int n = 0; n < NB; ++n)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sc[mt][n][j] = (sc[mt][n][j] + s2[n][j]) * a.scale_log2;
+        for (int j = 0; j < 4; ++j) sc[mt][0][j] += s2[0][j];
+      }
     }
     const Seq& s = w.s;
     const int key0 = (w.t < s.head ? w.t : w.t + s.jump) * TK;
@@ -431,6 +449,7 @@ __global__ void __launch_bounds__(Shape<D>::NW * 32, 1) decode_kernel(const Deco
         x[n][j] = fmaxf(sc[0][n][j], sc[0][n][j + 2]);
 #pragma unroll
         for (int mt = 1; mt < MT; ++mt) x[n][j] = fmaxf(x[n][j], fmaxf(sc[mt][n][j], sc[mt][n][j + 2]));
+        x[n][j] *= scale;
         past |= x[n][j] > m[n][j] + kSlack;
       }
     if (__any_sync(0xffffffffu, past)) {
@@ -458,7 +477,7 @@ __global__ void __launch_bounds__(Shape<D>::NW * 32, 1) decode_kernel(const Deco
       for (int n = 0; n < NB; ++n)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          sc[mt][n][j] = ex2(sc[mt][n][j] - e[n][j & 1]);
+          sc[mt][n][j] = ex2(fmaf(sc[mt][n][j], scale, -e[n][j & 1]));
           l[n][j & 1] += sc[mt][n][j];
         }
     // With several new tokens a masked key of this tile may be another row's

@@ -23,6 +23,10 @@
 // counting alone, over the ordered bit patterns inside the crossing bin until it holds
 // one value. Counts are integers and sums run in a fixed order, so a call repeats bit
 // for bit.
+//
+// Measured: one row of 151936 bf16 logits, top-k 50 and top-p, 8.5 us; 33 of 50003 float16 under
+// every filter 19.7 us; 64 of 151936 float32, top-p, with log-probabilities 73 us; 200 of 151936
+// bf16 unfiltered with log-probabilities 52 us, 3.5 TB/s of logits and noise.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -40,8 +44,11 @@ constexpr int kKeyBits = 9;                  // bins over bit patterns, one a th
 constexpr int kList = 2048;                  // gathered candidates of a row
 constexpr int kFew = kThreads / 2;           // of them that one CTA looks through by itself
 constexpr int kListBytes = kList * 12;       // keys with indices, and weights
-constexpr int kSliceTwo = 80 * 1024;         // logits a CTA holds when two share an SM,
-constexpr int kSliceOne = 176 * 1024;        // and when it has the SM to itself
+// Logits a CTA holds when two share an SM (200 rows of 151936 bf16, unfiltered, and the nucleus
+// of 64 float32 rows: 51.6 and 73.0 us; a cap of 40 KB 71.2 and 73.1, of 160 KB 65.7 and 79.2), and
+// when it has the SM to itself
+constexpr int kSliceTwo = 80 * 1024;
+constexpr int kSliceOne = 176 * 1024;
 constexpr int kMaxCluster = 8;
 constexpr float kSpan = 32.f;                // of z in the bins: e^-32 of the weight is past them
 constexpr float kFloatMax = 3.402823466e+38f;
@@ -1295,8 +1302,8 @@ template <int DT> cudaError_t launch_dt(const SampleArgs& a, int num_sms, cudaSt
   constexpr int VE = Slice<DT, true>::VE;
   const int64_t chunks = ((int64_t)a.vocab + 2 * VE - 2) / VE;   // of a row at any alignment
   // The smallest cluster that holds a row with two CTAs an SM (one computes while the
-  // other loads), larger while the GPU has room for more CTAs; a row past that is held
-  // by one CTA an SM, or read again each time.
+  // other loads), larger while the GPU has room for more CTAs (their steps get shorter);
+  // a row past that is held by one CTA an SM, or read again each time.
   int n = 1;
   while (n < kMaxCluster && (chunks + n - 1) / n * 16 > kSliceTwo) n *= 2;
   while (n < kMaxCluster && (int64_t)a.rows * n * 2 <= 2 * num_sms) n *= 2;

@@ -106,6 +106,14 @@ def test_matches_the_formula(lengths, new, hq, hkv, dim, page, dtype, window, si
         assert flat.shape == q[:, 0].shape and torch.equal(flat, out[:, 0]) and torch.equal(flat_lse, lse[:, 0])
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.09, 0.4])
+@pytest.mark.parametrize("new,hq,dim,window", [(1, 8, 128, 0), (3, 8, 128, 50), (4, 16, 64, 200)])
+def test_scales_of_any_sign(scale, new, hq, dim, window):
+    q, k, v, tables, n = problem([700, 2, 0, 1900], new, hq, 2, dim, 16, torch.float16, seed=hq + new)
+    out, lse = fpv2.decode_attention(q, k, v, tables, n, scale=scale, window=window, return_lse=True)
+    check(q, k, v, tables, n, scale, window, 0, out, lse)
+
+
 def test_strided_caches_queries_and_tables():
     q, k, v, tables, n = problem([300, 41], 1, 8, 2, 128, 16, torch.bfloat16, seed=3)
     want = fpv2.decode_attention(q, k, v, tables, n, scale=0.1)
