@@ -22,9 +22,9 @@
 // the result does not depend on timing.
 //
 // Measured (bf16, 32 + 8 heads of 128): 64 sequences of 129 to 16384 keys 175 us, 6.3 TB/s, a
-// copy's rate; one of 65536 keys 55 us, 4.8 TB/s (51 us without the join), of which about 3 us
+// copy's rate; one of 65536 keys 53 us, 5.0 TB/s (50 us without the join), of which about 3 us
 // pass before the first keys are asked for and 8 us while the last warps finish; one of 517 keys
-// 8.5 us, latency.
+// 7.9 us, latency.
 #include "common.cuh"
 #include "kernels.h"
 
@@ -598,6 +598,18 @@ __global__ void __maxnreg__((kRegs<D, NB>)) decode_kernel(const DecodeArgs a, in
   cp_wait<0>();
 }
 
+// *p, or 0; in program order, so that many of them do not hold their addresses meanwhile.
+__device__ __forceinline__ float load_if(const float* p, bool read) {
+  float v;
+  asm volatile(
+      "{\n\t.reg .pred r;\n\tsetp.ne.s32 r, %2, 0;\n\tmov.f32 %0, 0f00000000;\n\t"
+      "@r ld.global.f32 %0, [%1];\n\t}"
+      : "=f"(v)
+      : "l"(p), "r"((int)read)
+      : "memory");
+  return v;
+}
+
 // Joins the pieces of the sequences that were cut:
 //   m = max m_i,  o = sum 2^(m_i - m) o_i / sum 2^(m_i - m) l_i,
 // and fills the rows of empty sequences. A warp takes a row, or, for few rows of many
@@ -609,7 +621,7 @@ __global__ void __maxnreg__((kRegs<D, NB>)) decode_kernel(const DecodeArgs a, in
 template <int DT, int D, bool ROW_CTA>
 __global__ void __launch_bounds__(256, 4) decode_join_kernel(const DecodeArgs a, int parts) {
   constexpr int TK = Shape<D>::TK, NV = ROW_CTA ? 1 : D / 32, WARPS = 8, WPR = ROW_CTA ? WARPS : 1;
-  __shared__ float red[WPR][33];
+  __shared__ float red[WPR][34];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % WPR;
   const int R = a.G * a.T, per = 8 * blocks_of(R, D), groups = row_groups(R, D), cols = a.Hkv * groups;
   const unsigned id = ROW_CTA ? blockIdx.x / (D / 32) : blockIdx.x * WARPS + warp;   // (b * Hkv + h) * R + r
@@ -627,58 +639,68 @@ __global__ void __launch_bounds__(256, 4) decode_join_kernel(const DecodeArgs a,
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (n > 0 && p0 == p1) return;   // finished by its warp
-  const float2* ml = reinterpret_cast<const float2*>(a.workspace);
-  const float* po = reinterpret_cast<const float*>(ml + (int64_t)parts * 2 * cols * per);
   const int count = n > 0 ? p1 - p0 + 1 : 0;
-  const int col = h * groups + r / per, lr = r % per;
-  auto slot_row = [&](int i) {   // the piece of part p0 + i: slot 1 where the sequence starts
-    return ((int64_t)((p0 + i) * 2 + (i == 0 && late ? 1 : 0)) * cols + col) * per + lr;
-  };
-  float m = -INFINITY;
-  for (int i = lane; i < count; i += 32) m = fmaxf(m, ml[slot_row(i)].x);
-  float acc[NV], l = 0.f, base = 0.f;
+  // the piece of part p0 + i, in slot 1 where the sequence starts
+  const int64_t step = (int64_t)2 * cols * per, first = ((int64_t)p0 * 2 * cols + h * groups + r / per) * per + r % per;
+  const int64_t zero = late ? (int64_t)cols * per : 0;
+  const float2* ml = reinterpret_cast<const float2*>(a.workspace) + first;
+  const float* po = reinterpret_cast<const float*>(reinterpret_cast<const float2*>(a.workspace) +
+                                                   (int64_t)parts * step) + first * D + d0;
+  // U pieces at a time, a lane the weight of one: their maxima, sums and outputs are all on
+  // their way at once (with the maximum over all pieces taken first, 24 sequences of up to 17
+  // pieces took 5.3 us here instead of 3.5, one of 148 pieces 6.0 instead of 2.8)
+  constexpr int U = 24 / NV;
+  float m = -INFINITY, acc[NV], l = 0.f;
 #pragma unroll
   for (int j = 0; j < NV; ++j) acc[j] = 0.f;
-  constexpr int U = NV == 1 ? 10 : NV == 2 ? 8 : NV <= 4 ? 4 : 2;   // pieces in flight a warp
   for (int i0 = sub; i0 < count; i0 += U * WPR) {
-    float2 x[U];
+    const int mine = i0 + lane * WPR;
+    float2 x = make_float2(-INFINITY, 0.f);
+    if (lane < U && mine < count) x = ml[mine * step + (mine == 0 ? zero : 0)];
     float v[U][NV];
+    const float* from = po + (i0 * step + (i0 == 0 ? zero : 0)) * D;
+    const float* next = po + (i0 + WPR) * step * D;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * WPR;
-      x[u] = make_float2(-INFINITY, 0.f);
 #pragma unroll
-      for (int j = 0; j < NV; ++j) v[u][j] = 0.f;
-      if (i < count) {
-        const int64_t at = slot_row(i);
-        x[u] = ml[at];
-#pragma unroll
-        for (int j = 0; j < NV; ++j) v[u][j] = po[at * D + d0 + 32 * j];
-      }
+      for (int j = 0; j < NV; ++j) v[u][j] = load_if(from + 32 * j, i0 + u * WPR < count);
+      from = next;
+      next += WPR * step * D;
     }
-    if (i0 == sub) {   // the maximum, while the first outputs are on their way
+    float to = fmaxf(m, x.x);
 #pragma unroll
-      for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
-      base = m == -INFINITY ? 0.f : m;
-    }
+    for (int s = 16; s > 0; s >>= 1) to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, s));
+    const float base = to == -INFINITY ? 0.f : to, f = ex2(m - base), w = ex2(x.x - base);
+    m = to;
+    l = fmaf(w, x.y, l * f);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) acc[j] *= f;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const float w = ex2(x[u].x - base);
-      l = fmaf(w, x[u].y, l);
+      const float wu = __shfl_sync(0xffffffffu, w, u);
 #pragma unroll
-      for (int j = 0; j < NV; ++j) acc[j] = fmaf(w, v[u][j], acc[j]);
+      for (int j = 0; j < NV; ++j) acc[j] = fmaf(wu, v[u][j], acc[j]);
     }
   }
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) l += __shfl_xor_sync(0xffffffffu, l, s);
   if constexpr (ROW_CTA) {
-    // (a warp without pieces did not reduce its maximum: the first has one and writes)
     red[sub][lane] = acc[0];
-    if (lane == 0) red[sub][32] = l;
+    if (lane == 0) {
+      red[sub][32] = l;
+      red[sub][33] = m;
+    }
     __syncthreads();
     if (sub != 0) return;
 #pragma unroll
-    for (int w = 1; w < WPR; ++w) {
-      acc[0] += red[w][lane];
-      l += red[w][32];
+    for (int w = 1; w < WPR; ++w) m = fmaxf(m, red[w][33]);
+    const float base = m == -INFINITY ? 0.f : m;
+    acc[0] = l = 0.f;
+#pragma unroll
+    for (int w = 0; w < WPR; ++w) {
+      const float f = ex2(red[w][33] - base);
+      acc[0] = fmaf(f, red[w][lane], acc[0]);
+      l = fmaf(f, red[w][32], l);
     }
   }
   const bool any = l > 0.f || l != l;
