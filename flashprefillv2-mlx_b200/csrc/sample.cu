@@ -50,6 +50,7 @@ constexpr int kListBytes = kList * 12;       // keys with indices, and weights
 constexpr int kSliceTwo = 80 * 1024;
 constexpr int kSliceOne = 176 * 1024;
 constexpr int kMaxCluster = 8;
+constexpr int kStreamWaves = 4;
 constexpr float kSpan = 32.f;                // of z in the bins: e^-32 of the weight is past them
 constexpr float kFloatMax = 3.402823466e+38f;
 constexpr uint32_t kLowest = 0x00800000u;    // order() of -FLT_MAX
@@ -106,8 +107,8 @@ template <int DT, bool HELD> struct Slice {
     return load(j);
   }
   // the chunk as floats, NaN as -inf
-  __device__ __forceinline__ void get(int j, float (&x)[VE]) const {
-    const uint4 u = at(j);
+  __device__ __forceinline__ void get(int j, float (&x)[VE]) const { floats(at(j), x); }
+  __device__ __forceinline__ void floats(const uint4 u, float (&x)[VE]) const {
     const uint32_t r[4] = {u.x, u.y, u.z, u.w};
     if constexpr (DT == DT_F32) {
 #pragma unroll
@@ -147,8 +148,8 @@ template <int DT, bool HELD> struct Slice {
       }
   }
   // the largest logit of a chunk (NaN and a row with infinities aside: it may be too large)
-  __device__ __forceinline__ float highest(int j) const {
-    const uint4 u = at(j);
+  __device__ __forceinline__ float highest(int j) const { return highest_of(at(j)); }
+  __device__ __forceinline__ static float highest_of(const uint4 u) {
     if constexpr (DT == DT_F32) {
       return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)),
                    fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
@@ -851,32 +852,21 @@ __device__ bool nucleus(cg::cluster_group& cl, Shared& sh, const Slice<DT, HELD>
   return false;
 }
 
-// The race over a CTA's tokens that the cut keeps (all but -inf with ALL): its best
-// pack(order(score), index), thread by thread. With sum_here the weights of all tokens
-// are added to `sum`.
-//
-// A thread's noise is loaded 16 values ahead of their use. Scores are first taken
-// roughly, in powers of two: for e = 2^k (1 + m) the exponent and mantissa bits read as one
-// number are k + m = log2 e - [0, 0.0861], three integer and float operations in place of
-// the special-function unit's, which the weights' exponentials keep busy. A thread keeps
-// its best chunk of them; then only the chunks within reach of the CTA's best are scored
-// exactly.
-template <int DT, bool HELD, bool ALL>
-__device__ __forceinline__ unsigned long long race(Shared& sh, const Slice<DT, HELD>& sl, const RowState& row,
-                                                   const Cut cut, const float* noise, bool sum_here, float& sum) {
-  constexpr int VE = Slice<DT, HELD>::VE, DEPTH = 16 / VE;
-  constexpr float kReach = 0.0861f + 1e-3f;   // the log's error, and the rounding of scores to about 500
-  const int tid = threadIdx.x;
-  // chunks whose noise is whole 16-byte words: all but a row's first and last, or none
-  const bool aligned = reinterpret_cast<uintptr_t>(noise + sl.first) % 16 == 0;
-  const int whole0 = sl.chunks > 0 && !sl.inside(0) ? 1 : 0;
-  const int whole1 = !aligned ? 0 : sl.chunks > 0 && !sl.inside(sl.chunks - 1) ? sl.chunks - 1 : sl.chunks;
-  const int4* words = reinterpret_cast<const int4*>(noise + sl.first);
-  int e[DEPTH][VE];   // bit patterns
-  auto fetch = [&](int j, int (&to)[VE]) {
-#pragma unroll
-    for (int i = 0; i < VE; ++i) to[i] = 0x7F800000;
-    if (j >= sl.chunks || (!ALL && !(sl.highest(j) >= cut.x))) return;
+// A row's noise beside its slice of logits.
+template <int DT, bool HELD> struct Noise {
+  static constexpr int VE = Slice<DT, HELD>::VE;
+  const float* noise;
+  const int4* words;
+  int whole0, whole1;   // chunks whose noise is whole 16-byte words: all but a row's first and last, or none
+
+  __device__ __forceinline__ Noise(const Slice<DT, HELD>& sl, const float* noise) : noise(noise) {
+    const bool aligned = reinterpret_cast<uintptr_t>(noise + sl.first) % 16 == 0;
+    whole0 = sl.chunks > 0 && !sl.inside(0) ? 1 : 0;
+    whole1 = !aligned ? 0 : sl.chunks > 0 && !sl.inside(sl.chunks - 1) ? sl.chunks - 1 : sl.chunks;
+    words = reinterpret_cast<const int4*>(noise + sl.first);
+  }
+  // bit patterns of chunk j's, left as they are outside the row
+  __device__ __forceinline__ void fetch(const Slice<DT, HELD>& sl, int j, int (&to)[VE]) const {
     if (j >= whole0 && j < whole1) {
 #pragma unroll
       for (int i = 0; i < VE; i += 4) {
@@ -889,47 +879,24 @@ __device__ __forceinline__ unsigned long long race(Shared& sh, const Slice<DT, H
       for (int i = 0; i < VE; ++i)
         if (at + i >= 0 && at + i < sl.vocab) to[i] = __float_as_int(noise[at + i]);
     }
-  };
-#pragma unroll
-  for (int u = 0; u < DEPTH; ++u) fetch(tid + u * kThreads, e[u]);
-  float best = -INFINITY, second = -INFINITY;   // of the thread's chunks
-  int best_j = 0, least = 0x7F800000;
-  bool any = false;
-  for (int jw = tid; jw < sl.chunks; jw += DEPTH * kThreads) {
-#pragma unroll
-    for (int u = 0; u < DEPTH; ++u) {
-      const int j = jw + u * kThreads;
-      if (j < sl.chunks) {
-        float x[VE], near = -INFINITY;
-        sl.get(j, x);
-        const int at = (int)sl.first + j * VE;
-#pragma unroll
-        for (int i = 0; i < VE; ++i) {
-          const float t = (x[i] - row.top) * row.to_log2;
-          if (sum_here) sum += ex2(t);
-          least = min(least, e[u][i]);
-          // 2^23 + bits / 2^8, exactly: 2^15 (k + m) and a constant
-          const float bits = __int_as_float(0x4B000000 | e[u][i] >> 8);
-          const float score = fmaf(bits, -0x1p-15f, t);
-          if (ALL) {
-            near = fmaxf(near, score);
-          } else if (cut.keeps(x[i], at + i)) {
-            near = fmaxf(near, score);
-            any = true;
-          }
-        }
-        if (near > best) {
-          second = best;
-          best = near;
-          best_j = j;
-        } else {
-          second = fmaxf(second, near);
-        }
-        fetch(j + DEPTH * kThreads, e[u]);
-      }
-    }
   }
-  any |= ALL && sl.chunks > 0;
+};
+
+// The race's rough score: t less the logarithm of noise with this bit pattern. 2^23 + bits / 2^8
+// is exact as a float: 2^15 (k + m) and a constant.
+__device__ __forceinline__ float rough_score(float t, int bits) {
+  return fmaf(__int_as_float(0x4B000000 | bits >> 8), -0x1p-15f, t);
+}
+constexpr float kReach = 0.0861f + 1e-3f;   // the log's error, and the rounding of scores to about 500
+
+// The best token by exact scores, given every thread's best and second best rough score of
+// its chunks, the best one's chunk, and the smallest noise pattern it saw.
+template <int DT, bool HELD>
+__device__ __forceinline__ unsigned long long race_end(Shared& sh, const Slice<DT, HELD>& sl, const RowState& row,
+                                                       const Cut cut, const float* noise, float best,
+                                                       float second, int best_j, int least, bool any) {
+  constexpr int VE = Slice<DT, HELD>::VE;
+  const int tid = threadIdx.x;
   const unsigned high = __reduce_max_sync(0xffffffffu, order(best));
   __syncthreads();
   if ((tid & 31) == 0) sh.warp_best[tid >> 5] = high;
@@ -957,8 +924,8 @@ __device__ __forceinline__ unsigned long long race(Shared& sh, const Slice<DT, H
           mine = i == q ? x[q] : mine;
           its = i == q ? n[q] : its;
         }
-        const float bits = __int_as_float(0x4B000000 | __float_as_int(its) >> 8);
-        if (!cut.keeps(mine, at + i) || (!odd && fmaf(bits, -0x1p-15f, (mine - row.top) * row.to_log2) < bar))
+        if (!cut.keeps(mine, at + i) ||
+            (!odd && rough_score((mine - row.top) * row.to_log2, __float_as_int(its)) < bar))
           continue;
         const float z = row.z(mine);
         if (z > -INFINITY) best_key = max(best_key, pack(order(race_score(z, its)), at + i));
@@ -966,6 +933,69 @@ __device__ __forceinline__ unsigned long long race(Shared& sh, const Slice<DT, H
     }
   }
   return best_key;
+}
+// The race over a CTA's tokens that the cut keeps (all but -inf with ALL): its best
+// pack(order(score), index), thread by thread. With sum_here the weights of all tokens
+// are added to `sum`.
+//
+// A thread's noise is loaded 16 values ahead of their use. Scores are first taken
+// roughly, in powers of two: for e = 2^k (1 + m) the exponent and mantissa bits read as one
+// number are k + m = log2 e - [0, 0.0861], three integer and float operations in place of
+// the special-function unit's, which the weights' exponentials keep busy. A thread keeps
+// its best chunk of them; then only the chunks within reach of the CTA's best are scored
+// exactly.
+template <int DT, bool HELD, bool ALL>
+__device__ __forceinline__ unsigned long long race(Shared& sh, const Slice<DT, HELD>& sl, const RowState& row,
+                                                   const Cut cut, const float* noise, bool sum_here, float& sum) {
+  constexpr int VE = Slice<DT, HELD>::VE, DEPTH = 16 / VE;
+  const int tid = threadIdx.x;
+  const Noise<DT, HELD> from(sl, noise);
+  int e[DEPTH][VE];   // bit patterns
+  auto fetch = [&](int j, int (&to)[VE]) {
+#pragma unroll
+    for (int i = 0; i < VE; ++i) to[i] = 0x7F800000;
+    if (j >= sl.chunks || (!ALL && !(sl.highest(j) >= cut.x))) return;
+    from.fetch(sl, j, to);
+  };
+#pragma unroll
+  for (int u = 0; u < DEPTH; ++u) fetch(tid + u * kThreads, e[u]);
+  float best = -INFINITY, second = -INFINITY;   // of the thread's chunks
+  int best_j = 0, least = 0x7F800000;
+  bool any = false;
+  for (int jw = tid; jw < sl.chunks; jw += DEPTH * kThreads) {
+#pragma unroll
+    for (int u = 0; u < DEPTH; ++u) {
+      const int j = jw + u * kThreads;
+      if (j < sl.chunks) {
+        float x[VE], near = -INFINITY;
+        sl.get(j, x);
+        const int at = (int)sl.first + j * VE;
+#pragma unroll
+        for (int i = 0; i < VE; ++i) {
+          const float t = (x[i] - row.top) * row.to_log2;
+          if (sum_here) sum += ex2(t);
+          least = min(least, e[u][i]);
+          const float score = rough_score(t, e[u][i]);
+          if (ALL) {
+            near = fmaxf(near, score);
+          } else if (cut.keeps(x[i], at + i)) {
+            near = fmaxf(near, score);
+            any = true;
+          }
+        }
+        if (near > best) {
+          second = best;
+          best = near;
+          best_j = j;
+        } else {
+          second = fmaxf(second, near);
+        }
+        fetch(j + DEPTH * kThreads, e[u]);
+      }
+    }
+  }
+  any |= ALL && sl.chunks > 0;
+  return race_end(sh, sl, row, cut, noise, best, second, best_j, least, any);
 }
 
 // Hands a CTA's best token and its part of the sum (thread 0's) to CTA 0. True for the
@@ -980,6 +1010,27 @@ __device__ __forceinline__ bool leave(cg::cluster_group& cl, Shared& sh, unsigne
   if (cl.block_rank() != 0) return true;
   asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
   return false;
+}
+
+// CTA 0, after leave(): the row's token, and its log-probability.
+template <int DT, bool HELD>
+__device__ __forceinline__ void finish(const SampleArgs& a, Shared& sh, const Slice<DT, HELD>& sl,
+                                       const RowState& row, int r, int nblocks) {
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    const unsigned long long v = warp_best(threadIdx.x < nblocks ? sh.best_of[threadIdx.x] : 0ull);
+    double sum = threadIdx.x < nblocks ? sh.sum_of[threadIdx.x] : 0.0;
+#pragma unroll
+    for (int o = 1; o < kMaxCluster; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (threadIdx.x == 0) {
+      const int token = (int)~(uint32_t)v;
+      a.tokens[r] = token;
+      if (a.logprobs != nullptr) {
+        const float x = sl.infinite ? 0.f : Elem<DT>::to_f(sl.row[token]);
+        a.logprobs[r] = (float)((double)row.z(x) - log(sum));
+      }
+    }
+  }
 }
 
 template <int DT, bool HELD>
@@ -1281,25 +1332,187 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
   } else if (single) {
     if (leave(cl, sh, best, part)) return;
   }
-  __syncthreads();
-  if (tid < 32) {
-    const unsigned long long v = warp_best(tid < nblocks ? sh.best_of[tid] : 0ull);
-    double sum = tid < nblocks ? sh.sum_of[tid] : 0.0;
+  finish(a, sh, sl, row, r, nblocks);
+}
+
+// Rows that nothing filters, or of which the largest is taken (GREEDY), when the settings
+// say so for all of them at launch: a row is read once and nothing is held. A thread takes
+// its scores and weights relative to a logit of its own, moved when one passes it by 8
+// powers of two; the row's maximum is exchanged when all is read.
+template <int DT, bool GREEDY>
+__global__ void __launch_bounds__(kThreads, 2) sample_stream_kernel(const SampleArgs a) {
+  using T = typename Elem<DT>::T;
+  constexpr int VE = Slice<DT, false>::VE, DEPTH = 16 / VE;
+  __shared__ Shared sh;
+  cg::cluster_group cl = cg::this_cluster();
+  const int tid = threadIdx.x, rank = (int)cl.block_rank(), nblocks = (int)cl.num_blocks();
+  const int r = blockIdx.x / nblocks;
+  // (with the wait below: every CTA of the cluster runs before its shared memory is written)
+  asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+  Slice<DT, false> sl;
+  sl.row = reinterpret_cast<const T*>(a.logits) + r * a.logits_stride;
+  sl.held = nullptr;
+  sl.vocab = a.vocab;
+  sl.infinite = false;
+  const int mis = (int)(reinterpret_cast<uintptr_t>(sl.row) % 16 / sizeof(T));
+  const int all = (int)(((int64_t)mis + a.vocab + VE - 1) / VE);
+  const int share = (all + nblocks - 1) / nblocks;
+  const int c0 = min(all, rank * share);
+  sl.chunks = min(share, all - c0);
+  sl.first = (int64_t)c0 * VE - mis;
+  const float* const noise = a.noise + r * a.noise_stride;
+  const bool want_sum = a.logprobs != nullptr;
+  RowState row;
+  row.heat = a.temperature_s > 0.f ? fmaxf(a.temperature_s, 1e-30f) : 1.f;
+  row.inv_heat = 1.f / row.heat;
+  row.to_log2 = row.inv_heat * kLog2e;
+
+  const Noise<DT, false> from(sl, noise);
+  uint4 u[DEPTH];
+  int e[DEPTH][VE];
+  auto fetch = [&](int j, uint4& logits, int (&to)[VE]) {
+    if (j >= sl.chunks) return;
+    logits = sl.load(j);
+    if constexpr (!GREEDY) {
 #pragma unroll
-    for (int o = 1; o < kMaxCluster; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (tid == 0) {
-      const int token = (int)~(uint32_t)v;
-      a.tokens[r] = token;
-      if (want_sum) {
-        const float x = sl.infinite ? 0.f : Elem<DT>::to_f(sl.row[token]);
-        a.logprobs[r] = (float)((double)row.z(x) - log(sum));
+      for (int i = 0; i < VE; ++i) to[i] = 0x7F800000;
+      from.fetch(sl, j, to);
+    }
+  };
+#pragma unroll
+  for (int d = 0; d < DEPTH; ++d) fetch(tid + d * kThreads, u[d], e[d]);
+  const float slack = 8.f / row.to_log2;
+  float ref = -INFINITY, base = 0.f, most = -INFINITY, sum = 0.f;   // base: ref, or 0 for -inf
+  float best = -INFINITY, second = -INFINITY;
+  int best_j = 0, least = 0x7F800000;
+  for (int jw = tid; jw < sl.chunks; jw += DEPTH * kThreads) {
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      const int j = jw + d * kThreads;
+      if (j < sl.chunks) {
+        const float high = Slice<DT, false>::highest_of(u[d]);
+        if (GREEDY && high > most) best_j = j;
+        most = fmaxf(most, high);
+        if (high > ref + slack) {
+          const float by = (ref - high) * row.to_log2;
+          sum *= ex2(by);
+          best += by;
+          second += by;
+          ref = base = high;
+        }
+        if (!GREEDY || want_sum) {
+          float x[VE], near = -INFINITY;
+          sl.floats(u[d], x);
+#pragma unroll
+          for (int i = 0; i < VE; ++i) {
+            const float t = (x[i] - base) * row.to_log2;
+            if (want_sum) sum += ex2(t);
+            if constexpr (!GREEDY) {
+              least = min(least, e[d][i]);
+              near = fmaxf(near, rough_score(t, e[d][i]));
+            }
+          }
+          if constexpr (!GREEDY) {
+            if (near > best) {
+              second = best;
+              best = near;
+              best_j = j;
+            } else {
+              second = fmaxf(second, near);
+            }
+          }
+        }
+        fetch(j + DEPTH * kThreads, u[d], e[d]);
       }
     }
   }
+
+  // the row's maximum
+  {
+    const unsigned high = __reduce_max_sync(0xffffffffu, order(most));
+    if ((tid & 31) == 0) sh.warp_best[tid >> 5] = high;
+    __syncthreads();
+    const unsigned of_cta = __reduce_max_sync(0xffffffffu, (unsigned)sh.warp_best[tid & (kWarps - 1)]);
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    if (tid < nblocks) cl.map_shared_rank(&sh, tid)->top_of[rank] = of_cta;
+  }
+  cl.sync();
+  unsigned top = 0;
+  for (int q = 0; q < nblocks; ++q) top = max(top, sh.top_of[q]);
+  row.top = unorder(top);
+  if (row.top == -INFINITY) {
+    if (rank == 0 && tid == 0) {
+      a.tokens[r] = -1;
+      if (want_sum) a.logprobs[r] = -INFINITY;
+    }
+    return;
+  }
+  unsigned long long key = 0;
+  float s[1] = {sum * ex2((ref - row.top) * row.to_log2)};
+  if (row.top == INFINITY) {
+    sl.infinite = true;   // such logits count as 0, others as -inf
+    row.top = 0.f;
+    s[0] = 0.f;
+    for (int j = tid; j < sl.chunks; j += kThreads) {
+      float x[VE];
+      sl.get(j, x);
+#pragma unroll
+      for (int i = 0; i < VE; ++i) s[0] += row.weight(x[i]);
+    }
+    if (!GREEDY) least = 0;   // all is scored exactly
+  }
+  if constexpr (GREEDY) {
+    // the first of this thread's that equal the maximum are in its chunk best_j
+    if (sl.chunks > tid) {
+      float x[VE];
+      sl.get(best_j, x);
+      unsigned at = 0xffffffffu;
+#pragma unroll
+      for (int i = 0; i < VE; ++i)
+        if (x[i] == row.top) at = min(at, (unsigned)(sl.index(best_j) + i));
+      if (at != 0xffffffffu) key = pack(1u, at);
+    }
+  } else {
+    const float by = (ref - row.top) * row.to_log2;
+    key = race_end(sh, sl, row, Cut{-kFloatMax, kAnyIndex}, noise, best + by, second + by, best_j, least,
+                   sl.chunks > 0);
+  }
+  key = block_best(sh, key);
+  if (want_sum) block_sum(sh, s, 3);
+  if (leave(cl, sh, key, want_sum ? sh.row_sums[3] : 0.0)) return;
+  finish(a, sh, sl, row, r, nblocks);
+}
+
+// A launch of clusters of n CTAs, one a row.
+cudaError_t launch_clusters(void (*kernel)(SampleArgs), const SampleArgs& a, int n, int smem, cudaStream_t stream) {
+  if ((int64_t)a.rows * n > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.rows * n));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = n;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+  if (e == cudaSuccess) count_launch();
+  return e;
 }
 
 template <int DT> cudaError_t launch_dt(const SampleArgs& a, int num_sms, cudaStream_t stream) {
   constexpr int VE = Slice<DT, true>::VE;
+  // what all rows' settings say, where they are given for all
+  const bool known = a.temperature == nullptr && a.top_k == nullptr && a.top_p == nullptr && a.min_p == nullptr;
+  const bool greedy = !(a.temperature_s > 0.f) || a.top_k_s == 1 || !(a.top_p_s > 0.f) || !(a.min_p_s <= 1.f);
+  const bool open = (a.top_k_s <= 0 || a.top_k_s >= a.vocab) && a.top_p_s >= 1.f && !(a.min_p_s > 0.f);
+  if (known && (greedy || open)) {
+    int n = 1;
+    while (n < kMaxCluster && (int64_t)a.rows * n * 2 <= kStreamWaves * 2 * num_sms) n *= 2;
+    return launch_clusters(greedy ? sample_stream_kernel<DT, true> : sample_stream_kernel<DT, false>, a, n, 0, stream);
+  }
   const int64_t chunks = ((int64_t)a.vocab + 2 * VE - 2) / VE;   // of a row at any alignment
   // The smallest cluster that holds a row with two CTAs an SM (one computes while the
   // other loads), larger while the GPU has room for more CTAs (their steps get shorter);
@@ -1315,21 +1528,7 @@ template <int DT> cudaError_t launch_dt(const SampleArgs& a, int num_sms, cudaSt
   cudaError_t e = allow_shared(reinterpret_cast<const void*>(kernel), kListBytes + (held ? kSliceOne : 0),
                                allowed[held]);
   if (e != cudaSuccess) return e;
-  if ((int64_t)a.rows * n > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(a.rows * n));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = n;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, kernel, a);
-  if (e == cudaSuccess) count_launch();
-  return e;
+  return launch_clusters(kernel, a, n, smem, stream);
 }
 
 }  // namespace

@@ -189,3 +189,20 @@ def test_draws_follow_the_probabilities():
     assert float(share[2]) == 0 and float(share[4]) == 0
     for i, at in enumerate((0, 1, 3)):
         assert abs(float(share[at]) - float(p[i])) <= 5 * math.sqrt(float(p[i]) / rows)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (3, 7), (2, 4099), (1, 151937), (40, 30011), (700, 513)])
+@pytest.mark.parametrize("temperature", [0.0, 0.6, 1.7])
+def test_unfiltered_rows(rows, vocab, dtype, temperature):
+    """Whole rows: rising and falling ones (whose running maximum keeps moving), far offsets,
+    masked stretches, odd starts in memory."""
+    logits, noise = inputs(rows, vocab + 3, dtype, seed=rows + vocab)
+    at = torch.arange(vocab + 3, device=DEV) / vocab
+    logits[0::4] += (at * 60).to(dtype)
+    logits[1::4] -= (at * 60).to(dtype)
+    logits[2::4] += 300
+    logits[:, : vocab // 3: 2] = -INF
+    logits[:, vocab // 2] = math.nan
+    check(logits[:, 3:], noise[:, 3:], temperature=temperature)
+    check(logits[:, 1:-2], noise[:, 2:-1], temperature=temperature)
