@@ -9,9 +9,9 @@
 // for e ~ Exp(1) a draw with probabilities w / sum w. T <= 0 takes the lowest index
 // of the maximum. A row without a logit above -inf gives -1.
 //
-// A row is read from DRAM once, into the shared memory of a cluster of 1 to 8 CTAs,
-// and noise is read only where a token is still in the running, so the bytes of the
-// two bound large batches and the chain of cluster-wide steps bounds single rows.
+// A row is read from DRAM once by a cluster of 1 to 8 CTAs: streamed where nothing filters it,
+// else into shared memory, with noise read only where a token is still in the running. The
+// bytes of the two bound large batches and the chain of cluster-wide steps single rows.
 //
 // Nothing is sorted but short lists. Top-k: every thread knows the largest logit of
 // its share; the (k / CTAs)-th largest of a CTA's 512 such values is a bound that at
@@ -24,9 +24,11 @@
 // one value. Counts are integers and sums run in a fixed order, so a call repeats bit
 // for bit.
 //
-// Measured: one row of 151936 bf16 logits, top-k 50 and top-p, 8.5 us; 33 of 50003 float16 under
-// every filter 19.7 us; 64 of 151936 float32, top-p, with log-probabilities 73 us; 200 of 151936
-// bf16 unfiltered with log-probabilities 52 us, 3.5 TB/s of logits and noise.
+// Measured, 151936 logits a row: one bf16 row, top-k 50 and top-p, 8.4 us; 64 float32 rows, top-p,
+// with log-probabilities 73 us; 200 bf16 rows unfiltered, with log-probabilities 44 us, 4.1 TB/s of
+// logits and noise, their largest alone 18 us. 33 float16 rows of 50003 under every filter 19.7 us.
+#include <algorithm>
+
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -50,7 +52,6 @@ constexpr int kListBytes = kList * 12;       // keys with indices, and weights
 constexpr int kSliceTwo = 80 * 1024;
 constexpr int kSliceOne = 176 * 1024;
 constexpr int kMaxCluster = 8;
-constexpr int kStreamWaves = 4;
 constexpr float kSpan = 32.f;                // of z in the bins: e^-32 of the weight is past them
 constexpr float kFloatMax = 3.402823466e+38f;
 constexpr uint32_t kLowest = 0x00800000u;    // order() of -FLT_MAX
@@ -189,6 +190,31 @@ struct Cut {
   }
 };
 
+template <int BYTES> __device__ __forceinline__ void copy_async(void* to, const void* from) {
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+}
+
+// This CTA's slice of row r.
+template <int DT, bool HELD>
+__device__ __forceinline__ Slice<DT, HELD> slice_of(const SampleArgs& a, cg::cluster_group& cl, int r, uint4* held) {
+  using S = Slice<DT, HELD>;
+  S sl;
+  sl.row = reinterpret_cast<const typename S::T*>(a.logits) + r * a.logits_stride;
+  sl.held = held;
+  sl.vocab = a.vocab;
+  sl.infinite = false;
+  const int mis = (int)(reinterpret_cast<uintptr_t>(sl.row) % 16 / sizeof(typename S::T));
+  const int all = (int)(((int64_t)mis + a.vocab + S::VE - 1) / S::VE);
+  const int nblocks = (int)cl.num_blocks(), share = (all + nblocks - 1) / nblocks;
+  const int c0 = min(all, (int)cl.block_rank() * share);
+  sl.chunks = min(share, all - c0);
+  sl.first = (int64_t)c0 * S::VE - mis;
+  return sl;
+}
+
 struct Shared {
   unsigned hist[kBins];
   unsigned long long warp_best[kWarps];
@@ -321,6 +347,23 @@ struct RowState {
     return x == top ? 0 : (int)fminf((top - x) * scale * 0.5f, (float)(kThreads - 1));
   }
 };
+
+__device__ __forceinline__ RowState row_state(float heat, float top_p, float min_p) {
+  RowState row;
+  row.heat = heat > 0.f ? fmaxf(heat, 1e-30f) : 1.f;   // its reciprocal stays finite
+  row.inv_heat = 1.f / row.heat;
+  row.to_log2 = row.inv_heat * kLog2e;
+  row.scale = (float)kBins / kSpan * row.inv_heat;
+  row.top = 0.f;
+  row.top_p = top_p;
+  row.min_p = min_p;
+  return row;
+}
+
+// Settings that leave the largest logit's first token alone.
+__host__ __device__ inline bool takes_largest(float heat, int top_k, float top_p, float min_p) {
+  return !(heat > 0.f) || top_k == 1 || !(top_p > 0.f) || !(min_p <= 1.f);
+}
 
 // Descending bitonic sort of the n <= kList values of `v` (shared memory) by the first
 // warps of the CTA, four values a thread in registers: steps of 1 and 2 inside a
@@ -934,7 +977,7 @@ __device__ __forceinline__ unsigned long long race_end(Shared& sh, const Slice<D
   }
   return best_key;
 }
-// The race over a CTA's tokens that the cut keeps (all but -inf with ALL): its best
+// The race over a CTA's tokens that the cut keeps: its best
 // pack(order(score), index), thread by thread. With sum_here the weights of all tokens
 // are added to `sum`.
 //
@@ -944,7 +987,7 @@ __device__ __forceinline__ unsigned long long race_end(Shared& sh, const Slice<D
 // the special-function unit's, which the weights' exponentials keep busy. A thread keeps
 // its best chunk of them; then only the chunks within reach of the CTA's best are scored
 // exactly.
-template <int DT, bool HELD, bool ALL>
+template <int DT, bool HELD>
 __device__ __forceinline__ unsigned long long race(Shared& sh, const Slice<DT, HELD>& sl, const RowState& row,
                                                    const Cut cut, const float* noise, bool sum_here, float& sum) {
   constexpr int VE = Slice<DT, HELD>::VE, DEPTH = 16 / VE;
@@ -954,7 +997,7 @@ __device__ __forceinline__ unsigned long long race(Shared& sh, const Slice<DT, H
   auto fetch = [&](int j, int (&to)[VE]) {
 #pragma unroll
     for (int i = 0; i < VE; ++i) to[i] = 0x7F800000;
-    if (j >= sl.chunks || (!ALL && !(sl.highest(j) >= cut.x))) return;
+    if (j >= sl.chunks || !(sl.highest(j) >= cut.x)) return;
     from.fetch(sl, j, to);
   };
 #pragma unroll
@@ -976,9 +1019,7 @@ __device__ __forceinline__ unsigned long long race(Shared& sh, const Slice<DT, H
           if (sum_here) sum += ex2(t);
           least = min(least, e[u][i]);
           const float score = rough_score(t, e[u][i]);
-          if (ALL) {
-            near = fmaxf(near, score);
-          } else if (cut.keeps(x[i], at + i)) {
+          if (cut.keeps(x[i], at + i)) {
             near = fmaxf(near, score);
             any = true;
           }
@@ -994,7 +1035,6 @@ __device__ __forceinline__ unsigned long long race(Shared& sh, const Slice<DT, H
       }
     }
   }
-  any |= ALL && sl.chunks > 0;
   return race_end(sh, sl, row, cut, noise, best, second, best_j, least, any);
 }
 
@@ -1033,6 +1073,184 @@ __device__ __forceinline__ void finish(const SampleArgs& a, Shared& sh, const Sl
   }
 }
 
+// A row that nothing filters, or of which the largest is taken (GREEDY): it is read once and
+// not held. A thread takes its scores and weights relative to a logit of its own, moved when
+// one passes it by 8 powers of two; the row's maximum is exchanged when all is read. Chunks
+// on their way are in shared memory: loads to registers
+// would have to pass what the other uses of shared memory leave of the L1 (200 rows of 151936
+// bf16 54.8 us so, 44.8 us now).
+constexpr int kStages = 4;
+template <int DT> constexpr int kStreamBytes = kStages * kThreads * 16 * (1 + Slice<DT, false>::VE / 4);
+
+template <int DT, bool GREEDY>
+__device__ __forceinline__ void stream_row(const SampleArgs& a, cg::cluster_group& cl, Shared& sh,
+                                           Slice<DT, false> sl, RowState row, const float* noise, int r,
+                                           unsigned char* ring) {
+  constexpr int VE = Slice<DT, false>::VE, PARTS = 1 + VE / 4;
+  const int tid = threadIdx.x, rank = (int)cl.block_rank(), nblocks = (int)cl.num_blocks();
+  const bool want_sum = a.logprobs != nullptr;
+  const int lane = tid & 31;
+  const bool aligned = reinterpret_cast<uintptr_t>(noise + sl.first) % 16 == 0;
+  // a warp's stage: 32 chunks of logits, then their noise, in pieces of 16 bytes; with two
+  // pieces a chunk every other eight are swapped in pairs, for threads' reads to differ in banks
+  uint4* const stages = reinterpret_cast<uint4*>(ring) + (tid - lane) * PARTS;
+  auto piece = [](int c) { return 32 + (PARTS == 3 ? c ^ (c >> 3 & 1) : c); };
+  // chunks j0 to j0 + 31, whose noise the lanes copy in its order in memory
+  auto issue = [&](int j0, int stage) {
+    if (j0 < sl.chunks) {
+      uint4* const to = stages + stage * PARTS * kThreads;
+      const int j = j0 + lane;
+      const bool whole = !GREEDY && j0 + 31 < sl.chunks && sl.inside(j0) && sl.inside(j0 + 31);
+      if (whole || (j < sl.chunks && sl.inside(j)))
+        copy_async<16>(to + lane, sl.row + sl.index(j));
+      else if (j < sl.chunks)
+        to[lane] = sl.load(j);
+      if constexpr (!GREEDY) {
+        if (whole && aligned) {
+          const float* e = noise + sl.index(j0);
+#pragma unroll
+          for (int c = lane; c < 32 * (PARTS - 1); c += 32) copy_async<16>(to + piece(c), e + 4 * c);
+        } else if (j < sl.chunks) {
+#pragma unroll
+          for (int i = 0; i < VE; ++i) {
+            const int64_t at = sl.index(j) + i;
+            float* const one = reinterpret_cast<float*>(to + piece(lane * (PARTS - 1) + i / 4)) + i % 4;
+            if (at >= 0 && at < sl.vocab)
+              copy_async<4>(one, noise + at);
+            else
+              *one = INFINITY;
+          }
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) issue(tid - lane + i * kThreads, i);
+  const float slack = 8.f / row.to_log2;
+  float ref = -INFINITY, base = 0.f, most = -INFINITY, sum = 0.f;   // base: ref, or 0 for -inf
+  float best = -INFINITY, second = -INFINITY;
+  int best_j = 0, least = 0x7F800000, stage = 0;
+  for (int j0 = tid - lane; j0 < sl.chunks; j0 += kThreads) {
+    if constexpr (!GREEDY) __syncwarp();   // the last round's reads are over
+    issue(j0 + (kStages - 1) * kThreads, (stage + kStages - 1) % kStages);
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+    if constexpr (!GREEDY) __syncwarp();
+    const uint4* const from = stages + stage * PARTS * kThreads;
+    stage = (stage + 1) % kStages;
+    const int j = j0 + lane;
+    if (j >= sl.chunks) continue;
+    const uint4 u = from[lane];
+    const float high = Slice<DT, false>::highest_of(u);
+    if (GREEDY && high > most) best_j = j;
+    most = fmaxf(most, high);
+    if (high > ref + slack) {
+      const float by = (ref - high) * row.to_log2;
+      sum *= ex2(by);
+      best += by;
+      second += by;
+      ref = base = high;
+    }
+    if (GREEDY && !want_sum) continue;
+    float x[VE], near = -INFINITY;
+    sl.floats(u, x);
+    int e[VE];
+    if constexpr (!GREEDY) {
+#pragma unroll
+      for (int p = 1; p < PARTS; ++p) {
+        const uint4 w = from[piece(lane * (PARTS - 1) + p - 1)];
+        e[4 * p - 4] = (int)w.x, e[4 * p - 3] = (int)w.y, e[4 * p - 2] = (int)w.z, e[4 * p - 1] = (int)w.w;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VE; ++i) {
+      const float t = (x[i] - base) * row.to_log2;
+      if (want_sum) sum += ex2(t);
+      if constexpr (!GREEDY) {
+        least = min(least, e[i]);
+        near = fmaxf(near, rough_score(t, e[i]));
+      }
+    }
+    if constexpr (!GREEDY) {
+      if (near > best) {
+        second = best;
+        best = near;
+        best_j = j;
+      } else {
+        second = fmaxf(second, near);
+      }
+    }
+  }
+
+  // the row's maximum
+  {
+    const unsigned high = __reduce_max_sync(0xffffffffu, order(most));
+    if ((tid & 31) == 0) sh.warp_best[tid >> 5] = high;
+    __syncthreads();
+    const unsigned of_cta = __reduce_max_sync(0xffffffffu, (unsigned)sh.warp_best[tid & (kWarps - 1)]);
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    if (tid < nblocks) cl.map_shared_rank(&sh, tid)->top_of[rank] = of_cta;
+  }
+  cl.sync();
+  unsigned top = 0;
+  for (int q = 0; q < nblocks; ++q) top = max(top, sh.top_of[q]);
+  row.top = unorder(top);
+  if (row.top == -INFINITY) {
+    if (rank == 0 && tid == 0) {
+      a.tokens[r] = -1;
+      if (want_sum) a.logprobs[r] = -INFINITY;
+    }
+    return;
+  }
+  unsigned long long key = 0;
+  float s[1] = {sum * ex2((ref - row.top) * row.to_log2)};
+  if (row.top == INFINITY) {
+    sl.infinite = true;   // such logits count as 0, others as -inf
+    row.top = 0.f;
+    s[0] = 0.f;
+    for (int j = tid; j < sl.chunks; j += kThreads) {
+      float x[VE];
+      sl.get(j, x);
+#pragma unroll
+      for (int i = 0; i < VE; ++i) s[0] += row.weight(x[i]);
+    }
+    if (!GREEDY) least = 0;   // all is scored exactly
+  }
+  if constexpr (GREEDY) {
+    // the first of this thread's that equal the maximum are in its chunk best_j
+    if (sl.chunks > tid) {
+      float x[VE];
+      sl.get(best_j, x);
+      unsigned at = 0xffffffffu;
+#pragma unroll
+      for (int i = 0; i < VE; ++i)
+        if (x[i] == row.top) at = min(at, (unsigned)(sl.index(best_j) + i));
+      if (at != 0xffffffffu) key = pack(1u, at);
+    }
+  } else {
+    const float by = (ref - row.top) * row.to_log2;
+    key = race_end(sh, sl, row, Cut{-kFloatMax, kAnyIndex}, noise, best + by, second + by, best_j, least,
+                   sl.chunks > 0);
+  }
+  key = block_best(sh, key);
+  if (want_sum) block_sum(sh, s, 3);
+  if (leave(cl, sh, key, want_sum ? sh.row_sums[3] : 0.0)) return;
+  finish(a, sh, sl, row, r, nblocks);
+}
+
+// Rows whose settings are all known at launch to need stream_row().
+template <int DT, bool GREEDY>
+__global__ void __launch_bounds__(kThreads, 2) sample_stream_kernel(const SampleArgs a) {
+  extern __shared__ __align__(16) unsigned char dyn[];
+  __shared__ Shared sh;
+  cg::cluster_group cl = cg::this_cluster();
+  const int r = blockIdx.x / cl.num_blocks();
+  // (with the wait in stream_row(): every CTA of the cluster runs before its shared memory is written)
+  asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+  stream_row<DT, GREEDY>(a, cl, sh, slice_of<DT, false>(a, cl, r, nullptr), row_state(a.temperature_s, 1.f, 0.f),
+                         a.noise + r * a.noise_stride, r, dyn);
+}
+
 template <int DT, bool HELD>
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a) {
   using T = typename Elem<DT>::T;
@@ -1049,45 +1267,34 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
   // (with the wait below: every CTA of the cluster runs before its shared memory is written)
   asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
 
-  Slice<DT, HELD> sl;
-  sl.row = reinterpret_cast<const T*>(a.logits) + r * a.logits_stride;
-  sl.vocab = a.vocab;
-  sl.infinite = false;
-  const int mis = (int)(reinterpret_cast<uintptr_t>(sl.row) % 16 / sizeof(T));
-  const int all = (int)(((int64_t)mis + a.vocab + VE - 1) / VE);
-  const int share = (all + nblocks - 1) / nblocks;
-  const int c0 = min(all, rank * share);
-  sl.chunks = min(share, all - c0);
-  sl.first = (int64_t)c0 * VE - mis;
-  sl.held = held;
+  // settings
+  const float heat = a.temperature != nullptr ? a.temperature[r] : a.temperature_s;
+  const int k_set = a.top_k != nullptr ? a.top_k[r] : a.top_k_s;
+  RowState row = row_state(heat, a.top_p != nullptr ? a.top_p[r] : a.top_p_s, a.min_p != nullptr ? a.min_p[r] : a.min_p_s);
+  Slice<DT, HELD> sl = slice_of<DT, HELD>(a, cl, r, held);
+  const float* noise = a.noise + r * a.noise_stride;
+  const bool use_k = k_set > 0 && k_set < a.vocab;
+  const bool use_p = !(row.top_p >= 1.f);
+  const bool single = takes_largest(heat, k_set, row.top_p, row.min_p);
+  if (single || (!use_k && !use_p && !(row.min_p > 0.f))) {
+    const Slice<DT, false> all = slice_of<DT, false>(a, cl, r, nullptr);
+    if (single)
+      stream_row<DT, true>(a, cl, sh, all, row, noise, r, dyn);
+    else
+      stream_row<DT, false>(a, cl, sh, all, row, noise, r, dyn);
+    return;
+  }
   if constexpr (HELD) {
     for (int j = tid; j < sl.chunks; j += kThreads) {
       if (sl.inside(j))
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(held + j)),
-                     "l"(sl.row + sl.index(j))
-                     : "memory");
+        copy_async<16>(held + j, sl.row + sl.index(j));
       else
         held[j] = sl.load(j);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
-  // settings
-  RowState row;
-  const float heat = a.temperature != nullptr ? a.temperature[r] : a.temperature_s;
-  row.top_p = a.top_p != nullptr ? a.top_p[r] : a.top_p_s;
-  row.min_p = a.min_p != nullptr ? a.min_p[r] : a.min_p_s;
-  const int k_set = a.top_k != nullptr ? a.top_k[r] : a.top_k_s;
-  const bool greedy = !(heat > 0.f);
-  row.heat = greedy ? 1.f : fmaxf(heat, 1e-30f);   // its reciprocal stays finite
-  row.inv_heat = 1.f / row.heat;
-  row.to_log2 = row.inv_heat * kLog2e;
-  row.scale = (float)kBins / kSpan * row.inv_heat;
-  const bool use_k = k_set > 0 && k_set < a.vocab;
-  const bool use_p = !(row.top_p >= 1.f);
-  const bool single = greedy || k_set == 1 || !(row.top_p > 0.f) || !(row.min_p <= 1.f);
   const int need = (k_set + nblocks - 1) / nblocks;
-  const bool use_list = !single && use_k && need <= kThreads;
-  const float* noise = a.noise + r * a.noise_stride;
+  const bool use_list = use_k && need <= kThreads;
   sh.hist[tid] = sh.hist[tid + kThreads] = 0;
   if (tid == 0) sh.count = 0;
   // A thread reads back its own chunks only, here and below, but for tie_index().
@@ -1158,23 +1365,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
   double part = 0;
   const bool want_sum = a.logprobs != nullptr;
   bool done = false;
-  if (single) {
-    unsigned at = 0xffffffffu;
-    float s[1] = {0.f};
-    for (int j = tid; j < sl.chunks; j += kThreads) {
-      float x[VE];
-      sl.get(j, x);
-#pragma unroll
-      for (int i = 0; i < VE; ++i) {
-        if (x[i] == row.top) at = min(at, (unsigned)(sl.index(j) + i));
-        if (want_sum) s[0] += row.weight(x[i]);
-      }
-    }
-    best = block_best(sh, at == 0xffffffffu ? 0ull : pack(1u, at));
-    if (want_sum) block_sum(sh, s);
-    part = sh.row_sums[0];
-    done = true;
-  } else if (use_list) {
+  if (use_list) {
     float s[1] = {0.f};
     for (int j = tid; j < sl.chunks; j += kThreads) {
       if (!want_sum && !(sl.highest(j) >= bound)) continue;
@@ -1323,163 +1514,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     }
     const bool sum_here = want_sum && !have_sum;
     float s[1] = {0.f};
-    best = block_best(sh, cut.x == -kFloatMax && cut.last == kAnyIndex
-                              ? race<DT, HELD, true>(sh, sl, row, cut, noise, sum_here, s[0])
-                              : race<DT, HELD, false>(sh, sl, row, cut, noise, sum_here, s[0]));
+    best = block_best(sh, race(sh, sl, row, cut, noise, sum_here, s[0]));
     if (sum_here) block_sum(sh, s, 3);
     part = sum_here ? sh.row_sums[3] : rank == 0 ? whole : 0.0;
     if (leave(cl, sh, best, part)) return;
-  } else if (single) {
-    if (leave(cl, sh, best, part)) return;
   }
-  finish(a, sh, sl, row, r, nblocks);
-}
-
-// Rows that nothing filters, or of which the largest is taken (GREEDY), when the settings
-// say so for all of them at launch: a row is read once and nothing is held. A thread takes
-// its scores and weights relative to a logit of its own, moved when one passes it by 8
-// powers of two; the row's maximum is exchanged when all is read.
-template <int DT, bool GREEDY>
-__global__ void __launch_bounds__(kThreads, 2) sample_stream_kernel(const SampleArgs a) {
-  using T = typename Elem<DT>::T;
-  constexpr int VE = Slice<DT, false>::VE, DEPTH = 16 / VE;
-  __shared__ Shared sh;
-  cg::cluster_group cl = cg::this_cluster();
-  const int tid = threadIdx.x, rank = (int)cl.block_rank(), nblocks = (int)cl.num_blocks();
-  const int r = blockIdx.x / nblocks;
-  // (with the wait below: every CTA of the cluster runs before its shared memory is written)
-  asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
-  Slice<DT, false> sl;
-  sl.row = reinterpret_cast<const T*>(a.logits) + r * a.logits_stride;
-  sl.held = nullptr;
-  sl.vocab = a.vocab;
-  sl.infinite = false;
-  const int mis = (int)(reinterpret_cast<uintptr_t>(sl.row) % 16 / sizeof(T));
-  const int all = (int)(((int64_t)mis + a.vocab + VE - 1) / VE);
-  const int share = (all + nblocks - 1) / nblocks;
-  const int c0 = min(all, rank * share);
-  sl.chunks = min(share, all - c0);
-  sl.first = (int64_t)c0 * VE - mis;
-  const float* const noise = a.noise + r * a.noise_stride;
-  const bool want_sum = a.logprobs != nullptr;
-  RowState row;
-  row.heat = a.temperature_s > 0.f ? fmaxf(a.temperature_s, 1e-30f) : 1.f;
-  row.inv_heat = 1.f / row.heat;
-  row.to_log2 = row.inv_heat * kLog2e;
-
-  const Noise<DT, false> from(sl, noise);
-  uint4 u[DEPTH];
-  int e[DEPTH][VE];
-  auto fetch = [&](int j, uint4& logits, int (&to)[VE]) {
-    if (j >= sl.chunks) return;
-    logits = sl.load(j);
-    if constexpr (!GREEDY) {
-#pragma unroll
-      for (int i = 0; i < VE; ++i) to[i] = 0x7F800000;
-      from.fetch(sl, j, to);
-    }
-  };
-#pragma unroll
-  for (int d = 0; d < DEPTH; ++d) fetch(tid + d * kThreads, u[d], e[d]);
-  const float slack = 8.f / row.to_log2;
-  float ref = -INFINITY, base = 0.f, most = -INFINITY, sum = 0.f;   // base: ref, or 0 for -inf
-  float best = -INFINITY, second = -INFINITY;
-  int best_j = 0, least = 0x7F800000;
-  for (int jw = tid; jw < sl.chunks; jw += DEPTH * kThreads) {
-#pragma unroll
-    for (int d = 0; d < DEPTH; ++d) {
-      const int j = jw + d * kThreads;
-      if (j < sl.chunks) {
-        const float high = Slice<DT, false>::highest_of(u[d]);
-        if (GREEDY && high > most) best_j = j;
-        most = fmaxf(most, high);
-        if (high > ref + slack) {
-          const float by = (ref - high) * row.to_log2;
-          sum *= ex2(by);
-          best += by;
-          second += by;
-          ref = base = high;
-        }
-        if (!GREEDY || want_sum) {
-          float x[VE], near = -INFINITY;
-          sl.floats(u[d], x);
-#pragma unroll
-          for (int i = 0; i < VE; ++i) {
-            const float t = (x[i] - base) * row.to_log2;
-            if (want_sum) sum += ex2(t);
-            if constexpr (!GREEDY) {
-              least = min(least, e[d][i]);
-              near = fmaxf(near, rough_score(t, e[d][i]));
-            }
-          }
-          if constexpr (!GREEDY) {
-            if (near > best) {
-              second = best;
-              best = near;
-              best_j = j;
-            } else {
-              second = fmaxf(second, near);
-            }
-          }
-        }
-        fetch(j + DEPTH * kThreads, u[d], e[d]);
-      }
-    }
-  }
-
-  // the row's maximum
-  {
-    const unsigned high = __reduce_max_sync(0xffffffffu, order(most));
-    if ((tid & 31) == 0) sh.warp_best[tid >> 5] = high;
-    __syncthreads();
-    const unsigned of_cta = __reduce_max_sync(0xffffffffu, (unsigned)sh.warp_best[tid & (kWarps - 1)]);
-    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
-    if (tid < nblocks) cl.map_shared_rank(&sh, tid)->top_of[rank] = of_cta;
-  }
-  cl.sync();
-  unsigned top = 0;
-  for (int q = 0; q < nblocks; ++q) top = max(top, sh.top_of[q]);
-  row.top = unorder(top);
-  if (row.top == -INFINITY) {
-    if (rank == 0 && tid == 0) {
-      a.tokens[r] = -1;
-      if (want_sum) a.logprobs[r] = -INFINITY;
-    }
-    return;
-  }
-  unsigned long long key = 0;
-  float s[1] = {sum * ex2((ref - row.top) * row.to_log2)};
-  if (row.top == INFINITY) {
-    sl.infinite = true;   // such logits count as 0, others as -inf
-    row.top = 0.f;
-    s[0] = 0.f;
-    for (int j = tid; j < sl.chunks; j += kThreads) {
-      float x[VE];
-      sl.get(j, x);
-#pragma unroll
-      for (int i = 0; i < VE; ++i) s[0] += row.weight(x[i]);
-    }
-    if (!GREEDY) least = 0;   // all is scored exactly
-  }
-  if constexpr (GREEDY) {
-    // the first of this thread's that equal the maximum are in its chunk best_j
-    if (sl.chunks > tid) {
-      float x[VE];
-      sl.get(best_j, x);
-      unsigned at = 0xffffffffu;
-#pragma unroll
-      for (int i = 0; i < VE; ++i)
-        if (x[i] == row.top) at = min(at, (unsigned)(sl.index(best_j) + i));
-      if (at != 0xffffffffu) key = pack(1u, at);
-    }
-  } else {
-    const float by = (ref - row.top) * row.to_log2;
-    key = race_end(sh, sl, row, Cut{-kFloatMax, kAnyIndex}, noise, best + by, second + by, best_j, least,
-                   sl.chunks > 0);
-  }
-  key = block_best(sh, key);
-  if (want_sum) block_sum(sh, s, 3);
-  if (leave(cl, sh, key, want_sum ? sh.row_sums[3] : 0.0)) return;
   finish(a, sh, sl, row, r, nblocks);
 }
 
@@ -1506,12 +1545,27 @@ template <int DT> cudaError_t launch_dt(const SampleArgs& a, int num_sms, cudaSt
   constexpr int VE = Slice<DT, true>::VE;
   // what all rows' settings say, where they are given for all
   const bool known = a.temperature == nullptr && a.top_k == nullptr && a.top_p == nullptr && a.min_p == nullptr;
-  const bool greedy = !(a.temperature_s > 0.f) || a.top_k_s == 1 || !(a.top_p_s > 0.f) || !(a.min_p_s <= 1.f);
+  const bool greedy = takes_largest(a.temperature_s, a.top_k_s, a.top_p_s, a.min_p_s);
   const bool open = (a.top_k_s <= 0 || a.top_k_s >= a.vocab) && a.top_p_s >= 1.f && !(a.min_p_s > 0.f);
   if (known && (greedy || open)) {
+    // the shortest sum of waves of CTAs, what a CTA does besides reading its part counting as
+    // 150 KB (clusters of 1, 4 and 8: 64 rows of 151936 float32 32.1, 18.9 and 24.7 us; of 1 and
+    // 8: 200 rows of bf16 44 and 59 us, one row 24.4 and 8.3 us)
+    const int64_t bytes = (int64_t)a.vocab * ((DT == DT_F32 ? 4 : 2) + (greedy ? 0 : 4));
     int n = 1;
-    while (n < kMaxCluster && (int64_t)a.rows * n * 2 <= kStreamWaves * 2 * num_sms) n *= 2;
-    return launch_clusters(greedy ? sample_stream_kernel<DT, true> : sample_stream_kernel<DT, false>, a, n, 0, stream);
+    int64_t least = INT64_MAX;
+    for (int m = 1; m <= kMaxCluster; m *= 2) {
+      const int64_t cost = ((int64_t)a.rows * m + 2 * num_sms - 1) / (2 * num_sms) * (150 * 1024 + bytes / m);
+      if (cost < least) {
+        least = cost;
+        n = m;
+      }
+    }
+    auto kernel = greedy ? sample_stream_kernel<DT, true> : sample_stream_kernel<DT, false>;
+    static std::atomic<uint64_t> allowed[2];
+    const cudaError_t e = allow_shared(reinterpret_cast<const void*>(kernel), kStreamBytes<DT>, allowed[greedy]);
+    if (e != cudaSuccess) return e;
+    return launch_clusters(kernel, a, n, kStreamBytes<DT>, stream);
   }
   const int64_t chunks = ((int64_t)a.vocab + 2 * VE - 2) / VE;   // of a row at any alignment
   // The smallest cluster that holds a row with two CTAs an SM (one computes while the
@@ -1522,11 +1576,11 @@ template <int DT> cudaError_t launch_dt(const SampleArgs& a, int num_sms, cudaSt
   while (n < kMaxCluster && (int64_t)a.rows * n * 2 <= 2 * num_sms) n *= 2;
   const int64_t per = (chunks + n - 1) / n;
   const bool held = per * 16 <= kSliceOne;
-  const int smem = kListBytes + (held ? (int)per * 16 : 0);
+  const int smem = std::max(kListBytes + (held ? (int)per * 16 : 0), kStreamBytes<DT>);
   auto kernel = held ? sample_kernel<DT, true> : sample_kernel<DT, false>;
   static std::atomic<uint64_t> allowed[2];
-  cudaError_t e = allow_shared(reinterpret_cast<const void*>(kernel), kListBytes + (held ? kSliceOne : 0),
-                               allowed[held]);
+  cudaError_t e = allow_shared(reinterpret_cast<const void*>(kernel),
+                               std::max(kListBytes + (held ? kSliceOne : 0), kStreamBytes<DT>), allowed[held]);
   if (e != cudaSuccess) return e;
   return launch_clusters(kernel, a, n, smem, stream);
 }
