@@ -16,9 +16,9 @@
 // Nothing is sorted but short lists. Top-k: every thread knows the largest logit of
 // its share; the (k / CTAs)-th largest of a CTA's 512 such values is a bound that at
 // least k logits reach, and hardly more, so the few logits past it are gathered and
-// sorted. Top-p alone: logits are counted in 1024 bins linear in x over the 32 T below
-// the maximum, where all the weight is; the bin where the weight crosses p of it is
-// gathered and sorted, and the weight above it summed. Where such a list would not
+// sorted. Top-p alone: logits are counted in 1024 bins linear in x over the part below the
+// maximum where the prefix can end; the two bins around the place where the weight crosses
+// p of it are gathered and sorted, and the weight above them summed. Where such a list would not
 // hold the candidates (very large k, very many equal logits) the threshold is found by
 // counting alone, over the ordered bit patterns inside the crossing bin until it holds
 // one value. Counts are integers and sums run in a fixed order, so a call repeats bit
