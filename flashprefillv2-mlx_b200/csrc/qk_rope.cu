@@ -271,8 +271,10 @@ __global__ void __launch_bounds__(256, (kCtas<DT, AHEAD>)) qk_rope_vec_kernel(co
       issue(h + AHEAD * apart, fill);
       fill = slot;
       asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD) : "memory");
-      mine[0].load(ring + slot * 2 * 256 * BYTES + threadIdx.x * BYTES);
-      mine[1].load(ring + (slot * 2 + 1) * 256 * BYTES + threadIdx.x * BYTES);
+      if (live) {   // the other lanes' values stay 0, for the sum of squares
+        mine[0].load(ring + slot * 2 * 256 * BYTES + threadIdx.x * BYTES);
+        mine[1].load(ring + (slot * 2 + 1) * 256 * BYTES + threadIdx.x * BYTES);
+      }
       slot = slot == AHEAD ? 0 : slot + 1;
     }
     float2 y[2 * H];

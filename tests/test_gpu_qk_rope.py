@@ -149,3 +149,20 @@ def test_side_stream_and_mixed_weight_type():
         gq, _ = fpv2.qk_norm_rope(q, k, pos, table, q_weight=qw.float())
     torch.cuda.current_stream().wait_stream(side)
     assert close(gq, want, formula(q, qw.float(), table, pos, 1e-6, False)[1])
+
+
+@pytest.mark.parametrize("dim,rot", [(96, 64), (80, 40), (80, 80), (56, 16), (160, 32)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_heads_narrower_than_their_lanes_after_infinite_ones(dim, rot, dtype):
+    """Nothing of an earlier call's infinities, left in on-chip memory, gets into the norm."""
+    full = torch.full((3000, 24, 256), float("inf"), dtype=dtype, device=DEV)
+    table = fpv2.rope_table(500, 64, device=DEV)
+    pos = torch.zeros(3000, dtype=torch.int32, device=DEV)
+    fpv2.qk_norm_rope(full[:, :20], full[:, 20:], pos, table)
+    q, k, _, pos, qw, kw = inputs(3000, 20, 4, dim, dtype, seed=dim)
+    table = fpv2.rope_table(500, rot, device=DEV)
+    for interleaved in (False, True):
+        fpv2.qk_norm_rope(full[:, :20], full[:, 20:], torch.zeros_like(pos), table)
+        gq, gk = fpv2.qk_norm_rope(q, k, pos, table, q_weight=qw, k_weight=kw, eps=1e-5, interleaved=interleaved)
+        assert close(gq, *formula(q, qw, table, pos, 1e-5, interleaved))
+        assert close(gk, *formula(k, kw, table, pos, 1e-5, interleaved))
