@@ -124,12 +124,12 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
 }
 
 // Stream units a part. Not fewer than balances what a tile adds to the first kernel (about
-// 1000 cycles) with what a piece adds to the second (about 11: eight warps, ten in flight
-// each): the square root of total / 90. It matters with few KV heads, where one wave of
-// warps is many parts (1 x 20000 keys of one KV head of 64: 17.9 us in 1184 parts, 14.1 us in
-// 209).
+// 1000 cycles) with what a piece adds to the second (about 5: eight warps, 24 in flight each):
+// the square root of total / 200. It matters with few KV heads, where one wave of warps is
+// many parts (6 rows on one KV head of 128: 60000 keys 15.8 us, 64 sequences of 60 to 4000
+// 21.4 us; by total / 90 17.3 and 23.3, by total / 40 19.4 and 27.3).
 __device__ __forceinline__ int64_t part_tiles(int64_t total, int parts) {
-  return max(quotient(total + parts - 1, parts), (int64_t)sqrtf((float)total * (1.f / 90.f)));
+  return max(quotient(total + parts - 1, parts), (int64_t)sqrtf((float)total * (1.f / 200.f)));
 }
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
