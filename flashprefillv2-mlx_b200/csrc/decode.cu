@@ -343,6 +343,8 @@ __global__ void __maxnreg__((kRegs<D, NB>)) decode_kernel(const DecodeArgs a, in
     if (f.at < end) f.next(a, end);
     if (f.at < end) f.fetch(a, lane, whole);
   };
+  bool careful = false;   // a segment is taken a second time, for its values' infinities
+again:
   {
     Feed<TK> early[ST - 1];   // their table entries are loaded side by side
 #pragma unroll
@@ -482,9 +484,10 @@ __global__ void __maxnreg__((kRegs<D, NB>)) decode_kernel(const DecodeArgs a, in
         }
     // With several new tokens a masked key of this tile may be another row's
     // visible one, and 0 * (its infinity or NaN) would spoil this row: such a tile
-    // is added element by element, masked keys left out.
+    // is added element by element, masked keys left out. So is an infinity that is seen,
+    // as a weight's two parts may meet it with opposite signs, or one of them be 0.
     bool odd = false;
-    if (!open && a.T > 1) {
+    if ((!open && a.T > 1) || careful) {
       constexpr uint32_t EX = DT == DT_BF16 ? 0x7F80u : 0x7C00u;
       for (int id = lane; id < TK * CH; id += 32) {
         const uint4 u = *reinterpret_cast<const uint4*>(vtile + (id / CH) * PITCH + (id % CH) * 16);
@@ -549,11 +552,36 @@ __global__ void __maxnreg__((kRegs<D, NB>)) decode_kernel(const DecodeArgs a, in
           }
       }
     }
-    const int was_b = w.b;
+    const int was_b = w.b, was_t = w.t;
+    const int64_t was_at = w.at;
     const bool whole_seq = seg0 == 0 && w.t + 1 == s.tiles;
     w.next(a, end);
     if (w.b != was_b || w.at >= end) {
-      // the segment ends: its sums over the lanes' keys, then out or to the workspace
+      // the segment ends
+      if (!careful) {
+        // Looking for infinities tile by tile would cost every call; a sum that came out as no
+        // number says that there are some, and the segment is taken again with the look.
+        float all = 0.f;
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int k = 0; k < KS; ++k) all += (o[n][k][0] + o[n][k][1]) + (o[n][k][2] + o[n][k][3]);
+        if (__any_sync(0xffffffffu, all != all)) {
+          careful = true;
+          cp_wait<0>();
+          __syncwarp();
+          f.b = was_b;
+          f.s = seq_of<TK>(a, was_b);
+          f.t = seg0;
+          f.at = was_at - (was_t - seg0);
+          f.fetch(a, lane, whole);
+          w = f;
+          fill = 0;
+          goto again;
+        }
+      }
+      careful = false;
+      // its sums over the lanes' keys, then out or to the workspace
       const bool done = whole_seq;
       const int64_t piece = ((int64_t)part * 2 + (started ? 0 : 1)) * cols + col;
       float2* ml = reinterpret_cast<float2*>(a.workspace) + piece * (8 * NB);
