@@ -350,7 +350,8 @@ struct RowState {
 
 __device__ __forceinline__ RowState row_state(float heat, float top_p, float min_p) {
   RowState row;
-  row.heat = heat > 0.f ? fmaxf(heat, 1e-30f) : 1.f;   // its reciprocal stays finite
+  // its reciprocal stays finite and, if subnormal, above 0: an infinite one counts as the largest
+  row.heat = heat > 0.f ? fminf(fmaxf(heat, 1e-30f), kFloatMax) : 1.f;
   row.inv_heat = 1.f / row.heat;
   row.to_log2 = row.inv_heat * kLog2e;
   row.scale = (float)kBins / kSpan * row.inv_heat;
@@ -588,7 +589,7 @@ __device__ Found search(cg::cluster_group& cl, Shared& sh, const Slice<DT, HELD>
   }
   unsigned c = gather_bin(cl, sh);
   double mass = (double)c;
-  if (WEIGHT) mass *= (double)ex2(-((float)tid + (tid == 0 ? 0.f : 0.5f)) / (row.scale * 0.5f) * row.to_log2);
+  if (WEIGHT) mass *= (double)ex2(-((float)tid + (tid == 0 ? 0.f : 0.5f)) * (kSpan / (float)kThreads * kLog2e));
   double before = block_before(sh, mass);
   if (tid == 0) sh.found_bin = kThreads - 1;
   __syncthreads();
@@ -1127,7 +1128,7 @@ __device__ __forceinline__ void stream_row(const SampleArgs& a, cg::cluster_grou
   };
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) issue(tid - lane + i * kThreads, i);
-  const float slack = 8.f / row.to_log2;
+  const float slack = fminf(8.f / row.to_log2, kFloatMax);   // finite: added to a reference of -inf
   float ref = -INFINITY, base = 0.f, most = -INFINITY, sum = 0.f;   // base: ref, or 0 for -inf
   float best = -INFINITY, second = -INFINITY;
   int best_j = 0, least = 0x7F800000, stage = 0;

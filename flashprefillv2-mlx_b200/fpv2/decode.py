@@ -326,10 +326,11 @@ def sample_tokens(
     those whose weight reaches ``top_p`` of theirs; 1 or more: all), then ``min_p``
     (``w >= min_p``); the first token always stays. The result, int64 ``[rows]``, is the
     argmax of ``z - log(noise)`` over what is left: a draw with probabilities
-    proportional to ``w``. ``T <= 0`` takes the lowest index of the maximum. NaN logits
-    count as -inf; a row without a logit above -inf gives -1. With
-    ``return_logprobs`` also float32 ``[rows]``: the token's log-probability under
-    ``softmax(x / T)`` over the whole row (``T = 1`` where ``T <= 0``).
+    proportional to ``w``. ``T <= 0`` takes the lowest index of the maximum; an infinite
+    ``T`` counts as float32's largest number. NaN logits count as -inf; a row without a
+    logit above -inf gives -1. With ``return_logprobs`` also float32 ``[rows]``: the
+    token's log-probability under ``softmax(x / T)`` over the whole row (``T = 1`` where
+    ``T <= 0``).
     """
     if logits.ndim != 2 or logits.shape != noise.shape:
         raise ValueError("logits and noise must have the same shape [rows, vocab]")

@@ -362,8 +362,8 @@ FPV2_API int64_t fpv2_decode_workspace_bytes(int32_t new_tokens, int32_t q_heads
  * ascending): top_k > 0: the first top_k stay; top_p < 1: of those, the shortest prefix
  * whose weight reaches top_p times their weight; min_p > 0: of those, w >= min_p; the
  * first token always stays. tokens[r] = argmax of z - log(noise), ties to the lowest
- * index. T <= 0: the lowest index of the maximum. A row without a logit above -inf
- * gives -1. logprobs: log of the token's share of sum exp(x / T) over the whole row,
+ * index. T <= 0: the lowest index of the maximum; an infinite T counts as the largest
+ * float. A row without a logit above -inf gives -1. logprobs: log of the token's share of sum exp(x / T) over the whole row,
  * before the filters (T = 1 where T <= 0).
  */
 typedef struct {
