@@ -563,6 +563,12 @@ __device__ unsigned gather_bin(cg::cluster_group& cl, Shared& sh) {
 // `target` (a count, or a weight). On return the crossing value is `key` with `count`
 // logits equal to it and `above` of the target used up by larger ones; or, when not
 // `single`, `key` is a lower bound, and what reaches it is just what is needed.
+//
+// Logits are counted in bins, first linear in x, then over the bit patterns of the bin that the
+// target falls into, until a bin is one value. Until then counts only say about where a weight
+// is reached: a bin is off by as much as the weights in it differ (30 of 8000 tokens, where
+// it is half a power of two wide, at zero). So the weights above and in three bins there are
+// added up, and the three are moved on until the target lies in them.
 struct Found {
   uint32_t key;
   unsigned count;
@@ -575,130 +581,41 @@ __device__ Found search(cg::cluster_group& cl, Shared& sh, const Slice<DT, HELD>
                         double target, const Cut& within) {
   constexpr int VE = Slice<DT, HELD>::VE;
   const int tid = threadIdx.x;
-  // linear bins
-  for (int j = tid; j < sl.chunks; j += kThreads) {
-    float x[VE];
-    sl.get(j, x);
-#pragma unroll
-    for (int i = 0; i < VE; ++i) {
-      if (x[i] == -INFINITY || x[i] < within.x) continue;
-      const int b = row.coarse(x[i]);
-      // the last bin's weight is nothing next to the row's, and its count is what is left
-      if (!WEIGHT || b < kThreads - 1) atomicAdd(&sh.hist[b], 1u);
-    }
-  }
-  unsigned c = gather_bin(cl, sh);
-  double mass = (double)c;
-  if (WEIGHT) mass *= (double)ex2(-((float)tid + (tid == 0 ? 0.f : 0.5f)) * (kSpan / (float)kThreads * kLog2e));
-  double before = block_before(sh, mass);
-  if (tid == 0) sh.found_bin = kThreads - 1;
-  __syncthreads();
-  if (before + mass >= target) atomicMin(&sh.found_bin, (unsigned)tid);
-  __syncthreads();
-  int bin = (int)sh.found_bin;
-  double above;
-  unsigned count;
-  if (!WEIGHT) {
-    if (tid == bin) {
-      sh.found_above = before;
-      sh.found_count = c;
-    }
-    __syncthreads();
-    above = sh.found_above;
-    count = sh.found_count;
-  } else {
-    // The bins' weights were estimates: sum the weights above and in three bins around.
-    int moved = 0;
-    while (true) {
-      bin = min(max(bin, 1), kThreads - 2);
-      float s[4] = {0.f, 0.f, 0.f, 0.f};
-      for (int j = tid; j < sl.chunks; j += kThreads) {
-        float x[VE];
-        sl.get(j, x);
-        const int64_t at = sl.index(j);
-#pragma unroll
-        for (int i = 0; i < VE; ++i) {
-          if (x[i] == -INFINITY || !within.keeps(x[i], (int)at + i)) continue;
-          const int b = row.coarse(x[i]);
-          if (b > bin + 1) continue;
-          const float w = row.weight(x[i]);
-          s[0] += b < bin - 1 ? w : 0.f;
-          s[1] += b == bin - 1 ? w : 0.f;
-          s[2] += b == bin ? w : 0.f;
-          s[3] += b == bin + 1 ? w : 0.f;
-        }
-      }
-      double v[4];
-      cluster_sum(cl, sh, s, v);
-      if (v[0] >= target && bin > 1 && moved <= 0) {
-        bin -= 3;
-        moved = -1;
-        continue;
-      }
-      if (v[0] + v[1] + v[2] + v[3] < target && bin < kThreads - 2 && moved >= 0) {
-        bin += 3;
-        moved = 1;
-        continue;
-      }
-      above = v[0];
-      bin -= 1;
-      if (above + v[1] < target) {
-        above += v[1];
-        ++bin;
-        if (above + v[2] < target) {
-          above += v[2];
-          ++bin;
-        }
-      }
-      break;
-    }
-    count = 0xffffffffu;   // not known: the levels below count
-  }
-  // the keys of the bin: bin() falls as the key grows
-  uint32_t lo = kLowest, hi = order(row.top);
-  if (bin < kThreads - 1) {   // smallest key whose bin is <= bin
-    uint32_t a = kLowest, b = hi;
-    while (a < b) {
-      const uint32_t mid = a + (b - a) / 2;
-      if (row.coarse(unorder(mid)) <= bin) b = mid; else a = mid + 1;
-    }
-    lo = a;
-  }
-  if (bin > 0) {           // largest key whose bin is >= bin
-    uint32_t a = lo, b = hi;
-    while (a < b) {
-      const uint32_t mid = a + (b - a + 1) / 2;
-      if (row.coarse(unorder(mid)) >= bin) a = mid; else b = mid - 1;
-    }
-    hi = a;
-  }
-  if (within.x > -INFINITY && lo < order(within.x)) lo = order(within.x);
-  if (hi < lo) return {lo, 0, above, false};   // the target is just past all there is
-  while (true) {
-    if (!WEIGHT && above + (double)count <= target) return {lo, count, above, false};
-    if (count == 1) return {lo, 1, above, false};
-    if (lo >= hi && count != 0xffffffffu) return {lo, count, above, true};
-    const uint32_t width = hi - lo;   // keys less one
-    const int bits = 32 - __clz(width | 1), shift = bits > kKeyBits ? bits - kKeyBits : 0;
+  const uint32_t least = order(fmaxf(within.x, -kFloatMax));
+  uint32_t lo = least, hi = order(row.top);
+  double above = 0;
+  unsigned count = 0xffffffffu;   // not known
+  bool linear = true;
+  int shift = 0;
+  // calls each(logit, its bin) for those in the range
+  auto for_bins = [&](auto each) {
     for (int j = tid; j < sl.chunks; j += kThreads) {
       float x[VE];
       sl.get(j, x);
 #pragma unroll
       for (int i = 0; i < VE; ++i) {
         const uint32_t k = order(x[i]);
-        if (k >= lo && k <= hi) atomicAdd(&sh.hist[(hi - k) >> shift], 1u);
+        if (k >= lo && k <= hi) each(x[i], linear ? row.coarse(x[i]) : (int)((hi - k) >> shift));
       }
     }
-    c = gather_bin(cl, sh);
-    mass = (double)c;
-    const uint32_t off = (uint32_t)tid << shift;
-    if (WEIGHT && c != 0) {
-      // a bin of several values weighs as its middle one: it spans under 2^-12 of z
-      const uint32_t span = (1u << shift) - 1;
-      const uint32_t mid = hi - off - min(span / 2, (hi - off - lo) / 2);
-      mass *= (double)row.weight(unorder(mid));
+  };
+  while (true) {
+    if (!linear) {
+      if (!WEIGHT && above + (double)count <= target) return {lo, count, above, false};
+      if (count <= 1) return {lo, count, above, false};   // 0: rounding let the target end with what is above
+      if (lo >= hi && count != 0xffffffffu) return {lo, count, above, true};
+      const int bits = 32 - __clz((hi - lo) | 1);   // keys less one
+      shift = bits > kKeyBits ? bits - kKeyBits : 0;
     }
-    before = block_before(sh, mass) + above;
+    for_bins([&](float, int b) { atomicAdd(&sh.hist[b], 1u); });
+    const unsigned c = gather_bin(cl, sh);
+    const uint32_t span = (1u << shift) - 1, off = (uint32_t)tid << shift;
+    double mass = (double)c;
+    if (WEIGHT && c != 0) {   // as its middle
+      mass *= linear ? (double)ex2(-((float)tid + (tid == 0 ? 0.f : 0.5f)) * (kSpan / (float)kThreads * kLog2e))
+                     : (double)row.weight(unorder(hi - off - min(span / 2, (hi - off - lo) / 2)));
+    }
+    const double before = block_before(sh, mass) + above;
     __syncthreads();
     if (tid == 0) sh.found_bin = 0xffffffffu;
     __syncthreads();
@@ -711,17 +628,75 @@ __device__ Found search(cg::cluster_group& cl, Shared& sh, const Slice<DT, HELD>
       if (c != 0) atomicMax(&sh.found_bin, (unsigned)tid);
       __syncthreads();
     }
-    const unsigned at = sh.found_bin;
-    if (tid == (int)at) {
-      sh.found_above = before;
-      sh.found_count = c;
+    int bin = (int)sh.found_bin;
+    if (tid == bin) sh.found_above = before;
+    if (WEIGHT && (linear || shift > 0)) {
+      int moved = 0;
+      while (true) {
+        bin = min(max(bin, 1), kThreads - 2);
+        float s[4] = {0.f, 0.f, 0.f, 0.f};   // above, and in the three
+        for_bins([&](float x, int b) {
+          if (b > bin + 1) return;
+          const float w = row.weight(x);
+          s[0] += b < bin - 1 ? w : 0.f;
+          s[1] += b == bin - 1 ? w : 0.f;
+          s[2] += b == bin ? w : 0.f;
+          s[3] += b == bin + 1 ? w : 0.f;
+        });
+        double v[4];
+        cluster_sum(cl, sh, s, v);
+        // a step that would turn back has met the crossing
+        if (above + v[0] >= target && bin > 1 && moved <= 0) {
+          bin -= 3;
+          moved = -1;
+          continue;
+        }
+        if (above + v[0] + v[1] + v[2] + v[3] < target && bin < kThreads - 2 && moved >= 0) {
+          bin += 3;
+          moved = 1;
+          continue;
+        }
+        above += v[0];
+        --bin;
+        if (above + v[1] < target) {
+          above += v[1];
+          ++bin;
+          if (above + v[2] < target) {
+            above += v[2];
+            ++bin;
+          }
+        }
+        break;
+      }
+      if (tid == bin) sh.found_above = above;
     }
+    if (tid == bin) sh.found_count = c;
     __syncthreads();
     above = sh.found_above;
     count = sh.found_count;
-    hi = hi - (at << shift);
-    const uint32_t span = (1u << shift) - 1;
-    if (hi - lo > span) lo = hi - span;
+    if (linear) {
+      // the keys of the bin: coarse() falls as the key grows
+      linear = false;
+      if (bin < kThreads - 1) {   // smallest key whose bin is <= bin
+        uint32_t a = kLowest, b = hi;
+        while (a < b) {
+          const uint32_t mid = a + (b - a) / 2;
+          if (row.coarse(unorder(mid)) <= bin) b = mid; else a = mid + 1;
+        }
+        lo = max(a, least);
+      }
+      if (bin > 0) {           // largest key whose bin is >= bin
+        uint32_t a = lo, b = hi;
+        while (a < b) {
+          const uint32_t mid = a + (b - a + 1) / 2;
+          if (row.coarse(unorder(mid)) >= bin) a = mid; else b = mid - 1;
+        }
+        hi = a;
+      }
+    } else {
+      hi -= (uint32_t)bin << shift;
+      if (hi - lo > span) lo = hi - span;
+    }
     __syncthreads();
   }
 }
@@ -1484,16 +1459,19 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
         // the weight of what is left, by counting
         cl.sync();
         sh.hist[tid] = sh.hist[tid + kThreads] = 0;
-        float s[1] = {0.f};
-        for (int j = tid; j < sl.chunks; j += kThreads) {
-          float x[VE];
-          sl.get(j, x);
+        __syncthreads();
+        double left[1] = {whole};
+        if (use_k) {
+          float s[1] = {0.f};
+          for (int j = tid; j < sl.chunks; j += kThreads) {
+            float x[VE];
+            sl.get(j, x);
 #pragma unroll
-          for (int i = 0; i < VE; ++i)
-            if (cut.keeps(x[i], (int)sl.index(j) + i)) s[0] += row.weight(x[i]);
+            for (int i = 0; i < VE; ++i)
+              if (cut.keeps(x[i], (int)sl.index(j) + i)) s[0] += row.weight(x[i]);
+          }
+          cluster_sum(cl, sh, s, left);
         }
-        double left[1];
-        cluster_sum(cl, sh, s, left);
         const double target = (double)row.top_p * left[0];
         const Found f = search<DT, HELD, true>(cl, sh, sl, row, target, cut);
         const float x = fmaxf(unorder(f.key), cut.x);

@@ -1,5 +1,7 @@
-"""``sample_tokens`` at the largest temperatures: the comparison and its tolerances are
-``test_gpu_sample.check``'s.
+"""``sample_tokens`` at the ends of the temperatures' range and among thousands of ties.
+
+The comparison and its tolerances are ``test_gpu_sample.check``'s. A row's noise is small at
+one token alone, so the row answers whether that token is kept.
 """
 
 from __future__ import annotations
@@ -16,6 +18,25 @@ pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda", 0)
 INF = math.inf
 MOST = torch.finfo(torch.float32).max
+
+
+def probed(values, ranks, seed):
+    """Rows of the same shuffled logits; row r's noise singles out the token of rank ranks[r]."""
+    gen = torch.Generator().manual_seed(seed)
+    x = torch.cat([torch.full((n,), v) for v, n in values])
+    x = x[torch.randperm(len(x), generator=gen)]
+    order = torch.sort(x.double(), descending=True, stable=True).indices
+    noise = torch.empty(len(ranks), len(x)).exponential_(generator=gen).clamp_min_(0.5)
+    noise[torch.arange(len(ranks)), order[torch.tensor(ranks)]] = 1e-20
+    return x.expand(len(ranks), -1).contiguous(), noise.to(DEV)
+
+
+def kept(values, p, heat, k):
+    """How many tokens the nucleus of the first k holds, float64."""
+    x = torch.cat([torch.full((n,), v) for v, n in values]).double()
+    x = x.sort(descending=True).values[:k or None]
+    w = ((x - x[0]) / heat).exp()
+    return int((torch.cumsum(w, 0) - w < p * w.sum()).sum())
 
 
 @pytest.mark.parametrize("rows,vocab", [(6, 9001), (6, 151937)])
@@ -49,3 +70,27 @@ def test_filters_at_the_largest_temperatures(dtype, settings, heat):
     check(logits, noise, temperature=heat, **settings)
     tokens = fpv2.sample_tokens(logits, noise, temperature=MOST, **settings)
     assert torch.equal(fpv2.sample_tokens(logits, noise, temperature=INF, **settings), tokens)
+
+
+@pytest.mark.parametrize("values,heat,p,k", [
+    ([(0.05, 1), (0.035, 4000), (-0.004, 4000)], 1.0, 0.52, 0),     # both sides of zero
+    ([(0.04, 3000), (0.03125, 3000), (0.015625, 3000)], 1.0, 0.5, 0),
+    ([(0.04, 3000), (0.0, 3000), (-0.03, 3000)], 1.0, 0.9, 0),
+    ([(3.0, 2), (0.003, 5000), (-0.002, 5000), (-1e-5, 3000)], 0.9, 0.8, 0),
+    ([(0.05, 1), (0.035, 4000), (-0.004, 4000)], 1.0, 0.55, 7500),  # of the first k
+    ([(0.05, 1), (0.035, 4000), (-0.004, 4000)], 1.0, 0.9999, 7500),
+    ([(1e-3 * (50 - i), 211) for i in range(100)], 1.0, 0.63, 0),
+    ([(1e-3 * (50 - i), 211) for i in range(100)], 1.0, 0.63, 20001),
+    ([(0.25 * (4 - i), 4500) for i in range(9)], 0.7, 0.6, 0),
+    ([(0.0, 9000)], 1.0, 0.37, 0),
+])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("more_rows", [False, True])   # few CTAs a row
+def test_the_nucleus_of_thousands_of_ties(values, heat, p, k, dtype, more_rows):
+    if dtype == torch.float16:
+        values = [(float(torch.tensor(v).half()), n) for v, n in values]
+    count = kept(values, p, heat, k)
+    total = sum(n for _, n in values)
+    ranks = [min(max(count + d, 0), total - 1) for d in (-300, -40, -9, -3, -2, -1, 0, 1, 2, 8, 39, 299)]
+    logits, noise = probed(values, ranks * (12 if more_rows else 1), seed=count)
+    check(logits.to(dtype).to(DEV), noise, temperature=heat, top_p=p, top_k=k)
