@@ -308,7 +308,10 @@ __global__ void __maxnreg__((kRegs<D, NB>)) decode_kernel(const DecodeArgs a, in
       const uint32_t dst = ring + fill * kStageBytes<D> + ldst;
       fill = fill + 1 == ST ? 0 : fill + 1;
       const int key0 = f.key0();
-      const int page = clamp_entry(f.page, 0, a.num_pages - 1, a.status);
+      // a page of this lane's own row may hold no key that any query sees; its entry is not reported
+      const int mine = key0 + lane % TK;
+      const bool used = whole || (mine < f.s.len && (mine >= f.s.low || mine < a.sinks));
+      const int page = clamp_entry(f.page, 0, a.num_pages - 1, used ? a.status : nullptr);
       const int64_t ko = page * a.k_sp + f.in_page * a.k_sr, vo = page * a.v_sp + f.in_page * a.v_sr;
       const bool all = key0 + TK <= f.s.len && (key0 >= f.s.low || key0 + TK <= a.sinks);
       if (whole && all) {
