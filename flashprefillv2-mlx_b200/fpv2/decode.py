@@ -5,7 +5,8 @@ reference leaves it to its model library).
 the page pools that ``pool_pages`` / ``sparse_attention_paged`` prefill from and
 ``decode_attention`` reads; ``decode_attention`` attends the newest tokens of every
 sequence over them; ``sample_tokens`` picks the next tokens. The kernels have no
-backward: inputs that require grad are refused while grad mode is on.
+derivatives: inputs that require grad are refused while grad mode is on, and those with
+a forward-mode tangent always.
 """
 
 from __future__ import annotations
@@ -14,6 +15,7 @@ import functools
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from fpv2 import _lib
 
@@ -31,6 +33,15 @@ _pack_sample = struct.Struct("@5q 2q 1q1d 2q 1q1d 1q1d 2q").pack
 
 def _refuse_grad(what: str) -> None:
     raise ValueError(f"{what} has no backward; call it under torch.no_grad()")
+
+
+def _refuse_tangents(what: str, *tensors: object) -> None:
+    """Outside a forward-mode level (-1) no tensor has a tangent, and nothing is looked at."""
+    if getattr(forward_ad, "_current_level", 0) < 0:
+        return
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f"{what} has no forward-mode derivative; pass tensors without tangents")
 
 
 def _call(fn, device: int, params: bytes) -> None:
@@ -151,6 +162,7 @@ def qk_norm_rope(
             or k_weight is not None and k_weight.requires_grad
             or paged and (v.requires_grad or k_cache.requires_grad or v_cache.requires_grad)):
         _refuse_grad("qk_norm_rope")
+    _refuse_tangents("qk_norm_rope", q, k, table, q_weight, k_weight, v, k_cache, v_cache)
     device = q.get_device()
     if device < 0 or k.get_device() != device or positions.get_device() != device or table.get_device() != device \
             or q_weight is not None and q_weight.get_device() != device \
@@ -269,6 +281,7 @@ def decode_attention(
         raise ValueError("window and sinks must be non-negative 32-bit integers")
     if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         _refuse_grad("decode_attention")
+    _refuse_tangents("decode_attention", q, k_cache, v_cache)
     device = q.get_device()
     if device < 0 or k_cache.get_device() != device or v_cache.get_device() != device \
             or block_tables.get_device() != device or lengths.get_device() != device:
@@ -346,8 +359,9 @@ def sample_tokens(
     least, least_all = _setting(min_p, "min_p", torch.float32, rows, 0.0)
     if not -_INT32_MAX <= k_all <= _INT32_MAX:
         raise ValueError("top_k must be a 32-bit integer")
-    if logits.requires_grad and torch.is_grad_enabled():
+    if torch.is_grad_enabled() and (logits.requires_grad or heat is not None and heat.requires_grad):
         _refuse_grad("sample_tokens")
+    _refuse_tangents("sample_tokens", logits, heat)
     device = logits.get_device()
     if device < 0 or noise.get_device() != device or heat is not None and heat.get_device() != device \
             or k is not None and k.get_device() != device or p is not None and p.get_device() != device \
