@@ -1,6 +1,7 @@
 // C ABI of the decode step (declared in include/fpv2_b200.h): argument checks
 // and launches, as in capi.cu.
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <string>
 
@@ -43,7 +44,7 @@ int fpv2_qk_norm_rope(const fpv2_qk_norm_rope_params* p, void* stream) {
   if (p->rotary_dim <= 0 || p->rotary_dim % 2 || p->rotary_dim > p->head_dim)
     return invalid("rotary_dim must be even and in [2, head_dim]");
   if (p->table_positions <= 0) return invalid("the rotation table is empty");
-  if (!(p->eps >= 0.0) || std::isinf(p->eps)) return invalid("eps must be finite and non-negative");
+  if (!(p->eps >= 0.0 && p->eps <= FLT_MAX)) return invalid("eps must be non-negative and finite in float32");
   const bool paged = p->k_cache != nullptr || p->v_cache != nullptr;
   if (paged && (!p->k_cache || !p->v_cache || !p->slots || p->num_pages <= 0 || p->page_size <= 0 ||
                 p->page_size > kMaxSize))
@@ -70,7 +71,7 @@ int fpv2_qk_norm_rope(const fpv2_qk_norm_rope_params* p, void* stream) {
   a.q_weight = p->q_weight;
   a.k_weight = p->k_weight;
   a.weight_dt = (int)p->weight_dtype;
-  a.eps = (float)p->eps;
+  a.eps = p->eps > 0.0 ? std::max((float)p->eps, FLT_TRUE_MIN) : 0.f;   // a row of zeros stays one of zeros
   a.q_out = p->q_out;
   a.qo_st = p->q_out_token_stride;
   a.qo_sh = p->q_out_head_stride;
@@ -126,7 +127,7 @@ int fpv2_decode_attention(const fpv2_decode_attention_params* p, void* stream) {
   if (p->table_width * p->page_size > 0x7fffffff - 64) return invalid("sequences must be shorter than 2^31 keys");
   if (p->window < 0 || p->sinks < 0 || p->window > kMaxSize || p->sinks > kMaxSize)
     return invalid("window and sinks must be non-negative 32-bit integers");
-  if (!std::isfinite(p->scale)) return invalid("scale must be finite");
+  if (!(std::fabs(p->scale) * kLog2e <= FLT_MAX)) return invalid("scale must be finite, as its product with log2(e) in float32");
   if (p->batch == 0) return FPV2_OK;
   if (!p->q || !p->k_pages || !p->v_pages || !p->block_tables || !p->lengths || !p->out || !p->workspace)
     return invalid("null tensor pointer");
