@@ -74,6 +74,7 @@ class PagedModel:
         order = torch.randperm(requests * pages, device=device, dtype=torch.int32)
         self.tables = order.view(requests, pages)
         self.lengths = torch.zeros(requests, dtype=torch.int32, device=device)
+        self.held = [0] * requests   # the same on the host: a position past the pools is refused there
 
     def _slots(self, requests: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
         page = self.shape.page_size
@@ -99,6 +100,10 @@ class PagedModel:
     def prefill(self, request: int, ids: torch.Tensor, chunk: int = 2048) -> torch.Tensor:
         """Logits ``[vocab]`` after the prompt ``ids``, prefilled in chunks."""
         s, cfg = self.shape, self.config
+        if not 0 <= request < len(self.held):
+            raise ValueError(f"request must be in [0, {len(self.held)})")
+        if not 0 < ids.numel() <= s.max_tokens:
+            raise ValueError(f"a prompt must have 1 to max_tokens = {s.max_tokens} tokens")
         for offset in range(0, ids.numel(), chunk):
             n = min(chunk, ids.numel() - offset)
             length = offset + n
@@ -124,13 +129,18 @@ class PagedModel:
             x = self.weights["embed"][ids[offset:length]]
             for layer in range(s.layers):
                 x = self._block(x, layer, positions, slots, attend, heads_first=True)
-        self.lengths[request] = ids.numel()
+        self.lengths[request] = self.held[request] = ids.numel()
         return self._logits(x[-1])
 
     @torch.no_grad()
     def decode(self, ids: torch.Tensor) -> torch.Tensor:
         """Logits ``[requests, vocab]`` after one more token of every request."""
         s = self.shape
+        if len(ids) != len(self.held):
+            raise ValueError("every request needs its token")
+        if max(self.held) >= s.max_tokens:
+            raise ValueError(f"a request would pass max_tokens = {s.max_tokens}")
+        self.held = [n + 1 for n in self.held]
         positions = self.lengths.long()
         slots = self._slots(torch.arange(len(ids), device=ids.device), positions)
         lengths = self.lengths + 1
@@ -148,6 +158,10 @@ class PagedModel:
 def generate(model: PagedModel, prompts: list[torch.Tensor], new_tokens: int, *, temperature: float = 0.8,
              top_k: int = 50, top_p: float = 0.95, seed: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
     """``new_tokens`` tokens for each prompt and their log-probabilities."""
+    if len(prompts) != len(model.held):
+        raise ValueError(f"the model holds {len(model.held)} requests")
+    if max(ids.numel() for ids in prompts) + new_tokens - 1 > model.shape.max_tokens:
+        raise ValueError(f"prompt and new tokens would pass max_tokens = {model.shape.max_tokens}")
     logits = torch.stack([model.prefill(r, ids) for r, ids in enumerate(prompts)])
     gen = torch.Generator(device=logits.device).manual_seed(seed)
     noise = torch.empty(logits.shape, device=logits.device)
