@@ -6,10 +6,12 @@
 //   o = sum_j softmax_j(scale q.k_j) v_j,   lse = log sum_j exp(scale q.k_j)
 // A row that sees nothing gets o = 0 and lse = -inf.
 //
-// Every visible K and V row is read once for 4 G T D operations on 4 D bytes, so
-// DRAM bandwidth bounds the call until G * T passes about 100 query rows; the
-// tensor work is small and a few rows wide, so it runs on mma.sync m16n8k16 straight
-// from shared memory, without TMEM round trips.
+// Every visible K and V row takes 4 G T D operations on 4 D bytes, so DRAM bandwidth
+// bounds the call while few rows share a KV head; the tensor work is small and a few
+// rows wide, so it runs on mma.sync m16n8k16 straight from shared memory, without TMEM
+// round trips. A tile is fetched once for each group of up to 16 rows (32 for head_dim 64),
+// by warps of their own, so past that the time grows with the groups (16 sequences of 8000
+// keys, 8 KV heads of 128, 80 us at a copy's rate: up to 8 rows 98 us, 16 106, 32 156, 64 294).
 //
 // Split: the visible keys of all sequences are one stream of TK-key tiles, cut
 // into equal parts whatever the sequences' lengths are. One warp takes one part
@@ -21,10 +23,10 @@
 // kernel, launched early and waiting for the first, joins them in part order, so
 // the result does not depend on timing.
 //
-// Measured (bf16, 32 + 8 heads of 128): 64 sequences of 129 to 16384 keys 175 us, 6.3 TB/s, a
-// copy's rate; one of 65536 keys 53 us, 5.0 TB/s (50 us without the join), of which about 3 us
-// pass before the first keys are asked for and 8 us while the last warps finish; one of 517 keys
-// 7.9 us, latency.
+// Measured (bf16, 32 + 8 heads of 128): 64 sequences of 129 to 16384 keys 177 us for 975 MB
+// (means of three draws), 5.5 TB/s, 0.84 of a copy; one of 65536 keys 54 us, 5.0 TB/s (50 us without
+// the join), of which about 3 us pass before the first keys are asked for and 8 us while the last
+// warps finish; one of 517 keys 8.2 us, latency.
 #include "common.cuh"
 #include "kernels.h"
 
@@ -34,12 +36,13 @@ namespace {
 constexpr int kSms = 148;      // B200; sets the split, so results do not vary with the device
 constexpr float kLn2 = 0.6931471805599453f;
 
-// Keys a tile, ring stages, warps a CTA (about 200 KB of ring). Measured, head_dim 128, one
-// sequence of 65536 keys and a ragged batch of 64: {16, 3, 8} 56.3 and 175 us, {16, 6, 4} 58.5
-// and 170, {16, 5, 5} 56.7 and 189, {16, 2, 12} 62 and 173, {32, 2, 6} 64.6 and 166, {32, 3, 4}
-// 80 and 167. 64 (65536 keys): {32, 3, 8} 57.4, {16, 6, 8} 56.5, {32, 4, 6} 69.7 us, the first with
-// half the steps for compute. 96: {16, 4, 8} 76.5, {16, 3, 11} 82.9, {32, 3, 5} 148 us. 256
-// (16 x 8000 keys): {16, 3, 4} 96.9, {16, 2, 6} 100.3 us.
+// Keys a tile, ring stages, warps a CTA (about 200 KB of ring). Measured when they were chosen,
+// head_dim 128, one sequence of 65536 keys and a ragged batch of 64: {16, 3, 8} 56.3 and 175 us,
+// {16, 6, 4} 58.5 and 170, {16, 5, 5} 56.7 and 189, {16, 2, 12} 62 and 173, {32, 2, 6} 64.6 and 166,
+// {32, 3, 4} 80 and 167. The others by 16 sequences of 8000 keys in pages of 16, 8 KV heads: 64: {32,
+// 3, 8} 57.4 us, {16, 6, 8} 56.5, {32, 4, 6} 69.7, the first with half the steps for compute.
+// 96: {16, 4, 8} 76.5, {16, 3, 11} 82.9, {32, 3, 5} 148. 256 (4 KV heads): {16, 3, 4} 96.9, {16, 2, 6}
+// 100.3.
 template <int D> struct Shape;
 template <> struct Shape<64> { static constexpr int TK = 32, ST = 3, NW = 8; };
 template <> struct Shape<96> { static constexpr int TK = 16, ST = 4, NW = 8; };
@@ -650,8 +653,7 @@ __device__ __forceinline__ float load_if(const float* p, bool read) {
 // pieces each (ROW_CTA), a CTA takes 32 dimensions of a row, a warp an eighth of the
 // pieces.
 // It fits beside the first kernel's CTAs, so it is launched and has its part boundaries
-// when that one ends.
-
+// when that one ends; but for four row blocks of head_dim 64, which fill the registers.
 template <int DT, int D, bool ROW_CTA>
 __global__ void __launch_bounds__(256, 4) decode_join_kernel(const DecodeArgs a, int parts) {
   constexpr int TK = Shape<D>::TK, NV = ROW_CTA ? 1 : D / 32, WARPS = 8, WPR = ROW_CTA ? WARPS : 1;
