@@ -761,7 +761,7 @@ __device__ float min_p_logit(const RowState& row) {
 }
 
 // Top-p over the whole row: cut after the shortest prefix with p of the weight.
-// Returns false (everywhere) when the crossing bin does not fit the list.
+// Returns false (everywhere) when the crossing bin does not fit the list or lies below the others.
 template <int DT, bool HELD>
 __device__ bool nucleus(cg::cluster_group& cl, Shared& sh, const Slice<DT, HELD>& sl, RowState row,
                         unsigned long long* list, float* ahead, double& whole, Cut& cut) {
@@ -858,6 +858,8 @@ __device__ bool nucleus(cg::cluster_group& cl, Shared& sh, const Slice<DT, HELD>
     } else if (total < target && bin < kBins - 3 && moved >= 0) {
       moved = 1;
       bin = min(bin + 2, kBins - 3);
+    } else if (total < target && bin >= kBins - 3) {
+      return false;   // the prefix ends below the bins (millions of tokens past 32 nats, or rounding)
     } else {
       if (least == 0) {   // nothing of the bin is needed
         cut.x = row.top - ((float)bin - 0.5f) / row.scale;

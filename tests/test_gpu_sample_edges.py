@@ -94,3 +94,18 @@ def test_the_nucleus_of_thousands_of_ties(values, heat, p, k, dtype, more_rows):
     ranks = [min(max(count + d, 0), total - 1) for d in (-300, -40, -9, -3, -2, -1, 0, 1, 2, 8, 39, 299)]
     logits, noise = probed(values, ranks * (12 if more_rows else 1), seed=count)
     check(logits.to(dtype).to(DEV), noise, temperature=heat, top_p=p, top_k=k)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_nucleus_that_ends_past_32_nats(dtype):
+    """2^26 tokens of e^-32.25 each weigh 6.6e-7 of the first one, more than 1 - top_p."""
+    vocab, p = 2**26, 1 - 2.0**-24
+    x = torch.full((3, vocab), -32.25, dtype=dtype, device=DEV)
+    x[:, 12345] = 0
+    noise = torch.ones(3, vocab, device=DEV)
+    w = math.exp(-32.25)
+    count = math.ceil((p * (1 + (vocab - 1) * w) - 1) / w)   # of the equal ones that are kept, lowest first
+    for r, rank in enumerate((1_000_000, count - vocab // 100, count + vocab // 100)):
+        noise[r, rank if rank < 12345 else rank + 1] = 1e-30
+    got = fpv2.sample_tokens(x, noise, top_p=p).tolist()
+    assert got == [1_000_001, count - vocab // 100 + 1, 12345]
